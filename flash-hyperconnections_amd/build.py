@@ -42,8 +42,14 @@ KERNEL_SOURCES = [
     "expm_tile.hip",
     "expm_params.hip",
     "hc_mix.hip",
+    "layer_norm.hip",
+    "linear.hip",
+    "linear_product.hip",
+    "grad_clip.hip",
     "fh_capi.cpp",
 ]
+
+EXTENSION_SOURCES = ["register.cpp", "register_block.cpp"]
 
 # -ffp-contract=off: every fused multiply-add in the kernels is written out.
 # The packed-FP32 feature is switched off (no packed FP32 instructions are
@@ -126,13 +132,15 @@ def build_extension(out_dir: Path = PKG, obj_dir: Path = OBJ) -> Path:
         f"-I{INCLUDE}",
     ]
     obj_dir.mkdir(parents=True, exist_ok=True)
-    obj = obj_dir / "register.o"
     cxx = shutil.which("g++") or "g++"
-    _run([cxx, *flags, "-c", str(CSRC / "register.cpp"), "-o", str(obj)])
+    objs = [obj_dir / (Path(src).stem + ".o") for src in EXTENSION_SOURCES]
+    with ThreadPoolExecutor(max_workers=len(objs)) as pool:
+        list(pool.map(lambda so: _run([cxx, *flags, "-c", str(CSRC / so[0]), "-o", str(so[1])]),
+                      zip(EXTENSION_SOURCES, objs)))
     target = out_dir / "_C.so"
     tmp = target.with_suffix(".so.tmp")
     _run([
-        cxx, "-shared", str(obj), "-o", str(tmp),
+        cxx, "-shared", *map(str, objs), "-o", str(tmp),
         f"-L{out_dir}", "-l:" + LIB_NAME,
         f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
         f"-L{ROCM / 'lib'}", "-lamdhip64",

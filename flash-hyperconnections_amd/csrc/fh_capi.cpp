@@ -4,6 +4,7 @@
 // csrc/matrix_exp.cu:13-86 without its FP32/contiguous/padded staging copies:
 // the kernels read the caller's strided storage directly and write only the
 // logical n x n block.
+#include <cmath>
 #include <string>
 
 #include "fh_kernels.h"
@@ -195,6 +196,71 @@ int validate_apply(const float* e, const void* x, const int64_t* xs, const void*
   return FH_OK;
 }
 
+// ---- layer norm, linear, clipping ------------------------------------------------
+
+int launched(hipError_t err) {
+  if (err != hipSuccess) return fail(FH_ERR_LAUNCH, std::string("kernel launch failed: ") + hipGetErrorString(err));
+  g_error.clear();
+  return FH_OK;
+}
+
+// The workspace protocol of calls that need `need` bytes: FH_OK to go on, with
+// `*query` set where only the size was asked for.
+int check_workspace(const char* op, void* workspace, int64_t* bytes, int64_t need, bool* query) {
+  if (bytes == nullptr) return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": null workspace size");
+  *query = workspace == nullptr;
+  if (*query) {
+    *bytes = need;
+    g_error.clear();
+    return FH_OK;
+  }
+  if (*bytes < need || (need > 0 && !aligned(workspace, 16)))
+    return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": the workspace needs " + std::to_string(need) +
+                                             " bytes, 16-byte aligned");
+  return FH_OK;
+}
+
+bool rows_ok(const void* p, int64_t stride, int dtype) { return p != nullptr && stride >= 0 && aligned(p, element_size(dtype)); }
+
+int validate_norm(const void* x, int64_t x_stride, const void* y, int param_dtype, int dtype, int64_t rows,
+                  int64_t cols) {
+  if (!known_dtype(dtype) || (param_dtype != dtype && param_dtype != FH_DTYPE_F32) || rows < 0 ||
+      rows >= (int64_t{1} << 31) || cols < 1 || cols >= (int64_t{1} << 30))
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "layer_norm: expected x [rows, cols] in float32, float16, or bfloat16 with fewer than 2^31 rows and "
+                "1 <= cols < 2^30, and weight and bias of its type or float32");
+  if (rows > 0 && (!rows_ok(x, x_stride, dtype) || !rows_ok(y, 0, dtype)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "layer_norm: null or misaligned pointer, or negative stride");
+  return FH_OK;
+}
+
+int validate_linear(const fh::LinearArgs& a) {
+  constexpr int64_t most = int64_t{1} << 22;
+  if (!known_dtype(a.dtype) || (a.bias_dtype != a.dtype && a.bias_dtype != FH_DTYPE_F32) || a.rows < 0 ||
+      a.rows >= (int64_t{1} << 31) || a.cols < 1 || a.cols >= most || a.outs < 1 || a.outs >= most)
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "linear: expected x [rows, cols] and weight [outs, cols] in float32, float16, or bfloat16 with fewer "
+                "than 2^31 rows and 1 <= cols, outs < 2^22, and a bias of their type or float32");
+  if (a.act < FH_ACT_NONE || a.act > FH_ACT_SILU) return fail(FH_ERR_INVALID_ARGUMENT, "linear: unknown activation");
+  return FH_OK;
+}
+
+int validate_clip(const char* op, int count, const void* const* grads, void* const* out, const int64_t* sizes,
+                  const int* dtypes, double norm_type, const float* norm, int* power) {
+  if (norm_type != 1.0 && norm_type != 2.0 && !(std::isinf(norm_type) && norm_type > 0))
+    return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": norm_type is 1, 2 or infinity");
+  *power = std::isinf(norm_type) ? 0 : static_cast<int>(norm_type);
+  if (count < 0 || norm == nullptr || (count > 0 && (grads == nullptr || sizes == nullptr || dtypes == nullptr)))
+    return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": null list or negative count");
+  for (int i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || !known_dtype(dtypes[i]))
+      return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": expected float32, float16, or bfloat16 arrays");
+    if (sizes[i] > 0 && (!rows_ok(grads[i], 0, dtypes[i]) || (out != nullptr && !rows_ok(out[i], 0, dtypes[i]))))
+      return fail(FH_ERR_INVALID_ARGUMENT, std::string(op) + ": null or misaligned array");
+  }
+  return FH_OK;
+}
+
 }  // namespace
 
 namespace fh {
@@ -342,6 +408,151 @@ int fh_hc_apply_backward(const float* e, const void* x, const int64_t x_strides[
   const hipError_t err = fh::launch_hc_apply(e, x, x_strides, grad, grad_strides, dx, de, dtype, batch, n, cols, stream);
   if (err != hipSuccess) return fail(FH_ERR_LAUNCH, std::string("kernel launch failed: ") + hipGetErrorString(err));
   return FH_OK;
+}
+
+int fh_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias, int param_dtype, double eps,
+                  void* y, float* stats, int dtype, int64_t rows, int64_t cols, hipStream_t stream) {
+  const int rc = validate_norm(x, x_stride, y, param_dtype, dtype, rows, cols);
+  if (rc != FH_OK) return rc;
+  if (rows == 0) return launched(hipSuccess);
+  fh::NormArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.weight = weight;
+  a.bias = bias;
+  a.params_f32 = param_dtype == FH_DTYPE_F32;
+  a.eps = static_cast<float>(eps);
+  a.y = y;
+  a.stats = stats;
+  a.rows = rows;
+  a.cols = cols;
+  return launched(fh::launch_norm(a, dtype, stream));
+}
+
+int fh_layer_norm_backward(const void* x, int64_t x_stride, const void* grad, int64_t grad_stride, const void* weight,
+                           int param_dtype, const float* stats, void* dx, void* dweight, void* dbias, void* workspace,
+                           int64_t* workspace_bytes, int dtype, int64_t rows, int64_t cols, hipStream_t stream) {
+  int rc = validate_norm(x, x_stride, dx, param_dtype, dtype, rows, cols);
+  if (rc != FH_OK) return rc;
+  if (rows == 0) return fail(FH_ERR_INVALID_ARGUMENT, "layer_norm: no rows, whose gradients are zeros of the caller's");
+  if (!rows_ok(grad, grad_stride, dtype) || stats == nullptr)
+    return fail(FH_ERR_INVALID_ARGUMENT, "layer_norm: null or misaligned pointer, or negative stride");
+  const bool params = dweight != nullptr || dbias != nullptr;
+  const int64_t need = params ? fh::norm_blocks(dtype, rows, cols) * 2 * cols * static_cast<int64_t>(sizeof(float)) : 0;
+  bool query = false;
+  rc = check_workspace("layer_norm", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  fh::NormArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.grad = grad;
+  a.grad_stride = grad_stride;
+  a.weight = weight;
+  a.params_f32 = param_dtype == FH_DTYPE_F32;
+  a.y = dx;
+  a.stats = const_cast<float*>(stats);
+  a.partial = params ? static_cast<float*>(workspace) : nullptr;
+  a.rows = rows;
+  a.cols = cols;
+  return launched(fh::launch_norm_backward(a, dweight, dbias, param_dtype, dtype, stream));
+}
+
+int fh_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
+              int bias_dtype, const void* residual, int64_t residual_stride, int activation, void* y, void* saved,
+              void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows, int64_t cols, int64_t outs,
+              hipStream_t stream) {
+  fh::LinearArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.weight = weight;
+  a.w_stride = weight_stride;
+  a.bias = bias;
+  a.bias_dtype = bias_dtype;
+  a.residual = residual;
+  a.r_stride = residual_stride;
+  a.act = activation;
+  a.dtype = dtype;
+  a.saved = saved;
+  a.y = y;
+  a.rows = rows;
+  a.cols = cols;
+  a.outs = outs;
+  int rc = validate_linear(a);
+  if (rc != FH_OK) return rc;
+  int64_t need = 0;
+  bool query = false;
+  if (rows > 0) {
+    if (!rows_ok(x, x_stride, dtype) || !rows_ok(weight, weight_stride, dtype) || !rows_ok(y, 0, dtype) ||
+        (residual != nullptr && !rows_ok(residual, residual_stride, dtype)) ||
+        (bias != nullptr && !aligned(bias, element_size(bias_dtype))))
+      return fail(FH_ERR_INVALID_ARGUMENT, "linear: null or misaligned pointer, or negative stride");
+    (void)fh::launch_linear(a, nullptr, &need, stream);
+  }
+  rc = check_workspace("linear", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(rows > 0 ? fh::launch_linear(a, workspace, nullptr, stream) : hipSuccess);
+}
+
+int fh_linear_backward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* grad,
+                       int64_t grad_stride, const void* saved, int activation, void* dx, void* dweight, void* dbias,
+                       int bias_dtype, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                       int64_t cols, int64_t outs, hipStream_t stream) {
+  fh::LinearArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.weight = weight;
+  a.w_stride = weight_stride;
+  a.grad = grad;
+  a.g_stride = grad_stride;
+  a.bias_dtype = bias_dtype;
+  a.act = activation;
+  a.dtype = dtype;
+  a.saved = const_cast<void*>(saved);
+  a.dx = dx;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  a.rows = rows;
+  a.cols = cols;
+  a.outs = outs;
+  int rc = validate_linear(a);
+  if (rc != FH_OK) return rc;
+  if (rows == 0) return fail(FH_ERR_INVALID_ARGUMENT, "linear: no rows, whose gradients are zeros of the caller's");
+  if ((activation != FH_ACT_NONE) != (saved != nullptr))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear: the backward takes the forward's `saved` with an activation only");
+  if (!rows_ok(grad, grad_stride, dtype) || (dweight != nullptr && !rows_ok(x, x_stride, dtype)) ||
+      (dx != nullptr && !rows_ok(weight, weight_stride, dtype)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear: null or misaligned pointer, or negative stride");
+  int64_t need = 0;
+  bool query = false;
+  (void)fh::launch_linear_backward(a, nullptr, &need, stream);
+  rc = check_workspace("linear", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_linear_backward(a, workspace, nullptr, stream));
+}
+
+int fh_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, double norm_type,
+                 float* norm, void* workspace, int64_t* workspace_bytes, hipStream_t stream) {
+  int power = 0;
+  int rc = validate_clip("grad_norm", count, grads, nullptr, sizes, dtypes, norm_type, norm, &power);
+  if (rc != FH_OK) return rc;
+  const fh::ClipList list{count, grads, nullptr, sizes, dtypes};
+  bool query = false;
+  rc = check_workspace("grad_norm", workspace, workspace_bytes, fh::clip_partials(list) * 8, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_clip(list, power, 0.0, false, norm, static_cast<double*>(workspace), stream));
+}
+
+int fh_clip_gradients(int count, const void* const* grads, void* const* out, const int64_t* sizes, const int* dtypes,
+                      double norm_type, double max_norm, float* norm, void* workspace, int64_t* workspace_bytes,
+                      hipStream_t stream) {
+  int power = 0;
+  int rc = validate_clip("clip_gradients", count, grads, out, sizes, dtypes, norm_type, norm, &power);
+  if (rc != FH_OK) return rc;
+  const fh::ClipList list{count, grads, out, sizes, dtypes};
+  bool query = false;
+  rc = check_workspace("clip_gradients", workspace, workspace_bytes, fh::clip_partials(list) * 8, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_clip(list, power, max_norm, true, norm, static_cast<double*>(workspace), stream));
 }
 
 const char* fh_last_error(void) { return g_error.c_str(); }

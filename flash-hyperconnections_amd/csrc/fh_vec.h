@@ -1,0 +1,118 @@
+// Rows in 16-byte vectors: loads, stores, conversions and wavefront sums shared
+// by the kernels that stream whole rows.
+#pragma once
+
+#include "fh_common.h"
+
+namespace fh {
+
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(typename T::storage));
+
+// Calls f.template operator()<T>() for the element type of `dtype`.
+template <typename F>
+hipError_t with_type(int dtype, F f) {
+  if (dtype == F32::code) return f(F32{});
+  if (dtype == BF16::code) return f(BF16{});
+  return f(F16{});
+}
+
+// Elements c .. c + V - 1 of a row of `cols` (below 2^30), zero past its end.  Rows
+// start at any element: a 16-byte access needs no more than that here.
+template <typename T>
+__device__ __forceinline__ U32x4 load_row(const typename T::storage* row, int c, int cols) {
+  constexpr int V = kVec<T>;
+  U32x4 w{0, 0, 0, 0};
+  if (c + V <= cols) {
+    __builtin_memcpy(&w, row + c, 16);
+  } else if (c < cols) {
+    typename T::storage e[V] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < cols) e[i] = row[c + i];
+    __builtin_memcpy(&w, e, 16);
+  }
+  return w;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(U32x4 w, typename T::storage* row, int c, int cols) {
+  constexpr int V = kVec<T>;
+  if (c + V <= cols) {
+    __builtin_memcpy(row + c, &w, 16);
+  } else if (c < cols) {
+    typename T::storage e[V];
+    __builtin_memcpy(e, &w, 16);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < cols) row[c + i] = e[i];
+  }
+}
+
+// A vector's elements in FP32.
+template <typename T>
+__device__ __forceinline__ void to_floats(U32x4 w, float (&f)[kVec<T>]) {
+  using S = typename T::storage;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) {
+    if constexpr (sizeof(S) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else {
+      f[i] = to_f32<T>(__builtin_bit_cast(S, static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)))));
+    }
+  }
+}
+
+// Two values rounded to nearest even, in one dword (v_cvt_pk_bf16_f32 and its
+// FP16 counterpart; NaN stays NaN).
+template <typename T>
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  if constexpr (T::code == BF16::code) {
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{a, b}), B2));
+  } else {
+    typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (H2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
+  }
+}
+
+// FP32 values rounded to the storage type.
+template <typename T>
+__device__ __forceinline__ U32x4 from_floats(const float (&f)[kVec<T>]) {
+  U32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::code == F32::code) {
+      w[i] = __float_as_uint(f[i]);
+    } else {
+      w[i] = round_pair<T>(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  return w;
+}
+
+// One element of an array whose type is FP32 or T.
+template <typename T>
+__device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) {
+  return f32 ? static_cast<const float*>(p)[i] : to_f32<T>(static_cast<const typename T::storage*>(p)[i]);
+}
+
+// Elements c .. c + V - 1 of such an array of `cols`, `fill` past its end and
+// everywhere where it is null.
+template <typename T>
+__device__ __forceinline__ void load_params(const void* p, bool f32, int c, int cols, float fill,
+                                            float (&f)[kVec<T>]) {
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) f[i] = p != nullptr && c + i < cols ? load_param<T>(p, f32, c + i) : fill;
+}
+
+// Sum over the wavefront's lanes, the same bits in every lane (a butterfly adds
+// the same pairs everywhere).
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+}  // namespace fh

@@ -1,0 +1,275 @@
+// The linear layer around its matrix products:
+//   z = x W^T + b,  y = act(z) + residual;
+//   dz = g act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz.
+//
+// The products take 16-bit operands whose rows are whole 16-byte vectors.  Others
+// are laid out anew first (prepare_kernel): padded rows for odd widths, and for
+// FP32 three bf16 planes a, b, c with x = a + b + c exactly (8 bits each, cut off,
+// so that nothing overflows).  Six of the nine products of planes make an FP32
+// product to about 2^-23; on the bf16 matrix instructions, sixteen times the rate
+// of the FP32 ones, they take less than half the FP32 instructions' time.
+//
+// dz is formed by the same kernel on its way into such a layout, together with the
+// column sums that make db.  It is rounded to the storage type, as operands of
+// 16-bit products have to be; db adds the values before that rounding.
+#include <algorithm>
+
+#include "linear.h"
+
+namespace fh {
+namespace {
+
+struct PrepareArgs {
+  const void* src;   // [rows, cols], rows src_stride elements apart
+  int64_t src_stride;
+  const void* saved; // with an activation: [rows, cols] contiguous
+  int act;
+  uint16_t* out;     // [rows, ld] (FP32: three planes of that), zero past cols; or null
+  int64_t ld;
+  float* partial;    // [gridDim.y, cols] column sums, or null
+  int64_t rows;
+  int cols;
+};
+
+__device__ __forceinline__ uint32_t top_half(float v) { return __float_as_uint(v) & 0xFFFF0000u; }
+
+// The three bf16 planes of a value, as dwords with the bits on top.  An infinity or
+// NaN goes into the last plane, which meets only the other operand's first, beside a
+// one in the first plane: inf x (second or third plane 0) would be NaN, where inf x b
+// is an infinity.
+__device__ __forceinline__ void planes_of(float v, uint32_t (&part)[3]) {
+  if (finite_f32(v)) {
+    part[0] = top_half(v);
+    const float r = v - __uint_as_float(part[0]);
+    part[1] = top_half(r);
+    part[2] = top_half(r - __uint_as_float(part[1]));
+  } else {
+    part[0] = 0x3F800000u | (__float_as_uint(v) & 0x80000000u);
+    part[1] = 0;
+    part[2] = v != v ? 0x7FC00000u : __float_as_uint(v);
+  }
+}
+
+// Four wavefronts, 64 V columns, rows blockIdx.y, + gridDim.y, ....
+template <typename T, bool Sums>
+__global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
+  using S = typename T::storage;
+  using Z = Saved<T>;
+  constexpr int V = kVec<T>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (static_cast<int>(blockIdx.x) * 64 + lane) * V;
+  float sums[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[i] = 0.f;
+  for (int64_t row = blockIdx.y * 4 + wave; row < a.rows; row += gridDim.y * 4) {
+    const U32x4 raw = load_row<T>(static_cast<const S*>(a.src) + row * a.src_stride, c, a.cols);
+    float f[V];
+    to_floats<T>(raw, f);
+    U32x4 rounded = raw;
+    if (a.saved != nullptr) {
+      const auto* z = static_cast<const typename Z::storage*>(a.saved) + row * a.cols;
+      float zf[V];
+      to_floats<Z>(load_row<Z>(z, c, a.cols), zf);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] *= slope(zf[i], a.act);
+      rounded = from_floats<T>(f);
+    }
+    if constexpr (Sums) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[i] += c + i < a.cols ? f[i] : 0.f;
+    }
+    if (a.out != nullptr && c < a.ld) {
+      if constexpr (T::code != F32::code) {
+        *reinterpret_cast<U32x4*>(a.out + row * a.ld + c) = rounded;
+      } else {
+        uint32_t part[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) planes_of(c + i < a.cols ? f[i] : 0.f, part[i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const uint2 w = make_uint2((part[0][k] >> 16) | part[1][k], (part[2][k] >> 16) | part[3][k]);
+          *reinterpret_cast<uint2*>(a.out + (k * a.rows + row) * a.ld + c) = w;
+        }
+      }
+    }
+  }
+  if constexpr (Sums) {
+    __shared__ float area[4][V][64];
+#pragma unroll
+    for (int i = 0; i < V; ++i) area[wave][i][lane] = sums[i];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float s = ((area[0][i][lane] + area[1][i][lane]) + area[2][i][lane]) + area[3][i][lane];
+        if (c + i < a.cols) a.partial[static_cast<int64_t>(blockIdx.y) * a.cols + c + i] = s;
+      }
+    }
+  }
+}
+
+int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+// Rows blocks of a prepare: about four workgroups a compute unit, eight rows each at least.
+int prepare_blocks(int dtype, int64_t rows, int64_t cols) {
+  const int64_t across = (cols + 64 * (dtype == F32::code ? 4 : 8) - 1) / (64 * (dtype == F32::code ? 4 : 8));
+  const int64_t want = (4 * compute_units() + across - 1) / across;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, (rows + 7) / 8)));
+}
+
+hipError_t launch_prepare(const PrepareArgs& a, int dtype, int blocks, hipStream_t stream) {
+  const int v = dtype == F32::code ? 4 : 8;
+  const int64_t width = a.out != nullptr ? std::max<int64_t>(a.ld, a.cols) : a.cols;
+  const dim3 grid(static_cast<uint32_t>((width + 64 * v - 1) / (64 * v)), static_cast<uint32_t>(blocks));
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (a.partial != nullptr) prepare_kernel<T, true><<<grid, dim3(256), 0, stream>>>(a);
+    else prepare_kernel<T, false><<<grid, dim3(256), 0, stream>>>(a);
+    return hipGetLastError();
+  });
+}
+
+// Takes pieces of a workspace; without one it only adds up their sizes.
+class Workspace {
+ public:
+  explicit Workspace(void* base) : base_(static_cast<char*>(base)) {}
+  template <typename E>
+  E* take(int64_t count) {
+    const int64_t at = used_;
+    used_ += (count * static_cast<int64_t>(sizeof(E)) + 255) / 256 * 256;
+    return base_ != nullptr ? reinterpret_cast<E*>(base_ + at) : nullptr;
+  }
+  bool dry() const { return base_ == nullptr; }
+  int64_t used() const { return used_; }
+
+ private:
+  char* base_;
+  int64_t used_ = 0;
+};
+
+// An operand as the products read it.
+struct Operand16 {
+  const uint16_t* data;
+  int64_t ld, plane;
+};
+
+constexpr int64_t kMostStride = int64_t{1} << 22;  // 256 rows of a tile within 2^31 bytes
+
+// Whether the products read [rows, cols] as it is.
+bool as_it_is(const void* data, int64_t stride, int64_t cols, int dtype) {
+  return dtype != F32::code && reinterpret_cast<uintptr_t>(data) % 16 == 0 && cols % 8 == 0 && stride % 8 == 0 &&
+         stride >= 0 && stride < kMostStride;
+}
+
+// `data` as it is, or laid out anew in the workspace.
+hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws,
+                   Operand16& got, hipStream_t stream) {
+  if (as_it_is(data, stride, cols, dtype)) {
+    got = {static_cast<const uint16_t*>(data), stride, 0};
+    return hipSuccess;
+  }
+  const int64_t ld = padded(cols);
+  uint16_t* out = ws.take<uint16_t>(rows * ld * (dtype == F32::code ? 3 : 1));
+  got = {out, ld, rows * ld};
+  if (ws.dry()) return hipSuccess;
+  PrepareArgs p{};
+  p.src = data;
+  p.src_stride = stride;
+  p.out = out;
+  p.ld = ld;
+  p.rows = rows;
+  p.cols = static_cast<int>(cols);
+  return launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
+}
+
+hipError_t multiply(ProductArgs& p, const Operand16& a, const Operand16& b, int dtype, bool a_cols, bool b_cols,
+                    Workspace& ws, hipStream_t stream) {
+  p.a = a.data;
+  p.lda = a.ld;
+  p.plane_a = a.plane;
+  p.b = b.data;
+  p.ldb = b.ld;
+  p.plane_b = b.plane;
+  plan_product(p, dtype);
+  if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
+  return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream);
+}
+
+}  // namespace
+
+hipError_t launch_linear(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
+  Workspace ws(workspace);
+  Operand16 x, w;
+  hipError_t err = lay_out(a.x, a.x_stride, a.rows, a.cols, a.dtype, ws, x, stream);
+  if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.outs, a.cols, a.dtype, ws, w, stream);
+  if (err != hipSuccess) return err;
+  ProductArgs p{};
+  p.m = static_cast<int>(a.rows);
+  p.n = static_cast<int>(a.outs);
+  p.k = static_cast<int>(a.cols);
+  p.bias = a.bias;
+  p.bias_f32 = a.bias_dtype == F32::code;
+  p.residual = a.residual;
+  p.ldr = a.r_stride;
+  p.act = a.act;
+  p.saved = a.saved;
+  p.out = a.y;
+  err = multiply(p, x, w, a.dtype, false, false, ws, stream);
+  if (bytes != nullptr) *bytes = ws.used();
+  return err;
+}
+
+hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
+  Workspace ws(workspace);
+  const bool products = a.dx != nullptr || a.dweight != nullptr;
+  // dz, and the column sums for db.
+  Operand16 dz{static_cast<const uint16_t*>(a.grad), a.g_stride, 0};
+  const bool form = products && (a.saved != nullptr || !as_it_is(a.grad, a.g_stride, a.outs, a.dtype));
+  if (form || a.dbias != nullptr) {
+    const int blocks = prepare_blocks(a.dtype, a.rows, a.outs);
+    PrepareArgs p{};
+    p.src = a.grad;
+    p.src_stride = a.g_stride;
+    p.saved = a.saved;
+    p.act = a.act;
+    p.rows = a.rows;
+    p.cols = static_cast<int>(a.outs);
+    if (form) {
+      p.ld = padded(a.outs);
+      p.out = ws.take<uint16_t>(a.rows * p.ld * (a.dtype == F32::code ? 3 : 1));
+      dz = {p.out, p.ld, a.rows * p.ld};
+    }
+    if (a.dbias != nullptr) p.partial = ws.take<float>(static_cast<int64_t>(blocks) * a.outs);
+    if (!ws.dry()) {
+      hipError_t err = launch_prepare(p, a.dtype, blocks, stream);
+      if (err == hipSuccess && a.dbias != nullptr)
+        err = launch_column_sums(p.partial, blocks, a.outs, a.outs, a.dbias, nullptr, a.bias_dtype, stream);
+      if (err != hipSuccess) return err;
+    }
+  }
+  hipError_t err = hipSuccess;
+  if (a.dx != nullptr) {
+    Operand16 w;
+    err = lay_out(a.weight, a.w_stride, a.outs, a.cols, a.dtype, ws, w, stream);
+    ProductArgs p{};
+    p.m = static_cast<int>(a.rows);
+    p.n = static_cast<int>(a.cols);
+    p.k = static_cast<int>(a.outs);
+    p.out = a.dx;
+    if (err == hipSuccess) err = multiply(p, dz, w, a.dtype, false, true, ws, stream);
+  }
+  if (err == hipSuccess && a.dweight != nullptr) {
+    Operand16 x;
+    err = lay_out(a.x, a.x_stride, a.rows, a.cols, a.dtype, ws, x, stream);
+    ProductArgs p{};
+    p.m = static_cast<int>(a.outs);
+    p.n = static_cast<int>(a.cols);
+    p.k = static_cast<int>(a.rows);
+    p.out = a.dweight;
+    if (err == hipSuccess) err = multiply(p, dz, x, a.dtype, true, true, ws, stream);
+  }
+  if (bytes != nullptr) *bytes = ws.used();
+  return err;
+}
+
+}  // namespace fh

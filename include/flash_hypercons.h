@@ -143,6 +143,69 @@ FH_API int fh_hc_apply_backward(const float* e, const void* x, const int64_t x_s
                          const int64_t grad_strides[3], void* dx, float* de, int dtype, int64_t batch, int n,
                          int64_t cols, hipStream_t stream);
 
+/* ---- the block between two stream mixings --------------------------------------
+ *
+ * Layer norm, a linear layer with its epilogue and the clipping of gradients; the
+ * reference has none of them.  Arrays of rows have contiguous columns and rows
+ * `stride` elements apart (any stride >= 0, any element alignment); results are
+ * contiguous.  Calls with a workspace take its size in *workspace_bytes.  With a
+ * NULL workspace they check their arguments, write the size they need there and
+ * launch nothing; where that is 0, any non-NULL pointer will do.  The workspace
+ * needs 16-byte alignment and may be used again once the launch has run. */
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over each row of x [rows, cols],
+ * 1 <= cols < 2^30.  weight and bias (each [cols] or NULL) are of param_dtype: dtype
+ * or FH_DTYPE_F32.  stats (float [rows, 2], may be NULL) receives each row's mean
+ * and 1 / sqrt(var + eps) for the backward pass. */
+FH_API int fh_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias, int param_dtype,
+                  double eps, void* y, float* stats, int dtype, int64_t rows, int64_t cols, hipStream_t stream);
+
+/* Gradients of fh_layer_norm for the upstream gradient grad: dx [rows, cols], and
+ * dweight and dbias ([cols] of param_dtype; each may be NULL), summed over the rows
+ * in a fixed order. */
+FH_API int fh_layer_norm_backward(const void* x, int64_t x_stride, const void* grad, int64_t grad_stride,
+                           const void* weight, int param_dtype, const float* stats, void* dx, void* dweight,
+                           void* dbias, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                           int64_t cols, hipStream_t stream);
+
+/* Activations of fh_linear: z, max(z, 0), z Phi(z), z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 and
+ * z / (1 + exp(-z)). */
+#define FH_ACT_NONE 0
+#define FH_ACT_RELU 1
+#define FH_ACT_GELU 2
+#define FH_ACT_GELU_TANH 3
+#define FH_ACT_SILU 4
+
+/* y = act(x weight^T + bias) + residual for x [rows, cols] and weight [outs, cols],
+ * 1 <= cols, outs < 2^22.  bias ([outs] or NULL) is of bias_dtype: dtype or
+ * FH_DTYPE_F32; residual is [rows, outs] or NULL.  `saved` (may be NULL) receives
+ * what the backward needs of the sum before the activation: [rows, outs], float for
+ * FH_DTYPE_F32, half otherwise.  Sums are FP32. */
+FH_API int fh_linear(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
+              int bias_dtype, const void* residual, int64_t residual_stride, int activation, void* y, void* saved,
+              void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows, int64_t cols, int64_t outs,
+              hipStream_t stream);
+
+/* Gradients of fh_linear for the upstream gradient grad [rows, outs]: dx [rows, cols],
+ * dweight [outs, cols] and dbias [outs] (bias_dtype); each may be NULL.  The residual's
+ * gradient is grad itself.  `saved` is the forward's, NULL without an activation. */
+FH_API int fh_linear_backward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                       const void* grad, int64_t grad_stride, const void* saved, int activation, void* dx,
+                       void* dweight, void* dbias, int bias_dtype, void* workspace, int64_t* workspace_bytes,
+                       int dtype, int64_t rows, int64_t cols, int64_t outs, hipStream_t stream);
+
+/* *norm (a float on the device) = the norm of all elements of `count` arrays, of
+ * sizes[i] elements of dtypes[i] each, with norm_type 1, 2 or infinity.  Sums are FP64.
+ * The lists are host arrays, read before the call returns. */
+FH_API int fh_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes, double norm_type,
+                 float* norm, void* workspace, int64_t* workspace_bytes, hipStream_t stream);
+
+/* The same, and out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); `out` NULL: in
+ * place, where a norm that is allowed leaves the arrays untouched. */
+FH_API int fh_clip_gradients(int count, const void* const* grads, void* const* out, const int64_t* sizes,
+                      const int* dtypes, double norm_type, double max_norm, float* norm, void* workspace,
+                      int64_t* workspace_bytes, hipStream_t stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 FH_API const char* fh_last_error(void);
 
