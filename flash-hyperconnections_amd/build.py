@@ -45,6 +45,7 @@ KERNEL_SOURCES = [
     "layer_norm.hip",
     "linear.hip",
     "linear_product.hip",
+    "linear_wide.hip",
     "grad_clip.hip",
     "fh_capi.cpp",
 ]

@@ -18,14 +18,15 @@ hipError_t with_type(int dtype, F f) {
 }
 
 // Elements c .. c + V - 1 of a row of `cols` (below 2^30), zero past its end.  Rows
-// start at any element: a 16-byte access needs no more than that here.
-template <typename T>
+// start at any element: a 16-byte access needs no more than that here.  Whole: cols
+// is a whole number of vectors.
+template <typename T, bool Whole = false>
 __device__ __forceinline__ U32x4 load_row(const typename T::storage* row, int c, int cols) {
   constexpr int V = kVec<T>;
   U32x4 w{0, 0, 0, 0};
   if (c + V <= cols) {
     __builtin_memcpy(&w, row + c, 16);
-  } else if (c < cols) {
+  } else if (!Whole && c < cols) {
     typename T::storage e[V] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -35,17 +36,28 @@ __device__ __forceinline__ U32x4 load_row(const typename T::storage* row, int c,
   return w;
 }
 
-template <typename T>
+template <typename T, bool Whole = false>
 __device__ __forceinline__ void store_row(U32x4 w, typename T::storage* row, int c, int cols) {
   constexpr int V = kVec<T>;
   if (c + V <= cols) {
     __builtin_memcpy(row + c, &w, 16);
-  } else if (c < cols) {
+  } else if (!Whole && c < cols) {
     typename T::storage e[V];
     __builtin_memcpy(e, &w, 16);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (c + i < cols) row[c + i] = e[i];
+  }
+}
+
+// Keeps the compiler from carrying what it computed from these bits any further: a
+// second pass over a row converts them again rather than hold them in FP32.
+__device__ __forceinline__ void forget(U32x4& w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t e = w[i];
+    asm volatile("" : "+v"(e));
+    w[i] = e;
   }
 }
 
@@ -103,8 +115,19 @@ __device__ __forceinline__ float load_param(const void* p, bool f32, int64_t i) 
 template <typename T>
 __device__ __forceinline__ void load_params(const void* p, bool f32, int c, int cols, float fill,
                                             float (&f)[kVec<T>]) {
+  constexpr int V = kVec<T>;
+  if (p != nullptr && c + V <= cols) {
+    if (f32) {
+      __builtin_memcpy(f, static_cast<const float*>(p) + c, sizeof(f));
+    } else {
+      U32x4 w;
+      __builtin_memcpy(&w, static_cast<const typename T::storage*>(p) + c, 16);
+      to_floats<T>(w, f);
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < kVec<T>; ++i) f[i] = p != nullptr && c + i < cols ? load_param<T>(p, f32, c + i) : fill;
+    for (int i = 0; i < V; ++i) f[i] = p != nullptr && c + i < cols ? load_param<T>(p, f32, c + i) : fill;
+  }
 }
 
 // Sum over the wavefront's lanes, the same bits in every lane (a butterfly adds

@@ -23,6 +23,8 @@
 namespace fh {
 namespace {
 
+constexpr int kBwdWaves = 8;
+
 // Sum over the WPR wavefronts that share a row, through `area` (WPR floats a row
 // group, unused between two calls on different areas).
 template <int WPR>
@@ -38,12 +40,13 @@ __device__ __forceinline__ float row_sum(float v, float* area, int part) {
 }
 
 // WPR wavefronts a row, GROUPS rows a workgroup at a time, NC vectors a lane.
-template <typename T, int WPR, int GROUPS, int NC>
+template <typename T, bool Whole, int WPR, int GROUPS, int NC>
 __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_fwd_kernel(NormArgs a) {
   using S = typename T::storage;
   constexpr int V = kVec<T>;
   __shared__ float area[2][WPR * GROUPS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave / WPR, part = wave % WPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
   static_assert(WPR == 1 || GROUPS == 1, "barriers: a workgroup's wavefronts leave together");
@@ -54,7 +57,7 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_fwd_kernel(NormArgs a)
   U32x4 raw[NC];
   float sum = 0.f;
 #pragma unroll
-  for (int u = 0; u < NC; ++u) raw[u] = load_row<T>(x, first + u * (64 * WPR * V), cols);
+  for (int u = 0; u < NC; ++u) raw[u] = load_row<T, Whole>(x, first + u * (64 * WPR * V), cols);
 #pragma unroll
   for (int u = 0; u < NC; ++u) {
     float f[V];
@@ -66,16 +69,20 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_fwd_kernel(NormArgs a)
   const float mean = row_sum<WPR>(sum, area[0] + group * WPR, part) * inv;
   float square = 0.f;
 #pragma unroll
+  for (int u = 0; u < NC; ++u) forget(raw[u]);
+#pragma unroll
   for (int u = 0; u < NC; ++u) {
     const int c = first + u * (64 * WPR * V);
     float f[V];
     to_floats<T>(raw[u], f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = c + i < cols ? f[i] - mean : 0.f;
+      const float d = c + (Whole ? 0 : i) < cols ? f[i] - mean : 0.f;
       square = __builtin_fmaf(d, d, square);
     }
   }
+#pragma unroll
+  for (int u = 0; u < NC; ++u) forget(raw[u]);
   const float var = row_sum<WPR>(square, area[1] + group * WPR, part) * inv;
   const float rstd = 1.f / __builtin_sqrtf(var + a.eps);
   if (a.stats != nullptr && part == 0 && lane == 0) {
@@ -92,7 +99,7 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_fwd_kernel(NormArgs a)
     load_params<T>(a.bias, a.params_f32, c, cols, 0.f, b);
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = __builtin_fmaf((f[i] - mean) * rstd, w[i], b[i]);
-    store_row<T>(from_floats<T>(f), y, c, cols);
+    store_row<T, Whole>(from_floats<T>(f), y, c, cols);
   }
 }
 
@@ -142,18 +149,19 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(NormArgs a) {
   }
 }
 
-// dx, and with Params the workgroup's row of `partial` ([G, 2, C]: dw, db).  Sixteen
-// wavefronts: a lane's sums for more than two vectors of 16-bit columns would not
-// leave room in its registers for the next row, which is loaded while this one is
-// summed (the row groups wait for one another at every row).
-template <typename T, int WPR, int NC, bool Params>
-__global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
+// dx, and with Params the workgroup's row of `partial` ([G, 2, C]: dw, db).  Eight
+// wavefronts, whose registers hold the sums of up to four vectors of 16-bit columns a
+// lane and the next row, which is loaded while this one is summed (the row groups
+// wait for one another at every row).
+template <typename T, bool Whole, int WPR, int NC, bool Params>
+__global__ __launch_bounds__(64 * kBwdWaves) void norm_bwd_kernel(NormArgs a) {
   using S = typename T::storage;
-  constexpr int V = kVec<T>, GROUPS = 16 / WPR;
+  constexpr int V = kVec<T>, GROUPS = kBwdWaves / WPR;
   constexpr int kWidth = 64 * WPR * V;  // columns of one vector of every lane of a row group
-  __shared__ float2 area[2][16];
-  __shared__ float joined[Params && GROUPS > 1 ? 2 * kWidth : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float2 area[2][kBwdWaves];
+  __shared__ __attribute__((aligned(16))) float sums[Params ? GROUPS * 2 * kWidth : 1];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave / WPR, part = wave % WPR;
   const int first = (part * 64 + lane) * V, cols = static_cast<int>(a.cols);
   const float inv = 1.f / static_cast<float>(cols);
@@ -180,8 +188,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
     const S* g = static_cast<const S*>(a.grad) + at * a.grad_stride;
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
-      xr[u] = load_row<T>(x, first + u * kWidth, cols);
-      gr[u] = load_row<T>(g, first + u * kWidth, cols);
+      xr[u] = load_row<T, Whole>(x, first + u * kWidth, cols);
+      gr[u] = load_row<T, Whole>(g, first + u * kWidth, cols);
     }
     mean = a.stats[2 * at];
     rstd = a.stats[2 * at + 1];
@@ -195,22 +203,31 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
     const float m = mean, r = rstd;
     if (t + 1 < turns) fetch(row + stride);
     float s1 = 0.f, s2 = 0.f;
+    if (live) {
+#pragma unroll
+      for (int u = 0; u < NC; ++u) {
+        float xf[V], gf[V];
+        to_floats<T>(xc[u], xf);
+        to_floats<T>(gc[u], gf);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          // Past the row's end g and so q are 0.
+          const float n = (xf[i] - m) * r, q = gf[i] * w[u][i];
+          s1 += q;
+          s2 = __builtin_fmaf(q, n, s2);
+          if constexpr (Params) {
+            dw[u][i] = __builtin_fmaf(gf[i], n, dw[u][i]);
+            db[u][i] += gf[i];
+          }
+        }
+        // One vector's values at a time.
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
-      float xf[V], gf[V];
-      to_floats<T>(xc[u], xf);
-      to_floats<T>(gc[u], gf);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        // Past the row's end g and so q are 0.
-        const float n = (xf[i] - m) * r, q = gf[i] * w[u][i];
-        s1 += q;
-        s2 = __builtin_fmaf(q, n, s2);
-        if constexpr (Params) {
-          dw[u][i] = live ? __builtin_fmaf(gf[i], n, dw[u][i]) : dw[u][i];
-          db[u][i] = live ? db[u][i] + gf[i] : db[u][i];
-        }
-      }
+      forget(xc[u]);
+      forget(gc[u]);
     }
     s1 = wave_sum(s1);
     s2 = wave_sum(s2);
@@ -240,7 +257,8 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
           const float n = (xf[i] - m) * r, q = gf[i] * w[u][i];
           xf[i] = r * (__builtin_fmaf(-n, c2, q) - c1);
         }
-        store_row<T>(from_floats<T>(xf), dx, first + u * kWidth, cols);
+        store_row<T, Whole>(from_floats<T>(xf), dx, first + u * kWidth, cols);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -248,31 +266,21 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
     float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
 #pragma unroll
     for (int u = 0; u < NC; ++u) {
-      if constexpr (GROUPS > 1) {
-        // The groups' sums in order 0, 1, ...
-        for (int k = 0; k < GROUPS; ++k) {
-          __syncthreads();
-          if (group != k) continue;
+      // The groups' sums of this vector's columns, added in order 0, 1, ....
+      float* own = sums + group * 2 * kWidth + first;
+      if (u > 0) __syncthreads();
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float* at = joined + i * (64 * WPR) + part * 64 + lane;
-            if (k > 0) {
-              dw[u][i] += at[0];
-              db[u][i] += at[kWidth];
-            }
-            at[0] = dw[u][i];
-            at[kWidth] = db[u][i];
-          }
-        }
+      for (int i = 0; i < V; i += 4) {
+        *reinterpret_cast<float4*>(own + i) = make_float4(dw[u][i], dw[u][i + 1], dw[u][i + 2], dw[u][i + 3]);
+        *reinterpret_cast<float4*>(own + kWidth + i) = make_float4(db[u][i], db[u][i + 1], db[u][i + 2], db[u][i + 3]);
       }
-      if (group == GROUPS - 1) {
-        const int c = first + u * kWidth;
+      __syncthreads();
+      for (int j = threadIdx.x; j < 2 * kWidth; j += 64 * kBwdWaves) {
+        float s = sums[j];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (c + i < cols) {
-            out[c + i] = dw[u][i];
-            out[a.cols + c + i] = db[u][i];
-          }
+        for (int k = 1; k < GROUPS; ++k) s += sums[k * 2 * kWidth + j];
+        const int c = j % kWidth + u * kWidth;
+        if (c < cols) out[j / kWidth * a.cols + c] = s;
       }
     }
   }
@@ -350,6 +358,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial,
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float s = 0.f;
   if (c < width)
+#pragma unroll 8
     for (int k = wave; k < count; k += 16) s += partial[k * width + c];
   area[wave][lane] = s;
   __syncthreads();
@@ -366,20 +375,30 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial,
 
 template <typename T, int WPR, int GROUPS, int NC>
 hipError_t fwd(const NormArgs& a, hipStream_t stream) {
-  norm_fwd_kernel<T, WPR, GROUPS, NC>
-      <<<dim3(static_cast<uint32_t>((a.rows + GROUPS - 1) / GROUPS)), dim3(64 * WPR * GROUPS), 0, stream>>>(a);
+  const dim3 grid(static_cast<uint32_t>((a.rows + GROUPS - 1) / GROUPS)), block(64 * WPR * GROUPS);
+  if (a.cols % kVec<T> == 0) {
+    norm_fwd_kernel<T, true, WPR, GROUPS, NC><<<grid, block, 0, stream>>>(a);
+  } else {
+    norm_fwd_kernel<T, false, WPR, GROUPS, NC><<<grid, block, 0, stream>>>(a);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, bool Whole, int WPR, int NC>
+hipError_t bwd_rows(const NormArgs& a, int blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(64 * kBwdWaves);
+  if (a.partial != nullptr) {
+    norm_bwd_kernel<T, Whole, WPR, NC, true><<<grid, block, 0, stream>>>(a);
+  } else {
+    norm_bwd_kernel<T, Whole, WPR, NC, false><<<grid, block, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <typename T, int WPR, int NC>
 hipError_t bwd(const NormArgs& a, int blocks, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(blocks)), block(1024);
-  if (a.partial != nullptr) {
-    norm_bwd_kernel<T, WPR, NC, true><<<grid, block, 0, stream>>>(a);
-  } else {
-    norm_bwd_kernel<T, WPR, NC, false><<<grid, block, 0, stream>>>(a);
-  }
-  return hipGetLastError();
+  return a.cols % kVec<T> == 0 ? bwd_rows<T, true, WPR, NC>(a, blocks, stream)
+                               : bwd_rows<T, false, WPR, NC>(a, blocks, stream);
 }
 
 constexpr int64_t kMostVectors = 4096;    // of a forward row in registers
@@ -437,11 +456,11 @@ hipError_t launch_norm_backward(const NormArgs& a, void* dweight, void* dbias, i
     }
     if (nv <= 64) return bwd<T, 1, 1>(a, blocks, stream);
     if (nv <= 128) return bwd<T, 1, 2>(a, blocks, stream);
-    if (nv <= 256) return bwd<T, 2, 2>(a, blocks, stream);
-    if (nv <= 512) return bwd<T, 4, 2>(a, blocks, stream);
-    if (nv <= 1024) return bwd<T, 8, 2>(a, blocks, stream);
-    if (nv <= 2048) return bwd<T, 16, 2>(a, blocks, stream);
-    if constexpr (T::code == F32::code) return bwd<T, 16, 4>(a, blocks, stream);
+    if (nv <= 256) return bwd<T, 1, 4>(a, blocks, stream);
+    if (nv <= 512) return bwd<T, 2, 4>(a, blocks, stream);
+    if (nv <= 1024) return bwd<T, 4, 4>(a, blocks, stream);
+    if (nv <= 2048) return bwd<T, 8, 4>(a, blocks, stream);
+    if constexpr (T::code == F32::code) return bwd<T, 8, 8>(a, blocks, stream);
     return hipErrorInvalidValue;  // 16384 columns are 2048 vectors of a 16-bit type
   });
   if (err != hipSuccess || a.partial == nullptr) return err;

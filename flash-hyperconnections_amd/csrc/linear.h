@@ -22,6 +22,7 @@ struct ProductArgs {
   int64_t plane_a, plane_b;
   int m, n, k;
   int tiles_m, tiles_n;
+  int side;              // of a tile
   int slices;            // of the sum over k
   float* partial;        // [slices, m, n] where there are several
   const void* bias;      // [n] or null, FP32 or the output's type
@@ -43,90 +44,251 @@ using Saved = std::conditional_t<T::code == F32::code, F32, F16>;
 
 __device__ __forceinline__ float clamp_saved(float z) { return z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z; }
 
-// act(z); relu keeps a NaN.
-__device__ __forceinline__ float activate(float z, int act) {
+// Phi(z) and the normal density at z, by formula 7.1.26 of Abramowitz and Stegun's
+// handbook, whose error of 1.5e-7 is far below the last bit of a 16-bit result.  The
+// exponential it needs is the density's as well.  (The library's erff, in branches,
+// took 0.5 ms of the 1.0 that a gelu over 16384 x 16384 results cost.)
+struct Normal {
+  float phi, density;
+};
+__device__ __forceinline__ Normal normal_of(float z) {
+  const float x = __builtin_fabsf(z);
+  const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);  // exp(-z^2 / 2)
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164189f, x, 1.f));  // 0.3275911 / sqrt(2)
+  float s = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  s = __builtin_fmaf(s, t, 1.421413741f);
+  s = __builtin_fmaf(s, t, -0.284496736f);
+  s = __builtin_fmaf(s, t, 0.254829592f);
+  const float tail = 0.5f * (s * t) * e;  // Phi(-|z|)
+  return {z < 0.f ? tail : 1.f - tail, 0.39894228040143268f * e};
+}
+
+// 1 / (1 + exp(-v)), by the hardware's exp2 and reciprocal (one unit in the last place
+// each) for 16-bit results.
+template <typename T>
+__device__ __forceinline__ float logistic(float v) {
+  if constexpr (T::code == F32::code) return 1.f / (1.f + expf(-v));
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
+}
+
+// act(z) of eight; relu keeps a NaN.
+template <typename T>
+__device__ __forceinline__ void activate_eight(float (&v)[8], int act) {
   switch (act) {
-    case FH_ACT_RELU: return z < 0.f ? 0.f : z;
-    case FH_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
-    case FH_ACT_GELU_TANH: {
-      // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), without the difference of near values.
-      const float u2 = 1.5957691216057308f * __builtin_fmaf(0.044715f * z * z, z, z);
-      return z / (1.f + expf(-u2));
-    }
-    case FH_ACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
+    case FH_ACT_RELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+      break;
+    case FH_ACT_GELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (T::code == F32::code) v[k] *= 0.5f * (1.f + erff(v[k] * 0.70710678118654752f));
+        else v[k] *= normal_of(v[k]).phi;
+      }
+      break;
+    case FH_ACT_GELU_TANH:
+      // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), without the difference of near values.
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] *= logistic<T>(1.5957691216057308f * __builtin_fmaf(0.044715f * v[k] * v[k], v[k], v[k]));
+      break;
+    case FH_ACT_SILU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= logistic<T>(v[k]);
+      break;
+    default: break;
   }
 }
 
 // act'(z).
+template <typename T>
 __device__ __forceinline__ float slope(float z, int act) {
   switch (act) {
     case FH_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case FH_ACT_GELU:
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+    case FH_ACT_GELU: {
+      if constexpr (T::code == F32::code)
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+      const Normal n = normal_of(z);
+      return __builtin_fmaf(z, n.density, n.phi);
+    }
     case FH_ACT_GELU_TANH: {
-      const float u2 = 1.5957691216057308f * __builtin_fmaf(0.044715f * z * z, z, z);
-      const float q = 1.f / (1.f + expf(-u2));
+      const float q = logistic<T>(1.5957691216057308f * __builtin_fmaf(0.044715f * z * z, z, z));
       const float du2 = 1.5957691216057308f * __builtin_fmaf(0.134145f * z, z, 1.f);
       // q (1 - q) is 0 where exp has left its range, whatever z du2 is.
       const float curve = q * (1.f - q);
       return curve > 0.f ? __builtin_fmaf(z * du2, curve, q) : q;
     }
     case FH_ACT_SILU: {
-      const float q = 1.f / (1.f + expf(-z)), curve = q * (1.f - q);
+      const float q = logistic<T>(z), curve = q * (1.f - q);
       return curve > 0.f ? __builtin_fmaf(z, curve, q) : q;
     }
     default: return 1.f;
   }
 }
 
-// Four neighbouring results (row i, columns j .. j + 3) on their way out.
-template <typename T>
-__device__ __forceinline__ void finish_four(const ProductArgs& p, int i, int j, const float (&sum)[4]) {
-  using S = typename T::storage;
-  using Z = typename Saved<T>::storage;
-  const int64_t at = static_cast<int64_t>(i) * p.n + j;
-  const int left = p.n - j;
-  S r[4] = {};
-  if (p.residual != nullptr) {
-    const S* from = static_cast<const S*>(p.residual) + static_cast<int64_t>(i) * p.ldr + j;
-    if (left >= 4) {
-      __builtin_memcpy(r, from, sizeof(r));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (e < left) r[e] = from[e];
-    }
-  }
-  S y[4];
-  Z z[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float v = sum[e];
-    if (p.bias != nullptr) v += e < left ? load_param<T>(p.bias, p.bias_f32, j + e) : 0.f;
-    z[e] = T::code == F32::code ? static_cast<Z>(v) : static_cast<Z>(clamp_saved(v));
-    v = activate(v, p.act);
-    if (p.residual != nullptr) v += to_f32<T>(r[e]);
-    y[e] = from_f32<T>(v);
-  }
-  S* out = static_cast<S*>(p.out) + at;
-  Z* saved = static_cast<Z*>(p.saved) + at;
-  if (left >= 4) {
-    __builtin_memcpy(out, y, sizeof(y));
-    if (p.saved != nullptr) __builtin_memcpy(saved, z, sizeof(z));
+// Elements 0 .. count - 1 of eight, count at least 1.
+template <typename S>
+__device__ __forceinline__ void load_eight(const S* from, int count, S (&e)[8]) {
+  if (count >= 8) {
+    __builtin_memcpy(e, from, sizeof(e));
   } else {
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (e < left) {
-        out[e] = y[e];
-        if (p.saved != nullptr) saved[e] = z[e];
-      }
+    for (int i = 0; i < 8; ++i) e[i] = i < count ? from[i] : S{};
   }
 }
+template <typename S>
+__device__ __forceinline__ void store_eight(const S (&e)[8], S* to, int count) {
+  if (count >= 8) {
+    __builtin_memcpy(to, e, sizeof(e));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (i < count) to[i] = e[i];
+  }
+}
+
+// Eight values rounded to the storage type.
+template <typename T>
+__device__ __forceinline__ void round_eight(const float (&f)[8], typename T::storage (&e)[8]) {
+  if constexpr (T::code == F32::code) {
+    __builtin_memcpy(e, f, sizeof(e));
+  } else {
+    const U32x4 w{round_pair<T>(f[0], f[1]), round_pair<T>(f[2], f[3]), round_pair<T>(f[4], f[5]),
+                  round_pair<T>(f[6], f[7])};
+    __builtin_memcpy(e, &w, sizeof(e));
+  }
+}
+
+// Eight neighbouring results (row i, columns j .. j + 7) on their way out: bias,
+// activation, residual; or into the slice's partial sums.
+template <typename T>
+__device__ __forceinline__ void finish_eight(const ProductArgs& p, int slice, int i, int j, float (&v)[8]) {
+  using S = typename T::storage;
+  using Z = Saved<T>;
+  if (i >= p.m || j >= p.n) return;
+  const int64_t at = static_cast<int64_t>(i) * p.n + j;
+  const int left = p.n - j;
+  if (p.slices > 1) {
+    store_eight(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
+    return;
+  }
+  if (p.bias != nullptr) {
+    float b[8];
+    if (p.bias_f32) {
+      load_eight(static_cast<const float*>(p.bias) + j, left, b);
+    } else {
+      S e[8];
+      load_eight(static_cast<const S*>(p.bias) + j, left, e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[k] = to_f32<T>(e[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += b[k];
+  }
+  if (p.saved != nullptr) {
+    float z[8];
+    typename Z::storage e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] = T::code == F32::code ? v[k] : clamp_saved(v[k]);
+    round_eight<Z>(z, e);
+    store_eight(e, static_cast<typename Z::storage*>(p.saved) + at, left);
+  }
+  if (p.act != FH_ACT_NONE) activate_eight<T>(v, p.act);
+  S e[8];
+  if (p.residual != nullptr) {
+    load_eight(static_cast<const S*>(p.residual) + static_cast<int64_t>(i) * p.ldr + j, left, e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += to_f32<T>(e[k]);
+  }
+  round_eight<T>(v, e);
+  store_eight(e, static_cast<S*>(p.out) + at, left);
+}
+
+// 64 x 64 results of a wavefront, from the matrix instructions' accumulators (row
+// 16 i + lane % 16, columns 16 j + 4 (lane / 16) + 0..3) through 16 KB of its own LDS,
+// so that eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row
+// r is at place c ^ (r & 15), which spreads reads and writes over the banks.  (Stored
+// from the accumulators, a lane's four columns alone, a product of 16384 x 4096 x 16384
+// with gelu spent a third of its time here.)
+template <typename T>
+__device__ __forceinline__ void finish_block(const ProductArgs& p, int slice, const Floats4 (*acc)[4], char* area,
+                                             int row, int col, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 16 * i + (lane & 15), c = 4 * j + (lane >> 4);
+      *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = acc[i][j];
+    }
+  asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
+#pragma unroll 1
+  for (int it = 0; it < 8; ++it) {
+    const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
+    float v[8];
+    __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
+    __builtin_memcpy(v + 4, area + r * 256 + (((c + 1) ^ (r & 15)) << 4), 16);
+    finish_eight<T>(p, slice, row + r, col + 8 * (lane & 7), v);
+  }
+  asm volatile("" ::: "memory");
+}
+
+typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
+
+template <typename E>
+__device__ __forceinline__ Floats4 mfma16(U32x4 a, U32x4 b, Floats4 c) {
+  if constexpr (E::code == F16::code) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(F16x8, a), __builtin_bit_cast(F16x8, b), c, 0, 0,
+                                                  0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+}
+
+// The tile of a workgroup.  Workgroups go to the eight dies in turn; each die takes
+// one eighth of the tiles in a row, eight tiles of m for each n, so that what runs on
+// it at a time shares operands in its L2.
+struct Tile {
+  int m, n;
+};
+__device__ __forceinline__ Tile tile_of(const ProductArgs& p, int block) {
+  const int tiles = p.tiles_m * p.tiles_n, die = block & 7, each = tiles >> 3, more = tiles & 7;
+  const int at = die * each + (die < more ? die : more) + (block >> 3);
+  const int band = 8 * p.tiles_n, first = at / band * 8;
+  const int high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
+  const int in = at - first * p.tiles_n;
+  return {first + in % high, in / high};
+}
+
+// The steps of 64 in k that a slice of a sum takes; for FP32 once for each product of
+// planes, the smallest first (those of 2^-24 and below are left out).
+template <typename T>
+struct Steps {
+  int depth, begin, end;
+  __device__ __forceinline__ Steps(const ProductArgs& p, int slice) {
+    depth = (p.k + 63) / 64;
+    const int64_t steps = static_cast<int64_t>(depth) * (T::code == F32::code ? 6 : 1);
+    begin = static_cast<int>(steps * slice / p.slices);
+    end = static_cast<int>(steps * (slice + 1) / p.slices);
+  }
+  // Step s: its place in k, and the planes' offsets in bytes.
+  __device__ __forceinline__ void place(const ProductArgs& p, int s, int& t, int64_t& oa, int64_t& ob) const {
+    t = s;
+    oa = ob = 0;
+    if constexpr (T::code == F32::code) {
+      const int pair = s / depth;
+      t = s - pair * depth;
+      oa = 2 * ((0x210100 >> (20 - 4 * pair)) & 15) * p.plane_a;
+      ob = 2 * ((0x012010 >> (20 - 4 * pair)) & 15) * p.plane_b;
+    }
+  }
+};
 
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
 // floats.  `dtype` is the output's; FP32 runs on bf16 planes.
 void plan_product(ProductArgs& p, int dtype);
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 
 }  // namespace fh

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
       float zf[V];
       to_floats<Z>(load_row<Z>(z, c, a.cols), zf);
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] *= slope(zf[i], a.act);
+      for (int i = 0; i < V; ++i) f[i] *= slope<T>(zf[i], a.act);
       rounded = from_floats<T>(f);
     }
     if constexpr (Sums) {

@@ -7,23 +7,10 @@
 namespace fh {
 namespace {
 
-typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
 typedef short S16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 128, kDepth = 64;
 constexpr int kPanel = kTile * kDepth;  // elements of one operand's tile
-
-template <typename E>
-__device__ __forceinline__ Floats4 mfma(U32x4 a, U32x4 b, Floats4 c) {
-  if constexpr (E::code == F16::code) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(F16x8, a), __builtin_bit_cast(F16x8, b), c, 0, 0,
-                                                  0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0,
-                                                   0, 0);
-  }
-}
 
 // Exchange of 16-byte chunks along an LDS row of a tile in columns, by the row k.
 __device__ __forceinline__ int swap_of(int k) { return 2 * ((k & 3) | (((k >> 3) & 1) << 2)); }
@@ -92,27 +79,17 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[2][2][kPanel];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x, slice = blockIdx.y;
-  const int m0 = tile / p.tiles_n * kTile, n0 = tile % p.tiles_n * kTile;
+  const Tile tile = tile_of(p, blockIdx.x);
+  const int m0 = tile.m * kTile, n0 = tile.n * kTile, slice = blockIdx.y;
   Panel<ACols> a;
   Panel<BCols> b;
   a.init(p.a, p.lda, m0, p.m, lane, wave);
   b.init(p.b, p.ldb, n0, p.n, lane, wave);
-  // FP32: products of planes, the smallest first; those of 2^-24 and below are left out.
-  const int pairs = T::code == F32::code ? 6 : 1;
-  const int depth = (p.k + kDepth - 1) / kDepth, steps = depth * pairs;
-  const int begin = static_cast<int>(static_cast<int64_t>(steps) * slice / p.slices);
-  const int end = static_cast<int>(static_cast<int64_t>(steps) * (slice + 1) / p.slices);
+  const Steps<T> steps(p, slice);
   const auto stage = [&](int step, int buffer) {
-    int64_t oa = 0, ob = 0;
-    int t = step;
-    if constexpr (T::code == F32::code) {
-      const int pair = step / depth;
-      t -= pair * depth;
-      const int pa = (0x210100 >> (20 - 4 * pair)) & 15, pb = (0x012010 >> (20 - 4 * pair)) & 15;
-      oa = 2 * pa * p.plane_a;
-      ob = 2 * pb * p.plane_b;
-    }
+    int64_t oa, ob;
+    int t;
+    steps.place(p, step, t, oa, ob);
     a.stage(oa, t, p.k, lds_address(lds[buffer][0]), wave);
     b.stage(ob, t, p.k, lds_address(lds[buffer][1]), wave);
   };
@@ -122,12 +99,12 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = Floats4{0.f, 0.f, 0.f, 0.f};
-  if (begin < end) stage(begin, 0);
-  for (int s = begin; s < end; ++s) {
-    const int buffer = (s - begin) & 1;
+  if (steps.begin < steps.end) stage(steps.begin, 0);
+  for (int s = steps.begin; s < steps.end; ++s) {
+    const int buffer = (s - steps.begin) & 1;
     wait_vm<0>();
     __syncthreads();  // the tile is there, and the other buffer has been read
-    if (s + 1 < end) stage(s + 1, buffer ^ 1);
+    if (s + 1 < steps.end) stage(s + 1, buffer ^ 1);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       U32x4 fa[4], fb[4];
@@ -140,42 +117,30 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma<E>(fb[j], fa[i], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<E>(fb[j], fa[i], acc[i][j]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = m0 + wm + 16 * i + (lane & 15), col = n0 + wn + 16 * j + 4 * (lane >> 4);
-      if (row >= p.m || col >= p.n) continue;
-      if (p.slices > 1) {
-        float* to = p.partial + (static_cast<int64_t>(slice) * p.m + row) * p.n + col;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < p.n) to[e] = acc[i][j][e];
-      } else {
-        const float sum[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        finish_four<T>(p, row, col, sum);
-      }
-    }
+  __syncthreads();  // the buffers have been read: each wavefront takes 16 KB of them
+  finish_block<T>(p, slice, acc, reinterpret_cast<char*>(lds) + wave * 16384, m0 + wm, n0 + wn, lane);
 }
 
 // Adds the slices in order and finishes.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
-  const int quads = (p.n + 3) / 4;
-  const int64_t total = static_cast<int64_t>(p.m) * quads;
+  const int across = (p.n + 7) / 8, slices = p.slices;
+  const int64_t total = static_cast<int64_t>(p.m) * across, size = static_cast<int64_t>(p.m) * p.n;
+  p.slices = 1;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < total;
        q += static_cast<int64_t>(gridDim.x) * 256) {
-    const int row = static_cast<int>(q / quads), col = static_cast<int>(q % quads) * 4;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const int row = static_cast<int>(q / across), col = static_cast<int>(q % across) * 8;
+    float sum[8] = {}, v[8];
     const float* from = p.partial + static_cast<int64_t>(row) * p.n + col;
-    for (int s = 0; s < p.slices; ++s, from += static_cast<int64_t>(p.m) * p.n)
+    for (int s = 0; s < slices; ++s, from += size) {
+      load_eight(from, p.n - col, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < p.n) sum[e] += from[e];
-    finish_four<T>(p, row, col, sum);
+      for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+    finish_eight<T>(p, 0, row, col, sum);
   }
 }
 
@@ -186,25 +151,46 @@ hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t strea
   if (!a_cols && b_cols) product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
   if (a_cols && b_cols) product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
   if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
-  if (const hipError_t err = hipGetLastError(); err != hipSuccess || p.slices == 1) return err;
-  const int64_t quads = static_cast<int64_t>(p.m) * ((p.n + 3) / 4);
-  join_kernel<T><<<dim3(static_cast<uint32_t>(std::min<int64_t>((quads + 255) / 256, 4096))), block, 0, stream>>>(p);
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t join(const ProductArgs& p, hipStream_t stream) {
+  const int64_t groups = static_cast<int64_t>(p.m) * ((p.n + 7) / 8);
+  join_kernel<T><<<dim3(static_cast<uint32_t>(std::min<int64_t>((groups + 255) / 256, 4096))), dim3(256), 0,
+                   stream>>>(p);
+  return hipGetLastError();
+}
+
+void set_tiles(ProductArgs& p, int side) {
+  p.side = side;
+  p.tiles_m = (p.m + side - 1) / side;
+  p.tiles_n = (p.n + side - 1) / side;
 }
 
 }  // namespace
 
 void plan_product(ProductArgs& p, int dtype) {
-  p.tiles_m = (p.m + kTile - 1) / kTile;
-  p.tiles_n = (p.n + kTile - 1) / kTile;
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   const int64_t steps = static_cast<int64_t>((p.k + kDepth - 1) / kDepth) * (dtype == F32::code ? 6 : 1);
+  const int64_t units = compute_units();
+  // Tiles of 256 once they keep nearly all compute units at work to the end.
+  set_tiles(p, 256);
+  p.slices = 1;
+  const int64_t wide = static_cast<int64_t>(p.tiles_m) * p.tiles_n, rounds = (wide + units - 1) / units;
+  if (wide * 10 >= rounds * units * 8 && p.m > 128 && p.n > 128) return;
+  set_tiles(p, kTile);
   // Slices of at least eight steps until two workgroups a compute unit have work.
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * compute_units() / tiles, steps / 8)));
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * units / tiles, steps / 8)));
 }
 
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
-  return with_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
+  if (p.side == 256) return launch_wide_product(p, dtype, a_cols, b_cols, stream);
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const hipError_t err = run<T>(p, a_cols, b_cols, stream);
+    return err != hipSuccess || p.slices == 1 ? err : join<T>(p, stream);
+  });
 }
 
 }  // namespace fh
