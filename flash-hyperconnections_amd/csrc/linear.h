@@ -204,22 +204,17 @@ __device__ __forceinline__ void finish_eight(const ProductArgs& p, int slice, in
   store_eight(e, static_cast<S*>(p.out) + at, left);
 }
 
-// 64 x 64 results of a wavefront, from the matrix instructions' accumulators (row
-// 16 i + lane % 16, columns 16 j + 4 (lane / 16) + 0..3) through 16 KB of its own LDS,
-// so that eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row
-// r is at place c ^ (r & 15), which spreads reads and writes over the banks.  (Stored
-// from the accumulators, a lane's four columns alone, a product of 16384 x 4096 x 16384
-// with gelu spent a third of its time here.)
+// 64 x 64 results of a wavefront on their way out through 16 KB of its own LDS, so that
+// eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row r is at
+// place c ^ (r & 15), which spreads reads and writes over the banks.  (Stored from the
+// accumulators, a lane's four columns alone, a product of 16384 x 4096 x 16384 with
+// gelu spent a third of its time here.)
+__device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
+  *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;
+}
 template <typename T>
-__device__ __forceinline__ void finish_block(const ProductArgs& p, int slice, const Floats4 (*acc)[4], char* area,
-                                             int row, int col, int lane) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = 16 * i + (lane & 15), c = 4 * j + (lane >> 4);
-      *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = acc[i][j];
-    }
+__device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
+                                              int lane) {
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
 #pragma unroll 1
   for (int it = 0; it < 8; ++it) {
@@ -246,6 +241,19 @@ __device__ __forceinline__ Floats4 mfma16(U32x4 a, U32x4 b, Floats4 c) {
   }
 }
 
+typedef float Floats16 __attribute__((ext_vector_type(16)));
+
+template <typename E>
+__device__ __forceinline__ Floats16 mfma32(U32x4 a, U32x4 b, Floats16 c) {
+  if constexpr (E::code == F16::code) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(F16x8, a), __builtin_bit_cast(F16x8, b), c, 0, 0,
+                                                  0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+}
+
 // The tile of a workgroup.  Workgroups go to the eight dies in turn; each die takes
 // one eighth of the tiles in a row, eight tiles of m for each n, so that what runs on
 // it at a time shares operands in its L2.
@@ -261,13 +269,13 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int block) {
   return {first + in % high, in / high};
 }
 
-// The steps of 64 in k that a slice of a sum takes; for FP32 once for each product of
+// The steps of Depth in k that a slice of a sum takes; for FP32 once for each product of
 // planes, the smallest first (those of 2^-24 and below are left out).
-template <typename T>
+template <typename T, int Depth>
 struct Steps {
   int depth, begin, end;
   __device__ __forceinline__ Steps(const ProductArgs& p, int slice) {
-    depth = (p.k + 63) / 64;
+    depth = (p.k + Depth - 1) / Depth;
     const int64_t steps = static_cast<int64_t>(depth) * (T::code == F32::code ? 6 : 1);
     begin = static_cast<int>(steps * slice / p.slices);
     end = static_cast<int>(steps * (slice + 1) / p.slices);

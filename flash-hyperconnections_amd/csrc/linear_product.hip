@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
   Panel<BCols> b;
   a.init(p.a, p.lda, m0, p.m, lane, wave);
   b.init(p.b, p.ldb, n0, p.n, lane, wave);
-  const Steps<T> steps(p, slice);
+  const Steps<T, kDepth> steps(p, slice);
   const auto stage = [&](int step, int buffer) {
     int64_t oa, ob;
     int t;
@@ -121,7 +121,12 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
     }
   }
   __syncthreads();  // the buffers have been read: each wavefront takes 16 KB of them
-  finish_block<T>(p, slice, acc, reinterpret_cast<char*>(lds) + wave * 16384, m0 + wm, n0 + wn, lane);
+  char* area = reinterpret_cast<char*>(lds) + wave * 16384;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) park(area, 16 * i + (lane & 15), 4 * j + (lane >> 4), acc[i][j]);
+  finish_parked<T>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // Adds the slices in order and finishes.

@@ -1,14 +1,15 @@
 // Matrix products of the linear layer in 256 x 256 tiles, for sums large enough to
 // fill the card with them.
 //
-// Eight wavefronts of 128 x 64 results each: a wavefront reads 24 KB of LDS for 1 M
-// multiply-adds, three quarters of the time that its matrix instructions take (64 x 64
-// results of a 128 x 128 tile's wavefront read for as long as they compute).  The sum
-// runs in steps of 64 through two buffers, filled by loads that go to LDS directly.
-// A step has four phases of 16 matrix instructions, and each phase reads the next
-// one's operands, so that LDS works beside the matrix cores; before the last phase
-// the wavefronts meet, for by then this step's buffer has been read (it takes the
-// loads of the step after the next) and the next step's has been filled.
+// Eight wavefronts of 128 x 64 results each, on 32 x 32 x 16 instructions (half as many
+// to issue as 16 x 16 x 32, for the same work): a wavefront reads 24 KB of LDS for 1 M
+// multiply-adds (64 x 64 results of a 128 x 128 tile's wavefront need a third more).
+// The sum runs in steps of 64 through two buffers, filled by loads that go to LDS
+// directly, in whole cache lines (steps of 32 in four buffers asked the L2 for half
+// lines and took a tenth longer).  A step has four phases of eight matrix instructions;
+// every two of them go with reads of the phase to come or with a load, so that LDS and
+// the loads work beside the matrix cores.  Before the last phase the wavefronts meet:
+// by then this step's buffer has been read, and the next one's loads are there.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,65 +21,71 @@ namespace {
 constexpr int kSide = 256, kDepth = 64;
 constexpr int kBuffer = kSide * kDepth * 2;  // bytes of one operand's step
 
-__device__ __forceinline__ int swap_of(int k) { return 2 * ((k & 3) | (((k >> 3) & 1) << 2)); }
+__device__ __forceinline__ int swap_of(int k) { return 2 * (((k & 3) << 1) | ((k >> 3) & 1)); }
 
 // One operand's way into LDS.  In rows: 256 rows of 64 elements, 16-byte chunk c of
-// row r at place c ^ (r & 7).  In columns: 64 rows of 256, chunk c of row k at place
-// c ^ swap_of(k).  Both spread every wavefront's reads over all banks.
-//
-// A wavefront's four loads differ by a scalar: registers are short here, so a load has
-// its own resource and the lanes' offsets are common (in columns to loads 0, 2 and
-// 1, 3, whose chunks change places differently).
+// row r at place c ^ ((r >> 1) & 7).  In columns: 64 rows of 256, chunk c of row k at
+// place c ^ swap_of(k).  Both spread every wavefront's reads over all banks.  Each
+// wavefront has four loads a step, whose resources move with the steps: a full step
+// costs a few scalar instructions.
 template <bool Cols>
-struct WidePanel {
-  const char* base;  // of this wavefront's load 0
-  int64_t step;      // bytes from one step in k to the next
-  int32_t next;      // and from one load to the next (in columns to the next but one)
-  int32_t voff[Cols ? 2 : 1];
-  int at_k;          // the first k of this lane's chunk in load 0 (in columns 2 more each load)
-  int rows;          // in rows: those left from load 0 on
+struct Feeder {
+  uint64_t base[4];    // of the loads
+  uint32_t bytes[4];   // of their resources in a full step: the last valid row's end
+  int64_t step;        // bytes from one step in k to the next
+  int32_t voff[2];     // of the even and the odd loads
+  int at_k;            // the first k of this lane's chunk in load 0
+  int left;            // elements of the sum from here on
 
   __device__ __forceinline__ void init(const uint16_t* data, int64_t ld, int first, int count, int lane, int wave) {
+    const int32_t row = static_cast<int32_t>(2 * ld);
     if constexpr (Cols) {
-      base = reinterpret_cast<const char*>(data + first + wave * 8 * ld);
       step = 2 * kDepth * ld;
-      next = static_cast<int32_t>(8 * ld);
       at_k = wave * 8 + (lane >> 5);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int c = (lane & 31) ^ swap_of(at_k + 2 * u);
-        voff[u] = first + 8 * c < count ? static_cast<int32_t>(2 * (((lane >> 5) + 2 * u) * ld + 8 * c)) : kOutOfRange;
+        voff[u] = first + 8 * c < count ? ((lane >> 5) + 2 * u) * row + 16 * c : kOutOfRange;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        base[u] = reinterpret_cast<uint64_t>(data + first + (wave * 8 + (u & 2) * 2) * ld);
+        bytes[u] = 0x7FFFFFFFu;
       }
     } else {
-      base = reinterpret_cast<const char*>(data + (first + wave * 32) * ld);
       step = 2 * kDepth;
-      next = static_cast<int32_t>(16 * ld);
-      at_k = 8 * ((lane & 7) ^ (lane >> 3));
-      voff[0] = static_cast<int32_t>(2 * ((lane >> 3) * ld + at_k));
-      rows = count - first - wave * 32;
+      at_k = 8 * ((lane & 7) ^ (lane >> 4));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) voff[u] = (lane >> 3) * row + 2 * (at_k ^ (32 * u));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int from = first + wave * 32 + 8 * u, more = count - from < 8 ? count - from : 8;
+        base[u] = reinterpret_cast<uint64_t>(data + from * ld);
+        bytes[u] = more > 0 ? (more - 1) * row + 2 * kDepth : 0;
+      }
     }
   }
-  // Loads the elements from k0 = 64 tile on, zero past the sum's end `k` and the last
-  // row, to LDS address `lds`.
-  __device__ __forceinline__ void stage(int64_t offset, int tile, int k, uint32_t lds, int wave) const {
-    const char* from = base + offset + tile * step;
-    const int left = k - tile * kDepth;
+  // Moves to step t of a sum of k elements, `offset` bytes further on.
+  __device__ __forceinline__ void go(int64_t offset, int t, int k) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      int32_t at, records;
-      if constexpr (Cols) {
-        at = at_k + 2 * u < left ? voff[u & 1] : kOutOfRange;
-        records = 0x7FFFFFFF;
-      } else {
-        // The last valid row's last valid element of this step ends the resource.
-        const int more = rows - 8 * u < 8 ? rows - 8 * u : 8;
-        at = at_k < left ? voff[0] : kOutOfRange;
-        records = more > 0 ? (more - 1) * (next >> 3) + 2 * (left < kDepth ? left : kDepth) : 0;
-      }
-      U32x4 rs = rsrc_words(from + static_cast<int64_t>(next) * (Cols ? u >> 1 : u));
-      rs[2] = static_cast<uint32_t>(records);
-      lds_load16(rs, lds + (wave * 4 + u) * 1024, at, 0);
+    for (int u = 0; u < 4; ++u) base[u] += offset + t * step;
+    left = k - t * kDepth;
+  }
+  // Loads load u of this step to LDS address `lds`, zero past the sum's end and the last row.
+  __device__ __forceinline__ void stage(int u, uint32_t lds) const {
+    U32x4 rs{static_cast<uint32_t>(base[u]), static_cast<uint32_t>(base[u] >> 32) & 0xFFFFu, bytes[u], 0x00020000u};
+    if (__builtin_expect(left >= kDepth, 1)) {
+      lds_load16(rs, lds, voff[u & 1], 0);
+    } else {
+      if (!Cols) rs[2] = bytes[u] > 0 ? bytes[u] - 2 * (kDepth - left) : 0;
+      const int k = Cols ? at_k + 2 * u : at_k ^ (32 * (u & 1));
+      lds_load16(rs, lds, k < left ? voff[u & 1] : kOutOfRange, 0);
     }
+  }
+  __device__ __forceinline__ void advance() {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) base[u] += step;
+    left -= kDepth;
   }
 };
 
@@ -86,67 +93,39 @@ typedef short S16x4 __attribute__((ext_vector_type(4)));
 using LdsShorts = __attribute__((address_space(3))) S16x4;
 using LdsBytes = __attribute__((address_space(3))) char;
 
-// Where a lane finds its part of an operand: 8 elements k = 32 kk + 8 (lane / 16) + 0..7
-// of row (column) first + 16 i + lane % 16, `first` a multiple of 64.
+// Where a lane finds its part of an operand: 8 elements k = 16 kk + 8 (lane / 32) + 0..7
+// of row (column) first + 32 i + lane % 32, `first` a multiple of 64.
 template <bool Cols>
 struct Finder {
   uint32_t at;
   __device__ __forceinline__ Finder(uint32_t lds, int first, int lane) {
-    const int i = lane & 15, g = lane >> 4;
     if constexpr (Cols) {
-      const int k = 8 * g + (i >> 2);
-      at = lds + k * (2 * kSide) + (((first >> 4) ^ (swap_of(k) >> 1)) << 5) + (((i & 3) >> 1) << 4) + ((i & 1) << 3);
+      const int i = lane & 15, g = lane >> 4;
+      const int k = 8 * (g >> 1) + (i >> 2), c = (first >> 4) + (g & 1);
+      at = lds + k * (2 * kSide) + ((c ^ (swap_of(k) >> 1)) << 5) + (((i & 3) >> 1) << 4) + ((i & 1) << 3);
     } else {
-      at = lds + (first + i) * (2 * kDepth) + ((g ^ (i & 7)) << 4);
+      const int r = lane & 31;
+      at = lds + (first + r) * (2 * kDepth) + (((lane >> 5) ^ ((r >> 1) & 7)) << 4);
     }
   }
   template <int Buffer>
   __device__ __forceinline__ U32x4 read(int i, int kk) const {
     U32x4 w;
-    uint32_t at = this->at;
-    if constexpr (Cols) asm volatile("" : "+v"(at));  // formed anew for each read rather than kept in a register for each place
     if constexpr (Cols) {
-      auto* p = reinterpret_cast<LdsBytes*>(at ^ (i << 5)) + Buffer * kBuffer + kk * 32 * 2 * kSide;
+      uint32_t at = this->at;
+      asm volatile("" : "+v"(at));  // formed anew for each read rather than kept in a register for each place
+      auto* p = reinterpret_cast<LdsBytes*>(at ^ (i << 6)) + Buffer * kBuffer + kk * 16 * 2 * kSide;
       const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShorts*)p);
       const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShorts*)(p + 4 * 2 * kSide));
       const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
       w = U32x4{l.x, l.y, h.x, h.y};
     } else {
-      auto* p = reinterpret_cast<LdsBytes*>(at ^ (kk << 6)) + Buffer * kBuffer + i * 16 * 2 * kDepth;
+      auto* p = reinterpret_cast<LdsBytes*>(at ^ (kk << 5)) + Buffer * kBuffer + i * 32 * 2 * kDepth;
       w = *(__attribute__((address_space(3))) U32x4*)p;
     }
     return w;
   }
 };
-
-// Rows 64 Half .. + 63 of the wavefront's 128: B's rows go in as the instruction's rows,
-// so that a lane holds four neighbouring n of one m.
-template <typename E, int Half>
-__device__ __forceinline__ void multiply(Floats4 (&acc)[8][4], const U32x4 (&x)[4], const U32x4 (&y)[4]) {
-  __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[Half * 4 + i][j] = mfma16<E>(y[j], x[i], acc[Half * 4 + i][j]);
-  __builtin_amdgcn_s_setprio(0);
-}
-
-template <int Buffer, int First, bool Cols>
-__device__ __forceinline__ void read_four(const Finder<Cols>& f, int kk, U32x4 (&to)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) to[i] = f.template read<Buffer>(First + i, kk);
-}
-
-// One LDS read of the next phase beside each few matrix instructions of this one.
-template <int Reads>
-__device__ __forceinline__ void interleave() {
-#pragma unroll
-  for (int i = 0; i < Reads; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x8, 16 / Reads, 0);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-}
 
 __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
@@ -154,54 +133,91 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
-template <typename T, bool ACols, bool BCols>
-struct Work {
-  const ProductArgs& p;
-  const Steps<T> steps;
-  int count, wave;
+// An operand's steps of a slice: the next one to load.
+template <typename T, bool Cols>
+struct Feed {
+  Feeder<Cols> f, start;
+  Steps<T, kDepth> steps;
+  int next;
   uint32_t lds;
-  WidePanel<ACols> a;
-  WidePanel<BCols> b;
 
-  __device__ __forceinline__ void stage(int s, int buffer) const {
+  __device__ __forceinline__ void place(const ProductArgs& p, bool of_a) {
     int64_t oa, ob;
     int t;
-    steps.place(p, steps.begin + s, t, oa, ob);
-    a.stage(oa, t, p.k, lds + buffer * kBuffer, wave);
-    b.stage(ob, t, p.k, lds + (2 + buffer) * kBuffer, wave);
+    steps.place(p, next, t, oa, ob);
+    f = start;
+    f.go(of_a ? oa : ob, t, p.k);
+  }
+  __device__ __forceinline__ void stage(int u, int buffer) const { f.stage(u, lds + buffer * kBuffer + u * 1024); }
+  __device__ __forceinline__ void advance(const ProductArgs& p, bool of_a) {
+    ++next;
+    f.advance();
+    if constexpr (T::code == F32::code) {  // the next pair of planes begins
+      if (f.left <= 0 && next < steps.end) place(p, of_a);
+    }
   }
 };
 
-// Step s, in buffer B; x[0] and y[0] hold its first operands, and the next one's after it.
-// (Registers are passed by reference: captured ones went to memory.)
+// Two matrix instructions: B's rows go in as their rows, so that a lane holds four
+// neighbouring n of one m.
+template <typename E>
+__device__ __forceinline__ void two(Floats16 (&acc)[2], U32x4 x, U32x4 y0, U32x4 y1) {
+  acc[0] = mfma32<E>(y0, x, acc[0]);
+  acc[1] = mfma32<E>(y1, x, acc[1]);
+}
+
+template <int Buffer, bool Cols>
+__device__ __forceinline__ void read_two(const Finder<Cols>& f, int i, int kk, U32x4* to) {
+  to[0] = f.template read<Buffer>(i, kk);
+  to[1] = f.template read<Buffer>(i + 1, kk);
+}
+
+// Step s, in buffer B.  x0 and y hold A's rows 0..63 and B's rows of k = 0..31 of it
+// ([2 (k / 16) + tile]), and after it those of the next step.  (Registers are passed
+// by reference: captured ones went to memory.)
 template <int B, typename T, bool ACols, bool BCols>
-__device__ __forceinline__ void step(const Work<T, ACols, BCols>& w, const Finder<ACols>& fa, const Finder<BCols>& fb,
-                                     int s, Floats4 (&acc)[8][4], U32x4 (&x0)[4], U32x4 (&x1)[4], U32x4 (&y0)[4],
-                                     U32x4 (&y1)[4]) {
+__device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols>& a, Feed<T, BCols>& b,
+                                     const Finder<ACols>& fa, const Finder<BCols>& fb, int s, int count,
+                                     Floats16 (&acc)[4][2], U32x4 (&x0)[4], U32x4 (&x1)[4], U32x4 (&y)[4],
+                                     U32x4 (&z)[4]) {
   using E = std::conditional_t<T::code == F16::code, F16, BF16>;
-  constexpr int ra = ACols ? 8 : 4, rab = ra + (BCols ? 8 : 4);
-  read_four<B, 4>(fa, 0, x1);
-  multiply<E, 0>(acc, x0, y0);
-  interleave<ra>();
-  read_four<B, 0>(fa, 1, x0);
-  read_four<B, 0>(fb, 1, y1);
-  multiply<E, 1>(acc, x1, y0);
-  interleave<rab>();
-  read_four<B, 4>(fa, 1, x1);
-  multiply<E, 0>(acc, x0, y1);
-  interleave<ra>();
-  // This buffer has been read; the next one's loads are a step old.
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < 2) read_two<B>(fa, 2, i, x1 + 2 * i);
+    if (s + 1 < count) b.stage(i, B ^ 1);
+    two<E>(acc[i & 1], x0[i], y[i & 2], y[(i & 2) + 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (s + 1 < count) b.advance(p, false);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < 2) {
+      read_two<B>(fa, 0, 2 + i, x0 + 2 * i);
+      read_two<B>(fb, 0, 2 + i, z + 2 * i);
+    }
+    two<E>(acc[2 + (i & 1)], x1[i], y[i & 2], y[(i & 2) + 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < 2) read_two<B>(fa, 2, 2 + i, x1 + 2 * i);
+    two<E>(acc[i & 1], x0[i], z[i & 2], z[(i & 2) + 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   wait_lds();
   wait_vm<0>();
   meet();
-  if (s + 2 < w.count) w.stage(s + 2, B);
-  __builtin_amdgcn_sched_barrier(0);
-  if (s + 1 < w.count) {
-    read_four<B ^ 1, 0>(fa, 0, x0);
-    read_four<B ^ 1, 0>(fb, 0, y0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < 2 && s + 1 < count) {
+      read_two<B ^ 1>(fa, 0, i, x0 + 2 * i);
+      read_two<B ^ 1>(fb, 0, i, y + 2 * i);
+    }
+    if (s + 2 < count) a.stage(i, B);
+    two<E>(acc[2 + (i & 1)], x1[i], z[i & 2], z[(i & 2) + 1]);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  multiply<E, 1>(acc, x1, y1);
-  interleave<rab>();
+  if (s + 2 < count) a.advance(p, true);
 }
 
 template <typename T, bool ACols, bool BCols>
@@ -211,38 +227,66 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = tile_of(p, blockIdx.x);
   const int m0 = tile.m * kSide, n0 = tile.n * kSide, slice = blockIdx.y;
-  Work<T, ACols, BCols> w{p, Steps<T>(p, slice), 0, wave, lds_address(lds)};
-  w.count = w.steps.end - w.steps.begin;
-  w.a.init(p.a, p.lda, m0, p.m, lane, wave);
-  w.b.init(p.b, p.ldb, n0, p.n, lane, wave);
+  const Steps<T, kDepth> steps(p, slice);
+  const int count = steps.end - steps.begin;
+  Feed<T, ACols> a{{}, {}, steps, steps.begin, lds_address(lds) + wave * 4096};
+  Feed<T, BCols> b{{}, {}, steps, steps.begin, lds_address(lds) + 2 * kBuffer + wave * 4096};
+  a.start.init(p.a, p.lda, m0, p.m, lane, wave);
+  b.start.init(p.b, p.ldb, n0, p.n, lane, wave);
   const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
-  const Finder<ACols> fa(w.lds, wm, lane);
-  const Finder<BCols> fb(w.lds + 2 * kBuffer, wn, lane);
-  Floats4 acc[8][4];
+  const Finder<ACols> fa(lds_address(lds), wm, lane);
+  const Finder<BCols> fb(lds_address(lds) + 2 * kBuffer, wn, lane);
+  Floats16 acc[4][2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = Floats4{0.f, 0.f, 0.f, 0.f};
-  U32x4 x0[4], x1[4], y0[4], y1[4];  // A's rows in halves of 64, B's 64
-  if (w.count > 0) {
-    w.stage(0, 0);
-    if (w.count > 1) {
-      w.stage(1, 1);
-      wait_vm<8>();
-    } else {
-      wait_vm<0>();
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  U32x4 x0[4], x1[4], y[4], z[4];
+  if (count > 0) {
+    a.place(p, true);
+    b.place(p, false);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      a.stage(u, 0);
+      b.stage(u, 0);
     }
+    a.advance(p, true);
+    b.advance(p, false);
+    wait_vm<0>();
     meet();
-    read_four<0, 0>(fa, 0, x0);
-    read_four<0, 0>(fb, 0, y0);
-    for (int s = 0; s < w.count; s += 2) {
-      step<0>(w, fa, fb, s, acc, x0, x1, y0, y1);
-      if (s + 1 < w.count) step<1>(w, fa, fb, s + 1, acc, x0, x1, y0, y1);
+    if (count > 1) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a.stage(u, 1);
+      a.advance(p, true);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      read_two<0>(fa, 0, i, x0 + 2 * i);
+      read_two<0>(fb, 0, i, y + 2 * i);
+    }
+    for (int s = 0; s < count; s += 2) {
+      step<0>(p, a, b, fa, fb, s, count, acc, x0, x1, y, z);
+      if (s + 1 < count) step<1>(p, a, b, fa, fb, s + 1, count, acc, x0, x1, y, z);
     }
   }
   __syncthreads();  // the buffers have been read: each wavefront takes 16 KB of them
-  finish_block<T>(p, slice, acc, lds + wave * 16384, m0 + wm, n0 + wn, lane);
-  finish_block<T>(p, slice, acc + 4, lds + wave * 16384, m0 + wm + 64, n0 + wn, lane);
+  char* area = lds + wave * 16384;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const Floats16& v = acc[2 * half + i][j];
+          park(area, 32 * i + (lane & 31), 8 * j + 2 * q + (lane >> 5),
+               Floats4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+        }
+    finish_parked<T>(p, slice, area, m0 + wm + 64 * half, n0 + wn, lane);
+  }
 }
 
 template <typename T>
