@@ -46,6 +46,7 @@ KERNEL_SOURCES = [
     "linear.hip",
     "linear_product.hip",
     "linear_wide.hip",
+    "linear_narrow.hip",
     "grad_clip.hip",
     "fh_capi.cpp",
 ]

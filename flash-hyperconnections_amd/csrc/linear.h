@@ -204,20 +204,20 @@ __device__ __forceinline__ void finish_eight(const ProductArgs& p, int slice, in
   store_eight(e, static_cast<S*>(p.out) + at, left);
 }
 
-// 64 x 64 results of a wavefront on their way out through 16 KB of its own LDS, so that
-// eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row r is at
+// Rows x 64 results of a wavefront on their way out through 256 bytes a row of its own
+// LDS, so that eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row r is at
 // place c ^ (r & 15), which spreads reads and writes over the banks.  (Stored from the
 // accumulators, a lane's four columns alone, a product of 16384 x 4096 x 16384 with
 // gelu spent a third of its time here.)
 __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
   *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;
 }
-template <typename T>
+template <typename T, int Rows>
 __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
                                               int lane) {
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
 #pragma unroll 1
-  for (int it = 0; it < 8; ++it) {
+  for (int it = 0; it < Rows / 8; ++it) {
     const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
     float v[8];
     __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
@@ -293,10 +293,20 @@ struct Steps {
   }
 };
 
+// s_waitcnt vmcnt(N) for N up to 63.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt immediate");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
 // floats.  `dtype` is the output's; FP32 runs on bf16 planes.
-void plan_product(ProductArgs& p, int dtype);
+void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
+// The same for a product with at most 32 rows or columns; false for others.
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 
 }  // namespace fh

@@ -190,7 +190,7 @@ hipError_t multiply(ProductArgs& p, const Operand16& a, const Operand16& b, int 
   p.b = b.data;
   p.ldb = b.ld;
   p.plane_b = b.plane;
-  plan_product(p, dtype);
+  plan_product(p, dtype, a_cols, b_cols);
   if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
   return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream);
 }

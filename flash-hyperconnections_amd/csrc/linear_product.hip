@@ -1,132 +1,124 @@
-// Matrix products of the linear layer, in 128 x 128 tiles on the matrix cores.
+// Matrix products of the linear layer in 128 x 128 tiles, where tiles of 256 are too
+// few to fill the card, and the joining of sums in several slices.
+//
+// Such products are short: what costs is the time from one step's loads to the next.
+// So a compute unit holds one workgroup, of eight wavefronts with 32 x 64 results each,
+// whose four buffers keep three steps of 64 on their way (two workgroups with one step
+// each on its way took twice as long a step).  The wavefronts meet once a step.
 #include <algorithm>
 #include <type_traits>
 
-#include "linear.h"
+#include "linear_tiles.h"
 
 namespace fh {
 namespace {
 
-typedef short S16x4 __attribute__((ext_vector_type(4)));
+constexpr int kTile = 128, kRing = 4;
+constexpr int kBuffer = kTile * kStep * 2;  // bytes of one operand's step
 
-constexpr int kTile = 128, kDepth = 64;
-constexpr int kPanel = kTile * kDepth;  // elements of one operand's tile
-
-// Exchange of 16-byte chunks along an LDS row of a tile in columns, by the row k.
-__device__ __forceinline__ int swap_of(int k) { return 2 * ((k & 3) | (((k >> 3) & 1) << 2)); }
-
-// One operand's way through LDS.  In rows: 128 rows of 64 elements, chunk c of row
-// r at place c ^ (r & 7).  In columns: 64 rows of 128 elements, chunk c of row k at
-// place c ^ swap_of(k).
-template <bool Cols>
-struct Panel {
-  U32x4 rsrc;
-  int32_t voff[4];   // of the wavefront's four loads
-  int at_k[4];       // the first k of each lane's chunk, in the tile
-  int64_t step;      // bytes from one tile in k to the next
-  const char* base;
-
-  __device__ __forceinline__ void init(const uint16_t* data, int64_t ld, int first, int count, int lane, int wave) {
-    base = reinterpret_cast<const char*>(data + (Cols ? static_cast<int64_t>(first) : first * ld));
-    step = 2 * (Cols ? kDepth * ld : kDepth);
+// k = 32 half .. + 31 of the step in buffer R; y: [2 kk + tile].
+template <int R, bool ACols, bool BCols>
+__device__ __forceinline__ void read_half(const Finder<ACols, kTile>& fa, const Finder<BCols, kTile>& fb, int half,
+                                          U32x4 (&x)[2], U32x4 (&y)[4]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if constexpr (Cols) {
-        const int k = (wave * 4 + u) * 4 + (lane >> 4), c = (lane & 15) ^ swap_of(k);
-        voff[u] = first + 8 * c < count ? static_cast<int32_t>(2 * (k * ld + 8 * c)) : kOutOfRange;
-        at_k[u] = k;
-      } else {
-        const int r = (wave * 4 + u) * 8 + (lane >> 3), c = (lane & 7) ^ (r & 7);
-        const int row = first + r < count ? r : count - 1 - first;
-        voff[u] = static_cast<int32_t>(2 * (row * ld + 8 * c));
-        at_k[u] = 8 * c;
-      }
-    }
+  for (int kk = 0; kk < 2; ++kk) {
+    x[kk] = fa.read(R * kBuffer, 0, 2 * half + kk);
+    y[2 * kk] = fb.read(R * kBuffer, 0, 2 * half + kk);
+    y[2 * kk + 1] = fb.read(R * kBuffer, 1, 2 * half + kk);
   }
-  // Loads the tile from k0 on into `lds`; k is the sum's length.
-  __device__ __forceinline__ void stage(int64_t offset, int tile, int k, uint32_t lds, int wave) const {
-    const U32x4 rs = rsrc_words(base + offset + tile * step);
-    const int left = k - tile * kDepth;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      lds_load16(rs, lds + (wave * 4 + u) * 1024, at_k[u] < left ? voff[u] : kOutOfRange, 0);
-  }
-};
+}
 
-// Lane's 8 elements k = 32 kk + 8 (lane / 16) + 0..7 of row (column) first + lane % 16.
-template <bool Cols>
-__device__ __forceinline__ U32x4 fragment(const uint16_t* tile, int first, int kk, int lane) {
-  U32x4 w;
-  if constexpr (Cols) {
-    const int i = lane & 15, k = kk * 32 + 8 * (lane >> 4) + (i >> 2);
-    const int col = first + 4 * (i & 3);
-    const uint16_t* p = tile + k * kTile + (((col >> 3) ^ swap_of(k)) << 3) + (col & 7);
-    using Lds = __attribute__((address_space(3))) S16x4;
-    const S16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)p);
-    const S16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + 4 * kTile));
-    __builtin_memcpy(&w, &lo, 8);
-    __builtin_memcpy(reinterpret_cast<char*>(&w) + 8, &hi, 8);
-  } else {
-    const int r = first + (lane & 15), c = kk * 4 + (lane >> 4);
-    w = *reinterpret_cast<const U32x4*>(tile + r * kDepth + ((c ^ (r & 7)) << 3));
+// B's rows as the instruction's rows: a lane then holds four neighbouring n of one m.
+template <typename E>
+__device__ __forceinline__ void multiply(Floats16 (&acc)[2], U32x4 x, U32x4 y0, U32x4 y1) {
+  acc[0] = mfma32<E>(y0, x, acc[0]);
+  acc[1] = mfma32<E>(y1, x, acc[1]);
+}
+
+// The step in buffer R.  x0 and y0 hold its first half, and after it the next one's.
+template <int R, typename T, bool ACols, bool BCols>
+__device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols, kTile>& a, Feed<T, BCols, kTile>& b,
+                                     const Finder<ACols, kTile>& fa, const Finder<BCols, kTile>& fb,
+                                     Floats16 (&acc)[2], U32x4 (&x0)[2], U32x4 (&x1)[2], U32x4 (&y0)[4],
+                                     U32x4 (&y1)[4]) {
+  using E = std::conditional_t<T::code == F16::code, F16, BF16>;
+  read_half<R>(fa, fb, 1, x1, y1);
+  multiply<E>(acc, x0[0], y0[0], y0[1]);
+  multiply<E>(acc, x0[1], y0[2], y0[3]);
+  __builtin_amdgcn_sched_barrier(0);
+  // This step's buffer has been read, and the next one's loads are there once only the
+  // four of each of the two steps behind it are on their way.
+  wait_lds();
+  wait_loads<8>();
+  meet();
+  read_half<(R + 1) % kRing>(fa, fb, 0, x0, y0);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    a.stage(u, R * kBuffer);
+    b.stage(u, R * kBuffer);
+    multiply<E>(acc, x1[u], y1[2 * u], y1[2 * u + 1]);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  return w;
+  a.advance(p, true);
+  b.advance(p, false);
 }
 
 template <typename T, bool ACols, bool BCols>
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
-  using E = std::conditional_t<T::code == F16::code, F16, BF16>;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[2][2][kPanel];
+__global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kRing * kBuffer];  // A's ring, B's ring
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = tile_of(p, blockIdx.x);
   const int m0 = tile.m * kTile, n0 = tile.n * kTile, slice = blockIdx.y;
-  Panel<ACols> a;
-  Panel<BCols> b;
-  a.init(p.a, p.lda, m0, p.m, lane, wave);
-  b.init(p.b, p.ldb, n0, p.n, lane, wave);
-  const Steps<T, kDepth> steps(p, slice);
-  const auto stage = [&](int step, int buffer) {
-    int64_t oa, ob;
-    int t;
-    steps.place(p, step, t, oa, ob);
-    a.stage(oa, t, p.k, lds_address(lds[buffer][0]), wave);
-    b.stage(ob, t, p.k, lds_address(lds[buffer][1]), wave);
-  };
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  Floats4 acc[4][4];
+  const Steps<T, kStep> steps(p, slice);
+  const int count = steps.end - steps.begin;
+  Feed<T, ACols, kTile> a{{}, {}, steps, steps.begin, lds_address(lds) + wave * 2048};
+  Feed<T, BCols, kTile> b{{}, {}, steps, steps.begin, lds_address(lds) + kRing * kBuffer + wave * 2048};
+  a.start.init(p.a, p.lda, m0, p.m, p.k, lane, wave);
+  b.start.init(p.b, p.ldb, n0, p.n, p.k, lane, wave);
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
+  const Finder<ACols, kTile> fa(lds_address(lds), wm, lane);
+  const Finder<BCols, kTile> fb(lds_address(lds) + kRing * kBuffer, wn, lane);
+  Floats16 acc[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = Floats4{0.f, 0.f, 0.f, 0.f};
-  if (steps.begin < steps.end) stage(steps.begin, 0);
-  for (int s = steps.begin; s < steps.end; ++s) {
-    const int buffer = (s - steps.begin) & 1;
-    wait_vm<0>();
-    __syncthreads();  // the tile is there, and the other buffer has been read
-    if (s + 1 < steps.end) stage(s + 1, buffer ^ 1);
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+  if (count > 0) {
+    a.place(p, true);
+    b.place(p, false);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      U32x4 fa[4], fb[4];
+    for (int s = 0; s < kRing; ++s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = fragment<ACols>(lds[buffer][0], wm + 16 * i, kk, lane);
-        fb[i] = fragment<BCols>(lds[buffer][1], wn + 16 * i, kk, lane);
+      for (int u = 0; u < 2; ++u) {
+        a.stage(u, s * kBuffer);
+        b.stage(u, s * kBuffer);
       }
-      // B's rows as the instruction's rows: a lane then holds four neighbouring n of one m.
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<E>(fb[j], fa[i], acc[i][j]);
+      a.advance(p, true);
+      b.advance(p, false);
+    }
+    wait_loads<4 * (kRing - 1)>();
+    meet();
+    U32x4 x0[2], x1[2], y0[4], y1[4];
+    read_half<0>(fa, fb, 0, x0, y0);
+    // Loads and reads go on past the last step, of zeros.
+    for (int s = 0; s < count; s += 4) {
+      step<0>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 1 < count) step<1>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 2 < count) step<2>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 3 < count) step<3>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
     }
   }
-  __syncthreads();  // the buffers have been read: each wavefront takes 16 KB of them
-  char* area = reinterpret_cast<char*>(lds) + wave * 16384;
+  wait_loads<0>();
+  __syncthreads();  // the buffers have been read: each wavefront takes 8 KB of them
+  char* area = lds + wave * 8192;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) park(area, 16 * i + (lane & 15), 4 * j + (lane >> 4), acc[i][j]);
-  finish_parked<T>(p, slice, area, m0 + wm, n0 + wn, lane);
+    for (int q = 0; q < 4; ++q)
+      park(area, lane & 31, 8 * j + 2 * q + (lane >> 5),
+           Floats4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]});
+  finish_parked<T, 32>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // Adds the slices in order and finishes.
@@ -151,7 +143,7 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
 
 template <typename T>
 hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(256);
+  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
   if (!a_cols && !b_cols) product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
   if (!a_cols && b_cols) product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
   if (a_cols && b_cols) product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
@@ -175,25 +167,38 @@ void set_tiles(ProductArgs& p, int side) {
 
 }  // namespace
 
-void plan_product(ProductArgs& p, int dtype) {
-  const int64_t steps = static_cast<int64_t>((p.k + kDepth - 1) / kDepth) * (dtype == F32::code ? 6 : 1);
+void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
+  if (plan_narrow_product(p, dtype, a_cols, b_cols)) return;
+  const int64_t steps = static_cast<int64_t>((p.k + kStep - 1) / kStep) * (dtype == F32::code ? 6 : 1);
   const int64_t units = compute_units();
-  // Tiles of 256 once they keep nearly all compute units at work to the end.
-  set_tiles(p, 256);
-  p.slices = 1;
-  const int64_t wide = static_cast<int64_t>(p.tiles_m) * p.tiles_n, rounds = (wide + units - 1) / units;
-  if (wide * 10 >= rounds * units * 8 && p.m > 128 && p.n > 128) return;
+  const auto rounds = [&](int64_t groups) { return static_cast<double>((groups + units - 1) / units); };
+  // Microseconds, measured: a workgroup of a tile of 256 takes 5 and 1.15 a step of 64, one of a tile
+  // of 128 takes 3 and 0.4; slices cost a launch and their sums' way to memory and back.
   set_tiles(p, kTile);
-  // Slices of at least eight steps until two workgroups a compute unit have work.
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * units / tiles, steps / 8)));
+  const double results = static_cast<double>(p.m) * p.n;
+  double best = 0.0;
+  for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
+    const double us = rounds(tiles * s) * (3.0 + 0.4 * static_cast<double>((steps + s - 1) / s)) +
+                      (s > 1 ? 4.0 + results * 4e-6 * static_cast<double>(s + 1) / 4.0 : 0.0);
+    if (s == 1 || us < best) {
+      best = us;
+      p.slices = static_cast<int>(s);
+    }
+  }
+  ProductArgs wide = p;
+  set_tiles(wide, 256);
+  wide.slices = 1;
+  if (rounds(static_cast<int64_t>(wide.tiles_m) * wide.tiles_n) * (5.0 + 1.15 * static_cast<double>(steps)) < best)
+    p = wide;
 }
 
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
   if (p.side == 256) return launch_wide_product(p, dtype, a_cols, b_cols, stream);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const hipError_t err = run<T>(p, a_cols, b_cols, stream);
+    const hipError_t err = p.side == kTile ? run<T>(p, a_cols, b_cols, stream)
+                                           : launch_narrow_product(p, dtype, a_cols, b_cols, stream);
     return err != hipSuccess || p.slices == 1 ? err : join<T>(p, stream);
   });
 }

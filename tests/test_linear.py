@@ -124,6 +124,17 @@ def test_sizes(m, k, n, dtype):
     _compare(x, w, b, res if (m + n) % 2 else None, act, g)
 
 
+# Enough tiles of 256 for y, dx or dW, with ragged edges in every dimension.
+LARGE = [(4000, 203, 3990), (3990, 4001, 263), (264, 4000, 3990)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_large_sizes(m, k, n, dtype):
+    _compare(*_inputs(m, k, n, dtype, seed=m + k)[:4], "gelu" if k == 203 else None, _inputs(m, k, n, dtype)[4])
+
+
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("act", ACTS)
