@@ -47,6 +47,7 @@ KERNEL_SOURCES = [
     "linear_product.hip",
     "linear_wide.hip",
     "linear_narrow.hip",
+    "linear_f32.hip",
     "grad_clip.hip",
     "fh_capi.cpp",
 ]

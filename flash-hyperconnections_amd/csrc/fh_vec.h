@@ -9,10 +9,16 @@ namespace fh {
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(typename T::storage));
 
-// Calls f.template operator()<T>() for the element type of `dtype`.
+// Calls f with the element type of `dtype`, a 16-bit one in the second form.
 template <typename F>
 hipError_t with_type(int dtype, F f) {
   if (dtype == F32::code) return f(F32{});
+  if (dtype == BF16::code) return f(BF16{});
+  return f(F16{});
+}
+
+template <typename F>
+hipError_t with_half_type(int dtype, F f) {
   if (dtype == BF16::code) return f(BF16{});
   return f(F16{});
 }

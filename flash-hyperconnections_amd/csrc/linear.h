@@ -14,12 +14,11 @@ typedef float Floats4 __attribute__((ext_vector_type(4)));
 
 // D[m][n] = sum over k of A[m][k] B[n][k] and what follows it.  An operand is in
 // rows (k contiguous, rows ld elements apart) or in columns (m or n contiguous, a
-// row for each k).  FP32 operands come as three bf16 planes, `plane` elements
-// apart, whose sum they are.
+// row for each k).  16-bit operands have 16-byte aligned rows of whole 16-byte
+// vectors; FP32 ones any rows.
 struct ProductArgs {
-  const uint16_t *a, *b;
+  const void *a, *b;
   int64_t lda, ldb;
-  int64_t plane_a, plane_b;
   int m, n, k;
   int tiles_m, tiles_n;
   int side;              // of a tile
@@ -269,27 +268,14 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int block) {
   return {first + in % high, in / high};
 }
 
-// The steps of Depth in k that a slice of a sum takes; for FP32 once for each product of
-// planes, the smallest first (those of 2^-24 and below are left out).
-template <typename T, int Depth>
+// The steps of Depth in k that a slice of a sum takes.
+template <int Depth>
 struct Steps {
-  int depth, begin, end;
+  int begin, end;
   __device__ __forceinline__ Steps(const ProductArgs& p, int slice) {
-    depth = (p.k + Depth - 1) / Depth;
-    const int64_t steps = static_cast<int64_t>(depth) * (T::code == F32::code ? 6 : 1);
+    const int64_t steps = (p.k + Depth - 1) / Depth;
     begin = static_cast<int>(steps * slice / p.slices);
     end = static_cast<int>(steps * (slice + 1) / p.slices);
-  }
-  // Step s: its place in k, and the planes' offsets in bytes.
-  __device__ __forceinline__ void place(const ProductArgs& p, int s, int& t, int64_t& oa, int64_t& ob) const {
-    t = s;
-    oa = ob = 0;
-    if constexpr (T::code == F32::code) {
-      const int pair = s / depth;
-      t = s - pair * depth;
-      oa = 2 * ((0x210100 >> (20 - 4 * pair)) & 15) * p.plane_a;
-      ob = 2 * ((0x012010 >> (20 - 4 * pair)) & 15) * p.plane_b;
-    }
   }
 };
 
@@ -301,11 +287,13 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
-// floats.  `dtype` is the output's; FP32 runs on bf16 planes.
+// floats.  `dtype` is the operands' and the output's.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 // The same for a product with at most 32 rows or columns; false for others.
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
+bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols);
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream);
+// 16-bit types.
 hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 

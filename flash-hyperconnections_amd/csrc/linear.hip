@@ -2,16 +2,13 @@
 //   z = x W^T + b,  y = act(z) + residual;
 //   dz = g act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz.
 //
-// The products take 16-bit operands whose rows are whole 16-byte vectors.  Others
-// are laid out anew first (prepare_kernel): padded rows for odd widths, and for
-// FP32 three bf16 planes a, b, c with x = a + b + c exactly (8 bits each, cut off,
-// so that nothing overflows).  Six of the nine products of planes make an FP32
-// product to about 2^-23; on the bf16 matrix instructions, sixteen times the rate
-// of the FP32 ones, they take less than half the FP32 instructions' time.
+// The products take 16-bit operands whose rows are 16-byte aligned and whole 16-byte
+// vectors; others are laid out anew first, in padded rows (prepare_kernel).  FP32
+// operands they take as they are.
 //
-// dz is formed by the same kernel on its way into such a layout, together with the
-// column sums that make db.  It is rounded to the storage type, as operands of
-// 16-bit products have to be; db adds the values before that rounding.
+// dz is formed by the same kernel, together with the column sums that make db.  It is
+// rounded to the storage type, as operands of 16-bit products have to be; db adds the
+// values before that rounding.
 #include <algorithm>
 
 #include "linear.h"
@@ -24,31 +21,12 @@ struct PrepareArgs {
   int64_t src_stride;
   const void* saved; // with an activation: [rows, cols] contiguous
   int act;
-  uint16_t* out;     // [rows, ld] (FP32: three planes of that), zero past cols; or null
+  void* out;         // [rows, ld], zero past cols; or null
   int64_t ld;
   float* partial;    // [gridDim.y, cols] column sums, or null
   int64_t rows;
   int cols;
 };
-
-__device__ __forceinline__ uint32_t top_half(float v) { return __float_as_uint(v) & 0xFFFF0000u; }
-
-// The three bf16 planes of a value, as dwords with the bits on top.  An infinity or
-// NaN goes into the last plane, which meets only the other operand's first, beside a
-// one in the first plane: inf x (second or third plane 0) would be NaN, where inf x b
-// is an infinity.
-__device__ __forceinline__ void planes_of(float v, uint32_t (&part)[3]) {
-  if (finite_f32(v)) {
-    part[0] = top_half(v);
-    const float r = v - __uint_as_float(part[0]);
-    part[1] = top_half(r);
-    part[2] = top_half(r - __uint_as_float(part[1]));
-  } else {
-    part[0] = 0x3F800000u | (__float_as_uint(v) & 0x80000000u);
-    part[1] = 0;
-    part[2] = v != v ? 0x7FC00000u : __float_as_uint(v);
-  }
-}
 
 // Four wavefronts, 64 V columns, rows blockIdx.y, + gridDim.y, ....
 template <typename T, bool Sums>
@@ -78,20 +56,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) sums[i] += c + i < a.cols ? f[i] : 0.f;
     }
-    if (a.out != nullptr && c < a.ld) {
-      if constexpr (T::code != F32::code) {
-        *reinterpret_cast<U32x4*>(a.out + row * a.ld + c) = rounded;
-      } else {
-        uint32_t part[4][3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) planes_of(c + i < a.cols ? f[i] : 0.f, part[i]);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const uint2 w = make_uint2((part[0][k] >> 16) | part[1][k], (part[2][k] >> 16) | part[3][k]);
-          *reinterpret_cast<uint2*>(a.out + (k * a.rows + row) * a.ld + c) = w;
-        }
-      }
-    }
+    if (a.out != nullptr && c < a.ld)
+      *reinterpret_cast<U32x4*>(static_cast<S*>(a.out) + row * a.ld + c) = rounded;
   }
   if constexpr (Sums) {
     __shared__ float area[4][V][64];
@@ -148,48 +114,43 @@ class Workspace {
 };
 
 // An operand as the products read it.
-struct Operand16 {
-  const uint16_t* data;
-  int64_t ld, plane;
+struct Laid {
+  const void* data;
+  int64_t ld;
 };
 
 constexpr int64_t kMostStride = int64_t{1} << 22;  // 256 rows of a tile within 2^31 bytes
 
 // Whether the products read [rows, cols] as it is.
 bool as_it_is(const void* data, int64_t stride, int64_t cols, int dtype) {
-  return dtype != F32::code && reinterpret_cast<uintptr_t>(data) % 16 == 0 && cols % 8 == 0 && stride % 8 == 0 &&
-         stride >= 0 && stride < kMostStride;
+  if (dtype == F32::code) return true;
+  return reinterpret_cast<uintptr_t>(data) % 16 == 0 && cols % 8 == 0 && stride % 8 == 0 && stride < kMostStride;
 }
 
 // `data` as it is, or laid out anew in the workspace.
-hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws,
-                   Operand16& got, hipStream_t stream) {
+hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws, Laid& got,
+                   hipStream_t stream) {
   if (as_it_is(data, stride, cols, dtype)) {
-    got = {static_cast<const uint16_t*>(data), stride, 0};
+    got = {data, stride};
     return hipSuccess;
   }
-  const int64_t ld = padded(cols);
-  uint16_t* out = ws.take<uint16_t>(rows * ld * (dtype == F32::code ? 3 : 1));
-  got = {out, ld, rows * ld};
-  if (ws.dry()) return hipSuccess;
   PrepareArgs p{};
   p.src = data;
   p.src_stride = stride;
-  p.out = out;
-  p.ld = ld;
+  p.ld = padded(cols);
+  p.out = ws.take<uint16_t>(rows * p.ld);
   p.rows = rows;
   p.cols = static_cast<int>(cols);
-  return launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
+  got = {p.out, p.ld};
+  return ws.dry() ? hipSuccess : launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
 }
 
-hipError_t multiply(ProductArgs& p, const Operand16& a, const Operand16& b, int dtype, bool a_cols, bool b_cols,
+hipError_t multiply(ProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols,
                     Workspace& ws, hipStream_t stream) {
   p.a = a.data;
   p.lda = a.ld;
-  p.plane_a = a.plane;
   p.b = b.data;
   p.ldb = b.ld;
-  p.plane_b = b.plane;
   plan_product(p, dtype, a_cols, b_cols);
   if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
   return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream);
@@ -199,7 +160,7 @@ hipError_t multiply(ProductArgs& p, const Operand16& a, const Operand16& b, int 
 
 hipError_t launch_linear(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
   Workspace ws(workspace);
-  Operand16 x, w;
+  Laid x, w;
   hipError_t err = lay_out(a.x, a.x_stride, a.rows, a.cols, a.dtype, ws, x, stream);
   if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.outs, a.cols, a.dtype, ws, w, stream);
   if (err != hipSuccess) return err;
@@ -223,7 +184,7 @@ hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t*
   Workspace ws(workspace);
   const bool products = a.dx != nullptr || a.dweight != nullptr;
   // dz, and the column sums for db.
-  Operand16 dz{static_cast<const uint16_t*>(a.grad), a.g_stride, 0};
+  Laid dz{a.grad, a.g_stride};
   const bool form = products && (a.saved != nullptr || !as_it_is(a.grad, a.g_stride, a.outs, a.dtype));
   if (form || a.dbias != nullptr) {
     const int blocks = prepare_blocks(a.dtype, a.rows, a.outs);
@@ -236,8 +197,8 @@ hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t*
     p.cols = static_cast<int>(a.outs);
     if (form) {
       p.ld = padded(a.outs);
-      p.out = ws.take<uint16_t>(a.rows * p.ld * (a.dtype == F32::code ? 3 : 1));
-      dz = {p.out, p.ld, a.rows * p.ld};
+      p.out = ws.take<char>(a.rows * p.ld * (a.dtype == F32::code ? 4 : 2));
+      dz = {p.out, p.ld};
     }
     if (a.dbias != nullptr) p.partial = ws.take<float>(static_cast<int64_t>(blocks) * a.outs);
     if (!ws.dry()) {
@@ -249,7 +210,7 @@ hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t*
   }
   hipError_t err = hipSuccess;
   if (a.dx != nullptr) {
-    Operand16 w;
+    Laid w;
     err = lay_out(a.weight, a.w_stride, a.outs, a.cols, a.dtype, ws, w, stream);
     ProductArgs p{};
     p.m = static_cast<int>(a.rows);
@@ -259,7 +220,7 @@ hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t*
     if (err == hipSuccess) err = multiply(p, dz, w, a.dtype, false, true, ws, stream);
   }
   if (err == hipSuccess && a.dweight != nullptr) {
-    Operand16 x;
+    Laid x;
     err = lay_out(a.x, a.x_stride, a.rows, a.cols, a.dtype, ws, x, stream);
     ProductArgs p{};
     p.m = static_cast<int>(a.outs);

@@ -41,8 +41,8 @@ struct Strip {
   __device__ __forceinline__ static int swap_of(int k) {
     return Span == 64 ? (((k >> 1) & 1) << 2) | (((k >> 3) & 1) << 1) : ((k >> 3) & 1) << 1;
   }
-  __device__ __forceinline__ void init(const uint16_t* data, int64_t ld, int first, int count, int lane) {
-    base = reinterpret_cast<const char*>(Cols ? data + first : data + first * ld);
+  __device__ __forceinline__ void init(const void* operand, int64_t ld, int first, int count, int lane) {
+    base = static_cast<const char*>(operand) + 2 * (Cols ? static_cast<int64_t>(first) : first * ld);
     row = static_cast<int32_t>(2 * ld);
     step = Cols ? kDepth * static_cast<int64_t>(row) : 2 * kDepth;
     rows = count - first;
@@ -61,8 +61,8 @@ struct Strip {
     }
   }
   // Loads the strip of step t, zero past the sum's end and the last row.
-  __device__ __forceinline__ void stage(int64_t offset, int t, int k, uint32_t lds) const {
-    const char* from = base + offset + t * step;
+  __device__ __forceinline__ void stage(int t, int k, uint32_t lds) const {
+    const char* from = base + t * step;
     const int left = k - t * kDepth;
 #pragma unroll
     for (int u = 0; u < kCount; ++u) {
@@ -104,13 +104,12 @@ struct Strip {
 // LongA: A is the long operand.
 template <typename T, bool LongA, bool LongCols, bool ShortCols>
 __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
-  using E = std::conditional_t<T::code == F16::code, F16, BF16>;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kRing * kSlot];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slice = blockIdx.y;
   const int first = static_cast<int>(blockIdx.x) * (LongCols ? 4 * kLong : kLong) + (LongCols ? wave * kLong : 0);
-  const Steps<T, kDepth> steps(p, slice);
+  const Steps<kDepth> steps(p, slice);
   // In rows a wavefront takes every fourth strip.
   const int begin = steps.begin + (LongCols ? 0 : wave), by = LongCols ? 1 : 4;
   const int count = steps.end > begin ? (steps.end - begin + by - 1) / by : 0;
@@ -120,12 +119,9 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
   s.init(LongA ? p.b : p.a, LongA ? p.ldb : p.lda, 0, LongA ? p.n : p.m, lane);
   const uint32_t ring = lds_address(lds) + wave * kRing * kSlot;
   const auto stage = [&](int i) {
-    int64_t oa, ob;
-    int t;
-    steps.place(p, begin + i * by, t, oa, ob);
     const uint32_t to = ring + i % kRing * kSlot;
-    l.stage(LongA ? oa : ob, t, p.k, to);
-    s.stage(LongA ? ob : oa, t, p.k, to + kLongBytes);
+    l.stage(begin + i * by, p.k, to);
+    s.stage(begin + i * by, p.k, to + kLongBytes);
   };
   Floats16 acc[2];
 #pragma unroll
@@ -156,7 +152,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           // The operand whose rows are the results' columns first: a lane holds four neighbouring ones.
-          acc[j] = LongA ? mfma32<E>(y[kk], x[j][kk], acc[j]) : mfma32<E>(x[j][kk], y[kk], acc[j]);
+          acc[j] = LongA ? mfma32<T>(y[kk], x[j][kk], acc[j]) : mfma32<T>(x[j][kk], y[kk], acc[j]);
     }
   }
   // [m][n] of a wavefront's sums in its own part of the ring: 64 x 32 or 32 x 64.
@@ -214,7 +210,7 @@ hipError_t run(const ProductArgs& p, bool long_cols, bool short_cols, hipStream_
 
 }  // namespace
 
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
+bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols) {
   if (p.m > kShort && p.n > kShort) return false;
   const bool long_a = p.m > p.n, cols = long_a ? a_cols : b_cols;
   p.side = kShort;
@@ -222,7 +218,7 @@ bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   const int side = cols ? 4 * kLong : kLong;
   int& tiles = long_a ? p.tiles_m : p.tiles_n;
   tiles = ((long_a ? p.m : p.n) + side - 1) / side;
-  const int64_t steps = static_cast<int64_t>((p.k + kDepth - 1) / kDepth) * (dtype == F32::code ? 6 : 1);
+  const int64_t steps = (p.k + kDepth - 1) / kDepth;
   // Slices of at least four strips a wavefront until every compute unit has a workgroup.
   p.slices = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>((compute_units() + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
@@ -230,7 +226,7 @@ bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
 }
 
 hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
-  return with_type(dtype, [&](auto t) {
+  return with_half_type(dtype, [&](auto t) {
     using T = decltype(t);
     return p.m > p.n ? run<T, true>(p, a_cols, b_cols, stream) : run<T, false>(p, b_cols, a_cols, stream);
   });

@@ -37,14 +37,13 @@ __device__ __forceinline__ void multiply(Floats16 (&acc)[2], U32x4 x, U32x4 y0, 
 
 // The step in buffer R.  x0 and y0 hold its first half, and after it the next one's.
 template <int R, typename T, bool ACols, bool BCols>
-__device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols, kTile>& a, Feed<T, BCols, kTile>& b,
+__device__ __forceinline__ void step(Feeder<ACols, kTile>& a, Feeder<BCols, kTile>& b,
                                      const Finder<ACols, kTile>& fa, const Finder<BCols, kTile>& fb,
                                      Floats16 (&acc)[2], U32x4 (&x0)[2], U32x4 (&x1)[2], U32x4 (&y0)[4],
                                      U32x4 (&y1)[4]) {
-  using E = std::conditional_t<T::code == F16::code, F16, BF16>;
   read_half<R>(fa, fb, 1, x1, y1);
-  multiply<E>(acc, x0[0], y0[0], y0[1]);
-  multiply<E>(acc, x0[1], y0[2], y0[3]);
+  multiply<T>(acc, x0[0], y0[0], y0[1]);
+  multiply<T>(acc, x0[1], y0[2], y0[3]);
   __builtin_amdgcn_sched_barrier(0);
   // This step's buffer has been read, and the next one's loads are there once only the
   // four of each of the two steps behind it are on their way.
@@ -56,11 +55,11 @@ __device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols, kTile>
   for (int u = 0; u < 2; ++u) {
     a.stage(u, R * kBuffer);
     b.stage(u, R * kBuffer);
-    multiply<E>(acc, x1[u], y1[2 * u], y1[2 * u + 1]);
+    multiply<T>(acc, x1[u], y1[2 * u], y1[2 * u + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  a.advance(p, true);
-  b.advance(p, false);
+  a.advance();
+  b.advance();
 }
 
 template <typename T, bool ACols, bool BCols>
@@ -70,12 +69,12 @@ __global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = tile_of(p, blockIdx.x);
   const int m0 = tile.m * kTile, n0 = tile.n * kTile, slice = blockIdx.y;
-  const Steps<T, kStep> steps(p, slice);
+  const Steps<kStep> steps(p, slice);
   const int count = steps.end - steps.begin;
-  Feed<T, ACols, kTile> a{{}, {}, steps, steps.begin, lds_address(lds) + wave * 2048};
-  Feed<T, BCols, kTile> b{{}, {}, steps, steps.begin, lds_address(lds) + kRing * kBuffer + wave * 2048};
-  a.start.init(p.a, p.lda, m0, p.m, p.k, lane, wave);
-  b.start.init(p.b, p.ldb, n0, p.n, p.k, lane, wave);
+  Feeder<ACols, kTile> a;
+  Feeder<BCols, kTile> b;
+  a.init(p.a, p.lda, m0, p.m, p.k, steps.begin, lds_address(lds), lane, wave);
+  b.init(p.b, p.ldb, n0, p.n, p.k, steps.begin, lds_address(lds) + kRing * kBuffer, lane, wave);
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
   const Finder<ACols, kTile> fa(lds_address(lds), wm, lane);
   const Finder<BCols, kTile> fb(lds_address(lds) + kRing * kBuffer, wn, lane);
@@ -85,8 +84,6 @@ __global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
   if (count > 0) {
-    a.place(p, true);
-    b.place(p, false);
 #pragma unroll
     for (int s = 0; s < kRing; ++s) {
 #pragma unroll
@@ -94,8 +91,8 @@ __global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
         a.stage(u, s * kBuffer);
         b.stage(u, s * kBuffer);
       }
-      a.advance(p, true);
-      b.advance(p, false);
+      a.advance();
+      b.advance();
     }
     wait_loads<4 * (kRing - 1)>();
     meet();
@@ -103,10 +100,10 @@ __global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
     read_half<0>(fa, fb, 0, x0, y0);
     // Loads and reads go on past the last step, of zeros.
     for (int s = 0; s < count; s += 4) {
-      step<0>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 1 < count) step<1>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 2 < count) step<2>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 3 < count) step<3>(p, a, b, fa, fb, acc, x0, x1, y0, y1);
+      step<0, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 1 < count) step<1, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 2 < count) step<2, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 3 < count) step<3, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
     }
   }
   wait_loads<0>();
@@ -168,24 +165,28 @@ void set_tiles(ProductArgs& p, int side) {
 }  // namespace
 
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
-  if (plan_narrow_product(p, dtype, a_cols, b_cols)) return;
-  const int64_t steps = static_cast<int64_t>((p.k + kStep - 1) / kStep) * (dtype == F32::code ? 6 : 1);
+  const bool f32 = dtype == F32::code;
+  if (!f32 && plan_narrow_product(p, a_cols, b_cols)) return;
   const int64_t units = compute_units();
   const auto rounds = [&](int64_t groups) { return static_cast<double>((groups + units - 1) / units); };
   // Microseconds, measured: a workgroup of a tile of 256 takes 5 and 1.15 a step of 64, one of a tile
-  // of 128 takes 3 and 0.4; slices cost a launch and their sums' way to memory and back.
+  // of 128 takes 3 and 0.8 (FP32: 1.0 a step of 32); slices cost a launch and their sums' way to
+  // memory and back.
   set_tiles(p, kTile);
+  const int64_t steps = f32 ? (p.k + 31) / 32 : (p.k + 63) / 64;
+  const double step = f32 ? 1.0 : 0.8;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   const double results = static_cast<double>(p.m) * p.n;
   double best = 0.0;
   for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
-    const double us = rounds(tiles * s) * (3.0 + 0.4 * static_cast<double>((steps + s - 1) / s)) +
-                      (s > 1 ? 4.0 + results * 4e-6 * static_cast<double>(s + 1) / 4.0 : 0.0);
+    const double us = rounds(tiles * s) * (3.0 + step * static_cast<double>((steps + s - 1) / s)) +
+                      (s > 1 ? 4.0 + results * 1e-6 * static_cast<double>(s + 1) : 0.0);
     if (s == 1 || us < best) {
       best = us;
       p.slices = static_cast<int>(s);
     }
   }
+  if (f32) return;
   ProductArgs wide = p;
   set_tiles(wide, 256);
   wide.slices = 1;
@@ -194,13 +195,18 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
 }
 
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
-  if (p.side == 256) return launch_wide_product(p, dtype, a_cols, b_cols, stream);
-  return with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    const hipError_t err = p.side == kTile ? run<T>(p, a_cols, b_cols, stream)
-                                           : launch_narrow_product(p, dtype, a_cols, b_cols, stream);
-    return err != hipSuccess || p.slices == 1 ? err : join<T>(p, stream);
-  });
+  hipError_t err;
+  if (dtype == F32::code) {
+    err = launch_f32_product(p, a_cols, b_cols, stream);
+  } else if (p.side == 256) {
+    err = launch_wide_product(p, dtype, a_cols, b_cols, stream);
+  } else if (p.side == kTile) {
+    err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
+  } else {
+    err = launch_narrow_product(p, dtype, a_cols, b_cols, stream);
+  }
+  if (err != hipSuccess || p.slices == 1) return err;
+  return with_type(dtype, [&](auto t) { return join<decltype(t)>(p, stream); });
 }
 
 }  // namespace fh

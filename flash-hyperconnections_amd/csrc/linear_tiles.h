@@ -28,8 +28,13 @@ struct Feeder {
   int32_t voff[2];  // of the even and the odd loads
   int at_k;         // the first k of this lane's chunk in load 0
   int left;         // elements of the sum from here on
+  uint32_t lds;     // where this wavefront's loads go in the first buffer
 
-  __device__ __forceinline__ void init(const uint16_t* data, int64_t ld, int first, int count, int k, int lane, int wave) {
+  // Side rows (columns) from `first` on, of `count`; the sum has k terms, and `begin` steps of it are left out.
+  __device__ __forceinline__ void init(const void* operand, int64_t ld, int first, int count, int k, int begin,
+                                       uint32_t to, int lane, int wave) {
+    const auto* data = static_cast<const uint16_t*>(operand);
+    lds = to + wave * kLoads * 1024;
     const int32_t row = static_cast<int32_t>(2 * ld);
     if constexpr (Cols) {
       constexpr int across = Side / 8;  // chunks of a row
@@ -55,28 +60,22 @@ struct Feeder {
         rsrc[u][2] = more > 0 ? (more - 1) * row + 2 * (k < kStep ? (k + 7) & ~7 : kStep) : 0;
       }
     }
+    left = k;
+    advance(begin);
   }
-  __device__ __forceinline__ void move(int64_t by) {
+  // Loads load u of this step into the buffer `offset` bytes on, zero past the sum's end and the last row.
+  __device__ __forceinline__ void stage(int u, int offset) const {
+    const int k = Cols ? at_k + u * kRows : at_k ^ (32 * (u & 1));
+    lds_load16(rsrc[u], lds + offset + u * 1024, k < left ? voff[u & 1] : kOutOfRange, 0);
+  }
+  __device__ __forceinline__ void advance(int64_t steps = 1) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const uint64_t base = (static_cast<uint64_t>(rsrc[u][1]) << 32 | rsrc[u][0]) + by;
+      const uint64_t base = (static_cast<uint64_t>(rsrc[u][1]) << 32 | rsrc[u][0]) + steps * step;
       rsrc[u][0] = static_cast<uint32_t>(base);
       rsrc[u][1] = static_cast<uint32_t>(base >> 32);
     }
-  }
-  // Moves to step t of a sum of k elements, `offset` bytes further on.
-  __device__ __forceinline__ void go(int64_t offset, int t, int k) {
-    move(offset + t * step);
-    left = k - t * kStep;
-  }
-  // Loads load u of this step to LDS address `lds`, zero past the sum's end and the last row.
-  __device__ __forceinline__ void stage(int u, uint32_t lds) const {
-    const int k = Cols ? at_k + u * kRows : at_k ^ (32 * (u & 1));
-    lds_load16(rsrc[u], lds, k < left ? voff[u & 1] : kOutOfRange, 0);
-  }
-  __device__ __forceinline__ void advance() {
-    move(step);
-    left -= kStep;
+    left -= static_cast<int>(steps) * kStep;
   }
 };
 
@@ -124,32 +123,6 @@ __device__ __forceinline__ void meet() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-
-// An operand's steps of a slice: the next one to load.
-template <typename T, bool Cols, int Side>
-struct Feed {
-  static constexpr int kBuffer = Side * kStep * 2;  // bytes of a step
-  Feeder<Cols, Side> f, start;
-  Steps<T, kStep> steps;
-  int next;
-  uint32_t lds;  // where this wavefront's loads go in buffer 0
-
-  __device__ __forceinline__ void place(const ProductArgs& p, bool of_a) {
-    int64_t oa, ob;
-    int t;
-    steps.place(p, next, t, oa, ob);
-    f = start;
-    f.go(of_a ? oa : ob, t, p.k);
-  }
-  __device__ __forceinline__ void stage(int u, int offset) const { f.stage(u, lds + offset + u * 1024); }
-  __device__ __forceinline__ void advance(const ProductArgs& p, bool of_a) {
-    ++next;
-    f.advance();
-    if constexpr (T::code == F32::code) {  // the next pair of planes begins
-      if (f.left <= 0 && next < steps.end) place(p, of_a);
-    }
-  }
-};
 
 }  // namespace
 }  // namespace fh

@@ -39,32 +39,31 @@ __device__ __forceinline__ void read_two(const Finder<Cols, kSide>& f, int i, in
 // ([2 (k / 16) + tile]), and after it those of the next step.  (Registers are passed
 // by reference: captured ones went to memory.)
 template <int B, typename T, bool ACols, bool BCols>
-__device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols, kSide>& a, Feed<T, BCols, kSide>& b,
+__device__ __forceinline__ void step(Feeder<ACols, kSide>& a, Feeder<BCols, kSide>& b,
                                      const Finder<ACols, kSide>& fa, const Finder<BCols, kSide>& fb,
                                      Floats16 (&acc)[4][2], U32x4 (&x0)[4], U32x4 (&x1)[4], U32x4 (&y)[4],
                                      U32x4 (&z)[4]) {
-  using E = std::conditional_t<T::code == F16::code, F16, BF16>;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < 2) read_two<B>(fa, 2, i, x1 + 2 * i);
     b.stage(i, (B ^ 1) * kBuffer);
-    two<E>(acc[i & 1], x0[i], y[i & 2], y[(i & 2) + 1]);
+    two<T>(acc[i & 1], x0[i], y[i & 2], y[(i & 2) + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  b.advance(p, false);
+  b.advance();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < 2) {
       read_two<B>(fa, 0, 2 + i, x0 + 2 * i);
       read_two<B>(fb, 0, 2 + i, z + 2 * i);
     }
-    two<E>(acc[2 + (i & 1)], x1[i], y[i & 2], y[(i & 2) + 1]);
+    two<T>(acc[2 + (i & 1)], x1[i], y[i & 2], y[(i & 2) + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (i < 2) read_two<B>(fa, 2, 2 + i, x1 + 2 * i);
-    two<E>(acc[i & 1], x0[i], z[i & 2], z[(i & 2) + 1]);
+    two<T>(acc[i & 1], x0[i], z[i & 2], z[(i & 2) + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
   wait_lds();
@@ -77,10 +76,10 @@ __device__ __forceinline__ void step(const ProductArgs& p, Feed<T, ACols, kSide>
       read_two<B ^ 1>(fb, 0, i, y + 2 * i);
     }
     a.stage(i, B * kBuffer);
-    two<E>(acc[2 + (i & 1)], x1[i], z[i & 2], z[(i & 2) + 1]);
+    two<T>(acc[2 + (i & 1)], x1[i], z[i & 2], z[(i & 2) + 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  a.advance(p, true);
+  a.advance();
 }
 
 template <typename T, bool ACols, bool BCols>
@@ -90,12 +89,12 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = tile_of(p, blockIdx.x);
   const int m0 = tile.m * kSide, n0 = tile.n * kSide, slice = blockIdx.y;
-  const Steps<T, kStep> steps(p, slice);
+  const Steps<kStep> steps(p, slice);
   const int count = steps.end - steps.begin;
-  Feed<T, ACols, kSide> a{{}, {}, steps, steps.begin, lds_address(lds) + wave * 4096};
-  Feed<T, BCols, kSide> b{{}, {}, steps, steps.begin, lds_address(lds) + 2 * kBuffer + wave * 4096};
-  a.start.init(p.a, p.lda, m0, p.m, p.k, lane, wave);
-  b.start.init(p.b, p.ldb, n0, p.n, p.k, lane, wave);
+  Feeder<ACols, kSide> a;
+  Feeder<BCols, kSide> b;
+  a.init(p.a, p.lda, m0, p.m, p.k, steps.begin, lds_address(lds), lane, wave);
+  b.init(p.b, p.ldb, n0, p.n, p.k, steps.begin, lds_address(lds) + 2 * kBuffer, lane, wave);
   const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
   const Finder<ACols, kSide> fa(lds_address(lds), wm, lane);
   const Finder<BCols, kSide> fb(lds_address(lds) + 2 * kBuffer, wn, lane);
@@ -108,20 +107,18 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   U32x4 x0[4], x1[4], y[4], z[4];
   if (count > 0) {
-    a.place(p, true);
-    b.place(p, false);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       a.stage(u, 0);
       b.stage(u, 0);
     }
-    a.advance(p, true);
-    b.advance(p, false);
+    a.advance();
+    b.advance();
     wait_vm<0>();
     meet();
 #pragma unroll
     for (int u = 0; u < 4; ++u) a.stage(u, kBuffer);
-    a.advance(p, true);
+    a.advance();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       read_two<0>(fa, 0, i, x0 + 2 * i);
@@ -129,8 +126,8 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
     }
     // Loads and reads go on past the last step, of zeros.
     for (int s = 0; s < count; s += 2) {
-      step<0>(p, a, b, fa, fb, acc, x0, x1, y, z);
-      if (s + 1 < count) step<1>(p, a, b, fa, fb, acc, x0, x1, y, z);
+      step<0, T>(a, b, fa, fb, acc, x0, x1, y, z);
+      if (s + 1 < count) step<1, T>(a, b, fa, fb, acc, x0, x1, y, z);
     }
   }
   wait_vm<0>();
@@ -165,7 +162,7 @@ hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t strea
 }  // namespace
 
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
-  return with_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
+  return with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
 }
 
 }  // namespace fh
