@@ -138,7 +138,12 @@ __device__ __forceinline__ void load_eight(const S* from, int count, S (&e)[8]) 
 template <typename S>
 __device__ __forceinline__ void store_eight(const S (&e)[8], S* to, int count) {
   if (count >= 8) {
-    __builtin_memcpy(to, e, sizeof(e));
+    if constexpr (sizeof(e) == 16) {
+      U32x4 w;
+      __builtin_memcpy(&w, e, 16);
+      typedef U32x4 Unaligned __attribute__((aligned(2)));
+      __builtin_nontemporal_store(w, reinterpret_cast<Unaligned*>(to));
+    } else __builtin_memcpy(to, e, sizeof(e));
   } else {
 #pragma unroll
     for (int i = 0; i < 7; ++i)

@@ -108,7 +108,10 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slice = blockIdx.y;
-  const int first = static_cast<int>(blockIdx.x) * (LongCols ? 4 * kLong : kLong) + (LongCols ? wave * kLong : 0);
+  // Each die takes neighbouring tiles: in columns one tile's 512 bytes of a row lie in two
+  // of an L2's sixteen channels.
+  const Tile tile = tile_of(p, blockIdx.x);
+  const int first = (tile.m + tile.n) * (LongCols ? 4 * kLong : kLong) + (LongCols ? wave * kLong : 0);
   const Steps<kDepth> steps(p, slice);
   // In rows a wavefront takes every fourth strip.
   const int begin = steps.begin + (LongCols ? 0 : wave), by = LongCols ? 1 : 4;
@@ -221,7 +224,7 @@ bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols) {
   const int64_t steps = (p.k + kDepth - 1) / kDepth;
   // Slices of at least four strips a wavefront until every compute unit has a workgroup.
   p.slices = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>((compute_units() + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
+      1, std::min<int64_t>((compute_units() * (cols ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
   return true;
 }
 

@@ -118,6 +118,51 @@ __global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
   finish_parked<T, 32>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
+// Sums of one step, at most 64 terms: two workgroups a compute unit, one storing while
+// the other loads.
+template <typename T, bool ACols, bool BCols>
+__global__ __launch_bounds__(512, 4) void outer_product_kernel(ProductArgs p) {
+  __shared__ __attribute__((aligned(1024))) char lds[8 * 8192];  // A's and B's step, then the results
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Tile tile = tile_of(p, blockIdx.x);
+  const int m0 = tile.m * kTile, n0 = tile.n * kTile;
+  Feeder<ACols, kTile> a;
+  Feeder<BCols, kTile> b;
+  a.init(p.a, p.lda, m0, p.m, p.k, 0, lds_address(lds), lane, wave);
+  b.init(p.b, p.ldb, n0, p.n, p.k, 0, lds_address(lds) + kBuffer, lane, wave);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    a.stage(u, 0);
+    b.stage(u, 0);
+  }
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
+  const Finder<ACols, kTile> fa(lds_address(lds), wm, lane);
+  const Finder<BCols, kTile> fb(lds_address(lds) + kBuffer, wn, lane);
+  Floats16 acc[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+  wait_loads<0>();
+  meet();
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    if (16 * kk >= p.k) break;
+    multiply<T>(acc, fa.read(0, 0, kk), fb.read(0, 0, kk), fb.read(0, 1, kk));
+  }
+  wait_lds();
+  meet();
+  char* area = lds + wave * 8192;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      park(area, lane & 31, 8 * j + 2 * q + (lane >> 5),
+           Floats4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]});
+  finish_parked<T, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
+}
+
 // Adds the slices in order and finishes.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
@@ -141,6 +186,12 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
 template <typename T>
 hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
+  if (p.k <= kStep && p.slices == 1) {
+    if (!a_cols && !b_cols) outer_product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
+    if (!a_cols && b_cols) outer_product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
+    if (a_cols && b_cols) outer_product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
+    return hipGetLastError();
+  }
   if (!a_cols && !b_cols) product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
   if (!a_cols && b_cols) product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
   if (a_cols && b_cols) product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
@@ -167,6 +218,11 @@ void set_tiles(ProductArgs& p, int side) {
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   const bool f32 = dtype == F32::code;
   if (!f32 && plan_narrow_product(p, a_cols, b_cols)) return;
+  if (!f32 && p.k <= kStep) {
+    set_tiles(p, kTile);
+    p.slices = 1;
+    return;
+  }
   const int64_t units = compute_units();
   const auto rounds = [&](int64_t groups) { return static_cast<double>((groups + units - 1) / units); };
   // Microseconds, measured: a workgroup of a tile of 256 takes 5 and 1.15 a step of 64, one of a tile
