@@ -42,11 +42,19 @@ __device__ __forceinline__ U32x4 load_row(const typename T::storage* row, int c,
   return w;
 }
 
+// 16 bytes at any element, with the nontemporal hint: results are larger than the
+// caches where their way to memory counts.
+template <typename S>
+__device__ __forceinline__ void store16(U32x4 w, S* to) {
+  typedef U32x4 Unaligned __attribute__((aligned(2)));
+  __builtin_nontemporal_store(w, reinterpret_cast<Unaligned*>(to));
+}
+
 template <typename T, bool Whole = false>
 __device__ __forceinline__ void store_row(U32x4 w, typename T::storage* row, int c, int cols) {
   constexpr int V = kVec<T>;
   if (c + V <= cols) {
-    __builtin_memcpy(row + c, &w, 16);
+    store16(w, row + c);
   } else if (!Whole && c < cols) {
     typename T::storage e[V];
     __builtin_memcpy(e, &w, 16);

@@ -21,7 +21,7 @@ struct ProductArgs {
   int64_t lda, ldb;
   int m, n, k;
   int tiles_m, tiles_n;
-  int side;              // of a tile
+  int side_m, side_n;    // of a tile
   int slices;            // of the sum over k
   float* partial;        // [slices, m, n] where there are several
   const void* bias;      // [n] or null, FP32 or the output's type
@@ -135,15 +135,16 @@ __device__ __forceinline__ void load_eight(const S* from, int count, S (&e)[8]) 
     for (int i = 0; i < 8; ++i) e[i] = i < count ? from[i] : S{};
   }
 }
-template <typename S>
+// Nontemporal unless they are read again soon, as partial sums are.
+template <bool Soon = false, typename S>
 __device__ __forceinline__ void store_eight(const S (&e)[8], S* to, int count) {
-  if (count >= 8) {
-    if constexpr (sizeof(e) == 16) {
-      U32x4 w;
-      __builtin_memcpy(&w, e, 16);
-      typedef U32x4 Unaligned __attribute__((aligned(2)));
-      __builtin_nontemporal_store(w, reinterpret_cast<Unaligned*>(to));
-    } else __builtin_memcpy(to, e, sizeof(e));
+  if (Soon && count >= 8) {
+    __builtin_memcpy(to, e, sizeof(e));
+  } else if (count >= 8) {
+    U32x4 w[sizeof(e) / 16];
+    __builtin_memcpy(w, e, sizeof(e));
+#pragma unroll
+    for (size_t i = 0; i < sizeof(e) / 16; ++i) store16(w[i], to + i * (16 / sizeof(S)));
   } else {
 #pragma unroll
     for (int i = 0; i < 7; ++i)
@@ -173,7 +174,7 @@ __device__ __forceinline__ void finish_eight(const ProductArgs& p, int slice, in
   const int64_t at = static_cast<int64_t>(i) * p.n + j;
   const int left = p.n - j;
   if (p.slices > 1) {
-    store_eight(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
+    store_eight<true>(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
     return;
   }
   if (p.bias != nullptr) {

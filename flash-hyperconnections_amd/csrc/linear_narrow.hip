@@ -216,7 +216,7 @@ hipError_t run(const ProductArgs& p, bool long_cols, bool short_cols, hipStream_
 bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols) {
   if (p.m > kShort && p.n > kShort) return false;
   const bool long_a = p.m > p.n, cols = long_a ? a_cols : b_cols;
-  p.side = kShort;
+  p.side_m = p.side_n = kShort;
   p.tiles_m = p.tiles_n = 1;
   const int side = cols ? 4 * kLong : kLong;
   int& tiles = long_a ? p.tiles_m : p.tiles_n;

@@ -1,10 +1,11 @@
-// Matrix products of the linear layer in 128 x 128 tiles, where tiles of 256 are too
-// few to fill the card, and the joining of sums in several slices.
+// Matrix products of the linear layer in tiles of 128 or 256 rows by 128 columns, where
+// tiles of 256 x 256 are too few to fill the card, and the joining of sums in several
+// slices.
 //
-// Such products are short: what costs is the time from one step's loads to the next.
-// So a compute unit holds one workgroup, of eight wavefronts with 32 x 64 results each,
-// whose four buffers keep three steps of 64 on their way (two workgroups with one step
-// each on its way took twice as long a step).  The wavefronts meet once a step.
+// A compute unit holds one workgroup of eight wavefronts, whose buffers keep two or
+// three steps of 64 on their way (two workgroups with one step each on its way took
+// twice as long a step).  The wavefronts meet once a step.  What bounds the smaller tile
+// is the L2: 32 KB a step for 2 M multiply-adds, at about 10 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -13,16 +14,26 @@
 namespace fh {
 namespace {
 
-constexpr int kTile = 128, kRing = 4;
-constexpr int kBuffer = kTile * kStep * 2;  // bytes of one operand's step
+constexpr int kTile = 128;
+constexpr int kBuffer = kTile * kStep * 2;  // bytes of one operand's step of 128 rows
 
-// k = 32 half .. + 31 of the step in buffer R; y: [2 kk + tile].
-template <int R, bool ACols, bool BCols>
-__device__ __forceinline__ void read_half(const Finder<ACols, kTile>& fa, const Finder<BCols, kTile>& fb, int half,
-                                          U32x4 (&x)[2], U32x4 (&y)[4]) {
+// A tile of 128 or 256 rows by 128 columns: 32 Tall x 64 results a wavefront, and the
+// steps that its LDS holds.
+template <int Tall>
+struct Shape {
+  static constexpr int kRows = kTile * Tall, kRing = Tall == 1 ? 4 : 3;
+  static constexpr int kA = kRows * kStep * 2, kB = kBuffer;    // bytes of an operand's step
+  static constexpr int kLoads = 2 * Tall + 2;                   // of a wavefront's in a step
+};
+
+// k = 32 half .. + 31 of the step in buffer R; x: [Tall kk + tile], y: [2 kk + tile].
+template <int R, int Tall, bool ACols, bool BCols>
+__device__ __forceinline__ void read_half(const Finder<ACols, kTile * Tall>& fa, const Finder<BCols, kTile>& fb,
+                                          int half, U32x4 (&x)[2 * Tall], U32x4 (&y)[4]) {
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
-    x[kk] = fa.read(R * kBuffer, 0, 2 * half + kk);
+#pragma unroll
+    for (int i = 0; i < Tall; ++i) x[Tall * kk + i] = fa.read(R * Shape<Tall>::kA, i, 2 * half + kk);
     y[2 * kk] = fb.read(R * kBuffer, 0, 2 * half + kk);
     y[2 * kk + 1] = fb.read(R * kBuffer, 1, 2 * half + kk);
   }
@@ -36,86 +47,101 @@ __device__ __forceinline__ void multiply(Floats16 (&acc)[2], U32x4 x, U32x4 y0, 
 }
 
 // The step in buffer R.  x0 and y0 hold its first half, and after it the next one's.
-template <int R, typename T, bool ACols, bool BCols>
-__device__ __forceinline__ void step(Feeder<ACols, kTile>& a, Feeder<BCols, kTile>& b,
-                                     const Finder<ACols, kTile>& fa, const Finder<BCols, kTile>& fb,
-                                     Floats16 (&acc)[2], U32x4 (&x0)[2], U32x4 (&x1)[2], U32x4 (&y0)[4],
-                                     U32x4 (&y1)[4]) {
-  read_half<R>(fa, fb, 1, x1, y1);
-  multiply<T>(acc, x0[0], y0[0], y0[1]);
-  multiply<T>(acc, x0[1], y0[2], y0[3]);
+template <int R, typename T, int Tall, bool ACols, bool BCols>
+__device__ __forceinline__ void step(Feeder<ACols, kTile * Tall>& a, Feeder<BCols, kTile>& b,
+                                     const Finder<ACols, kTile * Tall>& fa, const Finder<BCols, kTile>& fb,
+                                     Floats16 (&acc)[Tall][2], U32x4 (&x0)[2 * Tall], U32x4 (&x1)[2 * Tall],
+                                     U32x4 (&y0)[4], U32x4 (&y1)[4]) {
+  constexpr int kRing = Shape<Tall>::kRing;
+  read_half<R, Tall>(fa, fb, 1, x1, y1);
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int i = 0; i < Tall; ++i) multiply<T>(acc[i], x0[Tall * kk + i], y0[2 * kk], y0[2 * kk + 1]);
   __builtin_amdgcn_sched_barrier(0);
-  // This step's buffer has been read, and the next one's loads are there once only the
-  // four of each of the two steps behind it are on their way.
+  // This step's buffer has been read, and the next one's loads are there once only those
+  // of the steps behind it are on their way.
   wait_lds();
-  wait_loads<8>();
+  wait_loads<(kRing - 2) * Shape<Tall>::kLoads>();
   meet();
-  read_half<(R + 1) % kRing>(fa, fb, 0, x0, y0);
+  read_half<(R + 1) % kRing, Tall>(fa, fb, 0, x0, y0);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    a.stage(u, R * kBuffer);
-    b.stage(u, R * kBuffer);
-    multiply<T>(acc, x1[u], y1[2 * u], y1[2 * u + 1]);
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < Tall; ++i) {
+      a.stage(Tall * u + i, R * Shape<Tall>::kA);
+      if (i == 0) b.stage(u, R * kBuffer);
+      multiply<T>(acc[i], x1[Tall * u + i], y1[2 * u], y1[2 * u + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   a.advance();
   b.advance();
 }
 
-template <typename T, bool ACols, bool BCols>
-__global__ __launch_bounds__(512) void product_kernel(ProductArgs p) {
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kRing * kBuffer];  // A's ring, B's ring
+template <typename T, int Tall, bool ACols, bool BCols>
+__global__ __launch_bounds__(512, 2) void product_kernel(ProductArgs p) {
+  using S = Shape<Tall>;
+  constexpr int kRing = S::kRing;
+  __shared__ __attribute__((aligned(1024))) char lds[kRing * (S::kA + S::kB)];  // A's ring, B's ring
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile tile = tile_of(p, blockIdx.x);
-  const int m0 = tile.m * kTile, n0 = tile.n * kTile, slice = blockIdx.y;
+  const int m0 = tile.m * S::kRows, n0 = tile.n * kTile, slice = blockIdx.y;
   const Steps<kStep> steps(p, slice);
   const int count = steps.end - steps.begin;
-  Feeder<ACols, kTile> a;
+  Feeder<ACols, kTile * Tall> a;
   Feeder<BCols, kTile> b;
   a.init(p.a, p.lda, m0, p.m, p.k, steps.begin, lds_address(lds), lane, wave);
-  b.init(p.b, p.ldb, n0, p.n, p.k, steps.begin, lds_address(lds) + kRing * kBuffer, lane, wave);
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
-  const Finder<ACols, kTile> fa(lds_address(lds), wm, lane);
-  const Finder<BCols, kTile> fb(lds_address(lds) + kRing * kBuffer, wn, lane);
-  Floats16 acc[2];
+  b.init(p.b, p.ldb, n0, p.n, p.k, steps.begin, lds_address(lds) + kRing * S::kA, lane, wave);
+  const int wm = (wave >> 1) * 32 * Tall, wn = (wave & 1) * 64;
+  const Finder<ACols, kTile * Tall> fa(lds_address(lds), wm, lane);
+  const Finder<BCols, kTile> fb(lds_address(lds) + kRing * S::kA, wn, lane);
+  Floats16 acc[Tall][2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < Tall; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   if (count > 0) {
 #pragma unroll
     for (int s = 0; s < kRing; ++s) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        a.stage(u, s * kBuffer);
-        b.stage(u, s * kBuffer);
-      }
+      for (int u = 0; u < 2 * Tall; ++u) a.stage(u, s * S::kA);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) b.stage(u, s * kBuffer);
       a.advance();
       b.advance();
     }
-    wait_loads<4 * (kRing - 1)>();
+    wait_loads<S::kLoads * (kRing - 1)>();
     meet();
-    U32x4 x0[2], x1[2], y0[4], y1[4];
-    read_half<0>(fa, fb, 0, x0, y0);
+    U32x4 x0[2 * Tall], x1[2 * Tall], y0[4], y1[4];
+    read_half<0, Tall>(fa, fb, 0, x0, y0);
     // Loads and reads go on past the last step, of zeros.
-    for (int s = 0; s < count; s += 4) {
-      step<0, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 1 < count) step<1, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 2 < count) step<2, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
-      if (s + 3 < count) step<3, T>(a, b, fa, fb, acc, x0, x1, y0, y1);
+    for (int s = 0; s < count; s += kRing) {
+      step<0, T, Tall>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 1 < count) step<1, T, Tall>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if (s + 2 < count) step<2, T, Tall>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      if constexpr (kRing == 4) {
+        if (s + 3 < count) step<3, T, Tall>(a, b, fa, fb, acc, x0, x1, y0, y1);
+      }
     }
   }
   wait_loads<0>();
-  __syncthreads();  // the buffers have been read: each wavefront takes 8 KB of them
-  char* area = lds + wave * 8192;
+  __syncthreads();  // the buffers have been read: each wavefront takes a part of them
+  char* area = lds + wave * 8192 * Tall;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < Tall; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      park(area, lane & 31, 8 * j + 2 * q + (lane >> 5),
-           Floats4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]});
-  finish_parked<T, 32>(p, slice, area, m0 + wm, n0 + wn, lane);
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const Floats16& v = acc[i][j];
+        park(area, 32 * i + (lane & 31), 8 * j + 2 * q + (lane >> 5),
+             Floats4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
+      }
+  finish_parked<T, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // Sums of one step, at most 64 terms: two workgroups a compute unit, one storing while
@@ -192,9 +218,15 @@ hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t strea
     if (a_cols && b_cols) outer_product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
     return hipGetLastError();
   }
-  if (!a_cols && !b_cols) product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
-  if (!a_cols && b_cols) product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
-  if (a_cols && b_cols) product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
+  if (p.side_m == kTile) {
+    if (!a_cols && !b_cols) product_kernel<T, 1, false, false><<<grid, block, 0, stream>>>(p);
+    if (!a_cols && b_cols) product_kernel<T, 1, false, true><<<grid, block, 0, stream>>>(p);
+    if (a_cols && b_cols) product_kernel<T, 1, true, true><<<grid, block, 0, stream>>>(p);
+  } else {
+    if (!a_cols && !b_cols) product_kernel<T, 2, false, false><<<grid, block, 0, stream>>>(p);
+    if (!a_cols && b_cols) product_kernel<T, 2, false, true><<<grid, block, 0, stream>>>(p);
+    if (a_cols && b_cols) product_kernel<T, 2, true, true><<<grid, block, 0, stream>>>(p);
+  }
   if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
   return hipGetLastError();
 }
@@ -207,10 +239,11 @@ hipError_t join(const ProductArgs& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-void set_tiles(ProductArgs& p, int side) {
-  p.side = side;
-  p.tiles_m = (p.m + side - 1) / side;
-  p.tiles_n = (p.n + side - 1) / side;
+void set_tiles(ProductArgs& p, int rows, int cols) {
+  p.side_m = rows;
+  p.side_n = cols;
+  p.tiles_m = (p.m + rows - 1) / rows;
+  p.tiles_n = (p.n + cols - 1) / cols;
 }
 
 }  // namespace
@@ -219,44 +252,57 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   const bool f32 = dtype == F32::code;
   if (!f32 && plan_narrow_product(p, a_cols, b_cols)) return;
   if (!f32 && p.k <= kStep) {
-    set_tiles(p, kTile);
+    set_tiles(p, kTile, kTile);
     p.slices = 1;
     return;
   }
   const int64_t units = compute_units();
   const auto rounds = [&](int64_t groups) { return static_cast<double>((groups + units - 1) / units); };
-  // Microseconds, measured: a workgroup of a tile of 256 takes 5 and 1.15 a step of 64, one of a tile
-  // of 128 takes 3 and 0.8 (FP32: 1.0 a step of 32); slices cost a launch and their sums' way to
-  // memory and back.
-  set_tiles(p, kTile);
+  // Microseconds of a workgroup: fixed, and a step of 64 (FP32: 32) with one workgroup on the
+  // card and what a full card adds.  Slices cost a launch and their sums' way to memory and
+  // back.  Fitted to 128 .. 4096 x 4096 x 4096, 2048 x 1024 x 4096, 64 x 16384 x 4096 and
+  // 3000 x 700 x 5000 in each tile and 1 to 16 slices; off by 10% at most where it decides.
+  struct Cost {
+    int rows, cols;
+    double fixed, step, shared;
+  };
+  constexpr Cost kF32[] = {{kTile, kTile, 4.2, 1.27, 0.3}};
+  constexpr Cost kHalf[] = {
+      {kTile, kTile, 4.2, 0.33, 0.2}, {2 * kTile, kTile, 7.0, 0.56, 0.34}, {256, 256, 10.0, 1.0, 0.55}};
   const int64_t steps = f32 ? (p.k + 31) / 32 : (p.k + 63) / 64;
-  const double step = f32 ? 1.0 : 0.8;
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   const double results = static_cast<double>(p.m) * p.n;
-  double best = 0.0;
-  for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
-    const double us = rounds(tiles * s) * (3.0 + step * static_cast<double>((steps + s - 1) / s)) +
-                      (s > 1 ? 4.0 + results * 1e-6 * static_cast<double>(s + 1) : 0.0);
-    if (s == 1 || us < best) {
-      best = us;
-      p.slices = static_cast<int>(s);
+  double best = -1.0;
+  ProductArgs chosen = p;
+  const auto consider = [&](const Cost& c) {
+    set_tiles(p, c.rows, c.cols);
+    const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+    for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
+      const double full = std::min(1.0, static_cast<double>(tiles * s) / static_cast<double>(units));
+      const double us =
+          rounds(tiles * s) * (c.fixed + (c.step + c.shared * full) * static_cast<double>((steps + s - 1) / s)) +
+          (s > 1 ? 3.5 + 1.3e-6 * results * static_cast<double>(s) : 0.0);
+      if (best < 0.0 || us < best) {
+        best = us;
+        p.slices = static_cast<int>(s);
+        chosen = p;
+      }
     }
+  };
+  if (f32) {
+    for (const Cost& c : kF32) consider(c);
+  } else {
+    for (const Cost& c : kHalf) consider(c);
   }
-  if (f32) return;
-  ProductArgs wide = p;
-  set_tiles(wide, 256);
-  wide.slices = 1;
-  if (rounds(static_cast<int64_t>(wide.tiles_m) * wide.tiles_n) * (5.0 + 1.15 * static_cast<double>(steps)) < best)
-    p = wide;
+  p = chosen;
 }
 
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
   hipError_t err;
   if (dtype == F32::code) {
     err = launch_f32_product(p, a_cols, b_cols, stream);
-  } else if (p.side == 256) {
+  } else if (p.side_n == 256) {
     err = launch_wide_product(p, dtype, a_cols, b_cols, stream);
-  } else if (p.side == kTile) {
+  } else if (p.side_n == kTile) {
     err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
   } else {
     err = launch_narrow_product(p, dtype, a_cols, b_cols, stream);
