@@ -221,7 +221,7 @@ template <typename T, int Rows>
 __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
                                               int lane) {
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
-#pragma unroll 1
+#pragma unroll 2
   for (int it = 0; it < Rows / 8; ++it) {
     const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
     float v[8];
