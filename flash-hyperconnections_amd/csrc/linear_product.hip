@@ -266,7 +266,7 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
     int rows, cols;
     double fixed, step, shared;
   };
-  constexpr Cost kF32[] = {{kTile, kTile, 4.2, 1.27, 0.3}};
+  constexpr Cost kF32[] = {{kTile, kTile, 4.2, 1.27, 0.3}, {2 * kTile, kTile, 7.0, 2.1, 0.55}};
   constexpr Cost kHalf[] = {
       {kTile, kTile, 4.2, 0.33, 0.2}, {2 * kTile, kTile, 7.0, 0.56, 0.34}, {256, 256, 10.0, 1.0, 0.55}};
   const int64_t steps = f32 ? (p.k + 31) / 32 : (p.k + 63) / 64;
