@@ -237,10 +237,10 @@ int validate_norm(const void* x, int64_t x_stride, const void* y, int param_dtyp
 int validate_linear(const fh::LinearArgs& a) {
   constexpr int64_t most = int64_t{1} << 22;
   if (!known_dtype(a.dtype) || (a.bias_dtype != a.dtype && a.bias_dtype != FH_DTYPE_F32) || a.rows < 0 ||
-      a.rows >= (int64_t{1} << 31) || a.cols < 1 || a.cols >= most || a.outs < 1 || a.outs >= most)
+      a.rows >= (int64_t{1} << 30) || a.cols < 1 || a.cols >= most || a.outs < 1 || a.outs >= most)
     return fail(FH_ERR_INVALID_ARGUMENT,
                 "linear: expected x [rows, cols] and weight [outs, cols] in float32, float16, or bfloat16 with fewer "
-                "than 2^31 rows and 1 <= cols, outs < 2^22, and a bias of their type or float32");
+                "than 2^30 rows and 1 <= cols, outs < 2^22, and a bias of their type or float32");
   if (a.act < FH_ACT_NONE || a.act > FH_ACT_SILU) return fail(FH_ERR_INVALID_ARGUMENT, "linear: unknown activation");
   return FH_OK;
 }

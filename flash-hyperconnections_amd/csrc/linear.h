@@ -99,29 +99,44 @@ __device__ __forceinline__ void activate_eight(float (&v)[8], int act) {
   }
 }
 
-// act'(z).
-template <typename T>
-__device__ __forceinline__ float slope(float z, int act) {
+// f times act'(z), of a vector.
+template <typename T, int V>
+__device__ __forceinline__ void slope_times(const float (&z)[V], int act, float (&f)[V]) {
   switch (act) {
-    case FH_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case FH_ACT_GELU: {
-      if constexpr (T::code == F32::code)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
-      const Normal n = normal_of(z);
-      return __builtin_fmaf(z, n.density, n.phi);
-    }
-    case FH_ACT_GELU_TANH: {
-      const float q = logistic<T>(1.5957691216057308f * __builtin_fmaf(0.044715f * z * z, z, z));
-      const float du2 = 1.5957691216057308f * __builtin_fmaf(0.134145f * z, z, 1.f);
-      // q (1 - q) is 0 where exp has left its range, whatever z du2 is.
-      const float curve = q * (1.f - q);
-      return curve > 0.f ? __builtin_fmaf(z * du2, curve, q) : q;
-    }
-    case FH_ACT_SILU: {
-      const float q = logistic<T>(z), curve = q * (1.f - q);
-      return curve > 0.f ? __builtin_fmaf(z, curve, q) : q;
-    }
-    default: return 1.f;
+    case FH_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = z[i] > 0.f ? f[i] : 0.f;
+      break;
+    case FH_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if constexpr (T::code == F32::code) {
+          f[i] *= 0.5f * (1.f + erff(z[i] * 0.70710678118654752f)) +
+                  z[i] * (0.39894228040143268f * expf(-0.5f * z[i] * z[i]));
+        } else {
+          const Normal n = normal_of(z[i]);
+          f[i] *= __builtin_fmaf(z[i], n.density, n.phi);
+        }
+      }
+      break;
+    case FH_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float q = logistic<T>(1.5957691216057308f * __builtin_fmaf(0.044715f * z[i] * z[i], z[i], z[i]));
+        const float du2 = 1.5957691216057308f * __builtin_fmaf(0.134145f * z[i], z[i], 1.f);
+        // q (1 - q) is 0 where exp has left its range, whatever z du2 is.
+        const float curve = q * (1.f - q);
+        f[i] *= curve > 0.f ? __builtin_fmaf(z[i] * du2, curve, q) : q;
+      }
+      break;
+    case FH_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float q = logistic<T>(z[i]), curve = q * (1.f - q);
+        f[i] *= curve > 0.f ? __builtin_fmaf(z[i], curve, q) : q;
+      }
+      break;
+    default: break;
   }
 }
 

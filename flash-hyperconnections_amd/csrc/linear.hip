@@ -39,25 +39,37 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
   float sums[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sums[i] = 0.f;
-  for (int64_t row = blockIdx.y * 4 + wave; row < a.rows; row += gridDim.y * 4) {
-    const U32x4 raw = load_row<T>(static_cast<const S*>(a.src) + row * a.src_stride, c, a.cols);
-    float f[V];
-    to_floats<T>(raw, f);
-    U32x4 rounded = raw;
-    if (a.saved != nullptr) {
-      const auto* z = static_cast<const typename Z::storage*>(a.saved) + row * a.cols;
-      float zf[V];
-      to_floats<Z>(load_row<Z>(z, c, a.cols), zf);
+  // Two rows at a time, for their loads to be on their way together.
+  const int64_t stride = static_cast<int64_t>(gridDim.y) * 4;
+  for (int64_t row = blockIdx.y * 4 + wave; row < a.rows; row += 2 * stride) {
+    const bool two = row + stride < a.rows;
+    U32x4 raw[2], saved[2];
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] *= slope<T>(zf[i], a.act);
-      rounded = from_floats<T>(f);
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1 && !two) break;
+      const int64_t r = row + u * stride;
+      raw[u] = load_row<T>(static_cast<const S*>(a.src) + r * a.src_stride, c, a.cols);
+      if (a.saved != nullptr)
+        saved[u] = load_row<Z>(static_cast<const typename Z::storage*>(a.saved) + r * a.cols, c, a.cols);
     }
-    if constexpr (Sums) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) sums[i] += c + i < a.cols ? f[i] : 0.f;
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1 && !two) break;
+      float f[V];
+      to_floats<T>(raw[u], f);
+      U32x4 rounded = raw[u];
+      if (a.saved != nullptr) {
+        float zf[V];
+        to_floats<Z>(saved[u], zf);
+        slope_times<T>(zf, a.act, f);
+        rounded = from_floats<T>(f);
+      }
+      if constexpr (Sums) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sums[i] += c + i < a.cols ? f[i] : 0.f;
+      }
+      if (a.out != nullptr && c < a.ld) store16(rounded, static_cast<S*>(a.out) + (row + u * stride) * a.ld + c);
     }
-    if (a.out != nullptr && c < a.ld)
-      *reinterpret_cast<U32x4*>(static_cast<S*>(a.out) + row * a.ld + c) = rounded;
   }
   if constexpr (Sums) {
     __shared__ float area[4][V][64];
