@@ -43,7 +43,8 @@ __device__ __forceinline__ U32x4 load_row(const typename T::storage* row, int c,
 }
 
 // 16 bytes at any element, with the nontemporal hint: results are larger than the
-// caches where their way to memory counts.
+// caches where their way to memory counts (layer norm 16384 x 4096 bf16: forward 56 us
+// without, 41 with; backward 85 and 67).
 template <typename S>
 __device__ __forceinline__ void store16(U32x4 w, S* to) {
   typedef U32x4 Unaligned __attribute__((aligned(2)));

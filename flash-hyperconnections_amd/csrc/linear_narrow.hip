@@ -9,6 +9,10 @@
 // busy.  Where the long operand is in rows the four wavefronts of a workgroup take
 // every fourth strip of the same rows and add their sums at the end; in columns they
 // take neighbouring 64 columns each.
+//
+// Taken up to 32 rows, one strip's worth of the short operand.  1 x 4096 x 16384 bf16 takes
+// 22 us (6.0 TB/s) in one launch, in 128 x 128 tiles 22 and 4 for the join; 16384 x 16384
+// into 16 takes 94 us (5.7 TB/s), 102 to 106 before in those tiles.
 #include <algorithm>
 #include <type_traits>
 
@@ -222,7 +226,8 @@ bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols) {
   int& tiles = long_a ? p.tiles_m : p.tiles_n;
   tiles = ((long_a ? p.m : p.n) + side - 1) / side;
   const int64_t steps = (p.k + kDepth - 1) / kDepth;
-  // Slices of at least four strips a wavefront until every compute unit has a workgroup.
+  // Slices of at least four strips a wavefront until every compute unit has a workgroup; in
+  // columns three for each (dW of 16384 x 16384 into 16: 149 us with 4 slices, 90 with 12).
   p.slices = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>((compute_units() * (cols ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
   return true;

@@ -10,6 +10,10 @@
 // every two of them go with reads of the phase to come or with a load, so that LDS and
 // the loads work beside the matrix cores.  Before the last phase the wavefronts meet:
 // by then this step's buffer has been read, and the next one's loads are there.
+//
+// 16384 x 4096 x 16384 bf16 (2.2 TFLOP) takes 1.93 ms forward with gelu and a saved sum,
+// 1.71 for dx and 1.68 for dW; the matrix cores are busy 64, 68 and 81% of the time, at a
+// clock of 1.6 to 1.8 GHz: on operands of zeros the three take 1.26, 1.55 and 1.33 ms.
 #include <algorithm>
 #include <type_traits>
 

@@ -177,7 +177,7 @@ FH_API int fh_layer_norm_backward(const void* x, int64_t x_stride, const void* g
 #define FH_ACT_SILU 4
 
 /* y = act(x weight^T + bias) + residual for x [rows, cols] and weight [outs, cols],
- * 1 <= cols, outs < 2^22.  bias ([outs] or NULL) is of bias_dtype: dtype or
+ * 0 <= rows < 2^30, 1 <= cols, outs < 2^22.  bias ([outs] or NULL) is of bias_dtype: dtype or
  * FH_DTYPE_F32; residual is [rows, outs] or NULL.  `saved` (may be NULL) receives
  * what the backward needs of the sum before the activation: [rows, outs], float for
  * FH_DTYPE_F32, half otherwise.  Sums are FP32. */
