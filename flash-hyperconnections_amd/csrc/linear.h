@@ -307,15 +307,18 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
+constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16-bit tile within 2^31 bytes
+
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
 // floats.  `dtype` is the operands' and the output's.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
-// The same for a product with at most 32 rows or columns; false for others.
-bool plan_narrow_product(ProductArgs& p, bool a_cols, bool b_cols);
+// The same for a product with at most 32 rows or columns, and in FP32 whole aligned
+// vectors; false for others.
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream);
-// 16-bit types.
 hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+// 16-bit types.
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
 
 }  // namespace fh

@@ -131,8 +131,6 @@ struct Laid {
   int64_t ld;
 };
 
-constexpr int64_t kMostStride = int64_t{1} << 22;  // 256 rows of a tile within 2^31 bytes
-
 // Whether the products read [rows, cols] as it is.
 bool as_it_is(const void* data, int64_t stride, int64_t cols, int dtype) {
   if (dtype == F32::code) return true;
