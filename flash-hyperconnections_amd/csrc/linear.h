@@ -70,17 +70,17 @@ __device__ __forceinline__ float logistic(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
 }
 
-// act(z) of eight; relu keeps a NaN.
-template <typename T>
-__device__ __forceinline__ void activate_eight(float (&v)[8], int act) {
+// act(z) of a vector; relu keeps a NaN.
+template <typename T, int V>
+__device__ __forceinline__ void activate(float (&v)[V], int act) {
   switch (act) {
     case FH_ACT_RELU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+      for (int k = 0; k < V; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
       break;
     case FH_ACT_GELU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < V; ++k) {
         if constexpr (T::code == F32::code) v[k] *= 0.5f * (1.f + erff(v[k] * 0.70710678118654752f));
         else v[k] *= normal_of(v[k]).phi;
       }
@@ -88,12 +88,12 @@ __device__ __forceinline__ void activate_eight(float (&v)[8], int act) {
     case FH_ACT_GELU_TANH:
       // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), without the difference of near values.
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < V; ++k)
         v[k] *= logistic<T>(1.5957691216057308f * __builtin_fmaf(0.044715f * v[k] * v[k], v[k], v[k]));
       break;
     case FH_ACT_SILU:
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= logistic<T>(v[k]);
+      for (int k = 0; k < V; ++k) v[k] *= logistic<T>(v[k]);
       break;
     default: break;
   }
@@ -140,95 +140,98 @@ __device__ __forceinline__ void slope_times(const float (&z)[V], int act, float 
   }
 }
 
-// Elements 0 .. count - 1 of eight, count at least 1.
-template <typename S>
-__device__ __forceinline__ void load_eight(const S* from, int count, S (&e)[8]) {
-  if (count >= 8) {
+// Elements 0 .. count - 1 of V, count at least 1.
+template <typename S, int V>
+__device__ __forceinline__ void load_some(const S* from, int count, S (&e)[V]) {
+  if (count >= V) {
     __builtin_memcpy(e, from, sizeof(e));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < count ? from[i] : S{};
+    for (int i = 0; i < V; ++i) e[i] = i < count ? from[i] : S{};
   }
 }
 // Nontemporal unless they are read again soon, as partial sums are.
-template <bool Soon = false, typename S>
-__device__ __forceinline__ void store_eight(const S (&e)[8], S* to, int count) {
-  if (Soon && count >= 8) {
+template <bool Soon = false, typename S, int V>
+__device__ __forceinline__ void store_some(const S (&e)[V], S* to, int count) {
+  if (Soon && count >= V) {
     __builtin_memcpy(to, e, sizeof(e));
-  } else if (count >= 8) {
+  } else if (count >= V) {
     U32x4 w[sizeof(e) / 16];
     __builtin_memcpy(w, e, sizeof(e));
 #pragma unroll
     for (size_t i = 0; i < sizeof(e) / 16; ++i) store16(w[i], to + i * (16 / sizeof(S)));
   } else {
 #pragma unroll
-    for (int i = 0; i < 7; ++i)
+    for (int i = 0; i < V - 1; ++i)
       if (i < count) to[i] = e[i];
   }
 }
 
-// Eight values rounded to the storage type.
-template <typename T>
-__device__ __forceinline__ void round_eight(const float (&f)[8], typename T::storage (&e)[8]) {
+// Values rounded to the storage type.
+template <typename T, int V>
+__device__ __forceinline__ void round_some(const float (&f)[V], typename T::storage (&e)[V]) {
   if constexpr (T::code == F32::code) {
     __builtin_memcpy(e, f, sizeof(e));
   } else {
+    static_assert(V == 8, "16 bytes");
     const U32x4 w{round_pair<T>(f[0], f[1]), round_pair<T>(f[2], f[3]), round_pair<T>(f[4], f[5]),
                   round_pair<T>(f[6], f[7])};
     __builtin_memcpy(e, &w, sizeof(e));
   }
 }
 
-// Eight neighbouring results (row i, columns j .. j + 7) on their way out: bias,
+// V neighbouring results (row i, columns j .. j + V - 1) on their way out: bias,
 // activation, residual; or into the slice's partial sums.
-template <typename T>
-__device__ __forceinline__ void finish_eight(const ProductArgs& p, int slice, int i, int j, float (&v)[8]) {
+template <typename T, int V>
+__device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int i, int j, float (&v)[V]) {
   using S = typename T::storage;
   using Z = Saved<T>;
   if (i >= p.m || j >= p.n) return;
   const int64_t at = static_cast<int64_t>(i) * p.n + j;
   const int left = p.n - j;
   if (p.slices > 1) {
-    store_eight<true>(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
+    store_some<true>(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
     return;
   }
   if (p.bias != nullptr) {
-    float b[8];
+    float b[V];
     if (p.bias_f32) {
-      load_eight(static_cast<const float*>(p.bias) + j, left, b);
+      load_some(static_cast<const float*>(p.bias) + j, left, b);
     } else {
-      S e[8];
-      load_eight(static_cast<const S*>(p.bias) + j, left, e);
+      S e[V];
+      load_some(static_cast<const S*>(p.bias) + j, left, e);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) b[k] = to_f32<T>(e[k]);
+      for (int k = 0; k < V; ++k) b[k] = to_f32<T>(e[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += b[k];
+    for (int k = 0; k < V; ++k) v[k] += b[k];
   }
   if (p.saved != nullptr) {
-    float z[8];
-    typename Z::storage e[8];
+    float z[V];
+    typename Z::storage e[V];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) z[k] = T::code == F32::code ? v[k] : clamp_saved(v[k]);
-    round_eight<Z>(z, e);
-    store_eight(e, static_cast<typename Z::storage*>(p.saved) + at, left);
+    for (int k = 0; k < V; ++k) z[k] = T::code == F32::code ? v[k] : clamp_saved(v[k]);
+    round_some<Z>(z, e);
+    store_some(e, static_cast<typename Z::storage*>(p.saved) + at, left);
   }
-  if (p.act != FH_ACT_NONE) activate_eight<T>(v, p.act);
-  S e[8];
+  if (p.act != FH_ACT_NONE) activate<T>(v, p.act);
+  S e[V];
   if (p.residual != nullptr) {
-    load_eight(static_cast<const S*>(p.residual) + static_cast<int64_t>(i) * p.ldr + j, left, e);
+    load_some(static_cast<const S*>(p.residual) + static_cast<int64_t>(i) * p.ldr + j, left, e);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += to_f32<T>(e[k]);
+    for (int k = 0; k < V; ++k) v[k] += to_f32<T>(e[k]);
   }
-  round_eight<T>(v, e);
-  store_eight(e, static_cast<S*>(p.out) + at, left);
+  round_some<T>(v, e);
+  store_some(e, static_cast<S*>(p.out) + at, left);
 }
 
 // Rows x 64 results of a wavefront on their way out through 256 bytes a row of its own
-// LDS, so that eight lanes store 64 neighbouring columns of a row.  16-byte chunk c of row r is at
-// place c ^ (r & 15), which spreads reads and writes over the banks.  (Stored from the
-// accumulators, a lane's four columns alone, a product of 16384 x 4096 x 16384 with
-// gelu spent a third of its time here.)
+// LDS, so that eight lanes (FP32: sixteen) store 64 neighbouring columns of a row, 16 bytes
+// each.  16-byte chunk c of row r is at place c ^ (r & 15), which spreads reads and writes
+// over the banks.  (Stored from the accumulators, a lane's four columns alone, a product of
+// 16384 x 4096 x 16384 with gelu spent a third of its time here.  FP32 in two stores of 16
+// bytes, 32 bytes a lane, each over every other half of 32 bytes, took 107 us for dx of
+// 16384 x 4096 into 16, where this takes 85 in the same kernel.)
 __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
   *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;
 }
@@ -236,13 +239,23 @@ template <typename T, int Rows>
 __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
                                               int lane) {
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
+  if constexpr (T::code == F32::code) {
 #pragma unroll 2
-  for (int it = 0; it < Rows / 8; ++it) {
-    const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
-    float v[8];
-    __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
-    __builtin_memcpy(v + 4, area + r * 256 + (((c + 1) ^ (r & 15)) << 4), 16);
-    finish_eight<T>(p, slice, row + r, col + 8 * (lane & 7), v);
+    for (int it = 0; it < Rows / 4; ++it) {
+      const int r = 4 * it + (lane >> 4), c = lane & 15;
+      float v[4];
+      __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
+      finish_some<T>(p, slice, row + r, col + 4 * c, v);
+    }
+  } else {
+#pragma unroll 2
+    for (int it = 0; it < Rows / 8; ++it) {
+      const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
+      float v[8];
+      __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
+      __builtin_memcpy(v + 4, area + r * 256 + (((c + 1) ^ (r & 15)) << 4), 16);
+      finish_some<T>(p, slice, row + r, col + 8 * (lane & 7), v);
+    }
   }
   asm volatile("" ::: "memory");
 }

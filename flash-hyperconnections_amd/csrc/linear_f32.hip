@@ -232,6 +232,51 @@ __global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ProductArgs p)
   finish_parked<F32, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
+// Sums of one step, at most 32 terms: one buffer, so that two workgroups share a compute
+// unit and one stores while the other loads.  Bound by the stores: dx of 16384 x 4096 into
+// 1 to 32 takes 56 to 63 us (268 MB), in the kernel above 79 to 85.
+template <bool ACols, bool BCols>
+__global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ProductArgs p) {
+  constexpr int kParked = 8 * 8192;  // 32 x 64 sums of each wavefront
+  static_assert(6 * kPanel<kTile> <= kParked, "the parts fit where the sums go");
+  __shared__ __attribute__((aligned(1024))) char lds[kParked];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Tile tile = tile_of(p, blockIdx.x);
+  const int m0 = tile.m * kTile, n0 = tile.n * kTile;
+  const uint32_t lds_a = lds_address(lds), lds_b = lds_a + 3 * kPanel<kTile>;
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
+  {
+    Mover<ACols, kTile> a;
+    Mover<BCols, kTile> b;
+    a.init(static_cast<const float*>(p.a), p.lda, m0, p.m, 0, p.k, lds_a);
+    b.init(static_cast<const float*>(p.b), p.ldb, n0, p.n, 0, p.k, lds_b);
+    a.fetch();
+    b.fetch();
+    a.put(0);
+    b.put(0);
+  }
+  __syncthreads();
+  Floats16 large[1][2], small[1][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) large[0][j][e] = small[0][j][e] = 0.f;
+  multiply<1>(Finder<ACols, kTile>(lds_a, wm, lane), Finder<BCols, kTile>(lds_b, wn, lane), 0, large, small);
+  __syncthreads();
+  char* area = lds + wave * 8192;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      Floats4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = large[0][j][4 * q + e] + small[0][j][4 * q + e];
+      park(area, lane & 31, 8 * j + 2 * q + (lane >> 5), v);
+    }
+  finish_parked<F32, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
+}
+
 template <int Tall>
 void run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(kThreads);
@@ -244,7 +289,12 @@ void run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
 
 hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
   if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
-  if (p.side_m == kTile) run<1>(p, a_cols, b_cols, stream);
+  if (p.side_m == kTile && p.k <= kDepth && p.slices == 1) {
+    const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n)), block(kThreads);
+    if (!a_cols && !b_cols) f32_outer_kernel<false, false><<<grid, block, 0, stream>>>(p);
+    if (!a_cols && b_cols) f32_outer_kernel<false, true><<<grid, block, 0, stream>>>(p);
+    if (a_cols && b_cols) f32_outer_kernel<true, true><<<grid, block, 0, stream>>>(p);
+  } else if (p.side_m == kTile) run<1>(p, a_cols, b_cols, stream);
   else run<2>(p, a_cols, b_cols, stream);
   return hipGetLastError();
 }

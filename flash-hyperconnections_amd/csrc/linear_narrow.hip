@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
       const int m = i / groups, n = i % groups * 8;
       float v[8];
       get(area, m, n, v);
-      finish_eight<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+      finish_some<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
     }
   } else {
     __syncthreads();
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    finish_eight<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+    finish_some<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
   }
 }
 

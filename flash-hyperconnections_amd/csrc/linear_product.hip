@@ -195,7 +195,7 @@ template <int Count>
 __device__ __forceinline__ void add_slices(const float*& from, int64_t size, int left, float (&sum)[8]) {
   float v[Count][8];
 #pragma unroll
-  for (int u = 0; u < Count; ++u, from += size) load_eight(from, left, v[u]);
+  for (int u = 0; u < Count; ++u, from += size) load_some(from, left, v[u]);
 #pragma unroll
   for (int u = 0; u < Count; ++u)
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
     if (slices & 4) add_slices<4>(from, size, left, sum);
     if (slices & 2) add_slices<2>(from, size, left, sum);
     if (slices & 1) add_slices<1>(from, size, left, sum);
-    finish_eight<T>(p, 0, row, col, sum);
+    finish_some<T>(p, 0, row, col, sum);
   }
 }
 
@@ -266,7 +266,7 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   const bool f32 = dtype == F32::code;
   if (plan_narrow_product(p, dtype, a_cols, b_cols)) return;
-  if (!f32 && p.k <= kStep) {
+  if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);
     p.slices = 1;
     return;

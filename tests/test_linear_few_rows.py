@@ -86,3 +86,15 @@ def test_large_and_small_values():
     g = torch.ones(3, 96, device="cuda")
     want, bound = _formula(x, w, None, None, None, g)
     _check(fh.linear(x, w), want[0], bound[0], "y")
+
+
+FEW_TERMS = [(130, 1, 200), (256, 31, 132), (300, 32, 129), (129, 33, 260), (500, 5, 70), (70, 32, 1000)]
+
+
+@pytest.mark.parametrize("m,k,n", FEW_TERMS)
+def test_sums_of_few_terms(m, k, n):
+    """One step of the sum and just more, tiles that end inside, results at every alignment."""
+    x, w, b, res, g = _inputs(m, k, n, torch.float32, seed=m)
+    _compare(x, w, b, res, "gelu_tanh", g)
+    x, w, b, res, g = _inputs(k, m, n, torch.float32, seed=n)
+    _compare(x, w, b, res, None, g)
