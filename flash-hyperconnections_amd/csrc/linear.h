@@ -36,8 +36,8 @@ struct ProductArgs {
 // What the backward needs of the sum z = x W^T + b: FP32 for FP32 results, and
 // FP16 for 16-bit ones, whatever they are.  Every activation's slope is 0 or 1 to
 // its last bit beyond +-65504, where values are clamped, and FP16's 11 bits keep
-// the slope's error well below that of rounding dz (bf16 would add a third to the
-// error of the weight's gradient).
+// the slope's error well below that of rounding dz: with gelu and normal z the
+// weight's gradient is off by 0.00233 with z exact or in FP16, by 0.00241 in bf16.
 template <typename T>
 using Saved = std::conditional_t<T::code == F32::code, F32, F16>;
 
@@ -230,7 +230,7 @@ __device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int
 // each.  16-byte chunk c of row r is at place c ^ (r & 15), which spreads reads and writes
 // over the banks.  (Stored from the accumulators, a lane's four columns alone, a product of
 // 16384 x 4096 x 16384 with gelu spent a third of its time here.  FP32 in two stores of 16
-// bytes, 32 bytes a lane, each over every other half of 32 bytes, took 107 us for dx of
+// bytes a lane, each instruction over every other 16 bytes, took 107 us for dx of
 // 16384 x 4096 into 16, where this takes 85 in the same kernel.)
 __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
   *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;

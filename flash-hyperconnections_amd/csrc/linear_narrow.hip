@@ -18,7 +18,7 @@
 // into bf16 parts on their way from LDS; they have to be whole aligned vectors, and go
 // through the tiles otherwise.  Calls, in the tiles before: 1 x 4096 x 16384 takes 46 us
 // forward (104) and 66 for dx (106), 1 x 4096 x 4096 20 (33) and 27 (33); dW of 16384 x
-// 4096 into 16 takes 70 (107).
+// 4096 into 16 takes 70 to 72 (107).
 #include <algorithm>
 #include <type_traits>
 
