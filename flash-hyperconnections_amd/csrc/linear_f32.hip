@@ -13,8 +13,9 @@
 // What bounds it are the matrix instructions and the splitting together, which share
 // the SIMDs' time: a step of 32 of the sum's terms takes a wavefront of the smaller tile
 // 24 matrix instructions and 150 others, 1.3 to 1.6 us; the larger tile's does twice
-// the products for 1.6 times the splitting in 2.1 to 2.7 us.  2048 x 4096 x 4096 takes
-// 405 us in the one and 352 us (195 TFLOP/s) in the other.
+// the products for 1.6 times the splitting in 2.1 to 2.7 us.  2048 x 4096 x 4096
+// took 405 us in the one and 352 in the other, and takes 337 (204 TFLOP/s) since results
+// leave in whole lines.
 #include <algorithm>
 
 #include "linear_parts.h"

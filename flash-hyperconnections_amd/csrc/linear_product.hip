@@ -3,9 +3,8 @@
 // slices.
 //
 // A compute unit holds one workgroup of eight wavefronts, whose buffers keep two or
-// three steps of 64 on their way (two workgroups with one step each on its way took
-// twice as long a step).  The wavefronts meet once a step.  What bounds the smaller tile
-// is the L2: 32 KB a step for 2 M multiply-adds, at about 10 TB/s.
+// three steps of 64 on their way.  The wavefronts meet once a step.  The smaller tile asks
+// the L2 for 32 KB a step of 1 M multiply-adds: 14 TB/s over 1024 x 4096 x 4096 in 37 us.
 #include <algorithm>
 #include <type_traits>
 

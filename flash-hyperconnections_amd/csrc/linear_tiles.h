@@ -17,8 +17,7 @@ __device__ __forceinline__ int swap_of(int k) { return 2 * (((k & 3) << 1) | ((k
 //
 // Each of eight wavefronts has kLoads loads a step, whose resources move with the steps.
 // Nothing here branches: a lane past the sum's end, in its last step or beyond it,
-// loads from out of range, which gives zeros.  (With branches for the edges a step
-// took 1000 cycles longer, whatever else it did.)
+// loads from out of range, which gives zeros.
 template <bool Cols, int Side>
 struct Feeder {
   static constexpr int kLoads = Side / 64;

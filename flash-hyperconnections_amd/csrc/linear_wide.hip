@@ -2,7 +2,7 @@
 // fill the card with them.
 //
 // Eight wavefronts of 128 x 64 results each, on 32 x 32 x 16 instructions (half as many
-// to issue as 16 x 16 x 32, for the same work): a wavefront reads 24 KB of LDS for 1 M
+// to issue as 16 x 16 x 32, for the same work): a wavefront reads 24 KB of LDS for 0.5 M
 // multiply-adds (64 x 64 results of a 128 x 128 tile's wavefront need a third more).
 // The sum runs in steps of 64 through two buffers, filled by loads that go to LDS
 // directly, in whole cache lines (steps of 32 in four buffers asked the L2 for half
