@@ -46,4 +46,8 @@ auto in_slices(int64_t batch, int64_t most, F f) {
   }
 }
 
+// Workgroups of `threads` threads that one launch may have: a dispatch counts fewer
+// than 2^32 work-items in a dimension.
+constexpr int64_t most_groups(int threads) { return (int64_t{1} << 31) / threads; }
+
 }  // namespace fh

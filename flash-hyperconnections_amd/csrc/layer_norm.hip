@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "fh_kernels.h"
+#include "fh_plan.h"
 #include "fh_vec.h"
 
 namespace fh {
@@ -350,14 +351,15 @@ __global__ __launch_bounds__(1024) void norm_params_long_kernel(NormArgs a) {
   out[a.cols + c] = db;
 }
 
-// Column sums of `partial` [count, width]: sixteen wavefronts take every
-// sixteenth row, their sums are added in order.  Columns below `split` go to
+// Column sums of `partial` [count, width] from column `begin` on: sixteen wavefronts take
+// every sixteenth row, their sums are added in order.  Columns below `split` go to
 // `first`, the others to `second`.
 __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int count, int64_t width,
-                                                           int64_t split, void* first, void* second, int dtype) {
+                                                           int64_t begin, int64_t split, void* first, void* second,
+                                                           int dtype) {
   __shared__ float area[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int64_t c = begin + static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float s = 0.f;
   if (c < width)
 #pragma unroll 8
@@ -375,15 +377,33 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial,
   if (dtype == F16::code) store_elem<F16>(out, at, s);
 }
 
+// launch(args, workgroups) for as many rows at a time as workgroups of `threads` threads and
+// `groups` rows may be in one launch, up to the first that fails.
+template <typename T, typename Launch>
+hipError_t in_row_ranges(const NormArgs& a, int groups, int threads, Launch launch) {
+  return in_slices(a.rows, most_groups(threads) * groups, [&](int64_t first, int64_t count) {
+    using S = typename T::storage;
+    NormArgs part = a;
+    part.x = static_cast<const S*>(a.x) + first * a.x_stride;
+    if (a.grad != nullptr) part.grad = static_cast<const S*>(a.grad) + first * a.grad_stride;
+    part.y = static_cast<S*>(a.y) + first * a.cols;
+    if (a.stats != nullptr) part.stats = a.stats + 2 * first;
+    part.rows = count;
+    launch(part, dim3(static_cast<uint32_t>((count + groups - 1) / groups)));
+    return hipGetLastError();
+  });
+}
+
 template <typename T, int WPR, int GROUPS, int NC>
 hipError_t fwd(const NormArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>((a.rows + GROUPS - 1) / GROUPS)), block(64 * WPR * GROUPS);
-  if (a.cols % kVec<T> == 0) {
-    norm_fwd_kernel<T, true, WPR, GROUPS, NC><<<grid, block, 0, stream>>>(a);
-  } else {
-    norm_fwd_kernel<T, false, WPR, GROUPS, NC><<<grid, block, 0, stream>>>(a);
-  }
-  return hipGetLastError();
+  constexpr int threads = 64 * WPR * GROUPS;
+  return in_row_ranges<T>(a, GROUPS, threads, [&](const NormArgs& part, dim3 grid) {
+    if (a.cols % kVec<T> == 0) {
+      norm_fwd_kernel<T, true, WPR, GROUPS, NC><<<grid, dim3(threads), 0, stream>>>(part);
+    } else {
+      norm_fwd_kernel<T, false, WPR, GROUPS, NC><<<grid, dim3(threads), 0, stream>>>(part);
+    }
+  });
 }
 
 template <typename T, bool Whole, int WPR, int NC>
@@ -415,9 +435,11 @@ int64_t vectors(int dtype, int64_t cols) {
 
 hipError_t launch_column_sums(const float* partial, int count, int64_t width, int64_t split, void* first,
                               void* second, int dtype, hipStream_t stream) {
-  column_sums_kernel<<<dim3(static_cast<uint32_t>((width + 63) / 64)), dim3(1024), 0, stream>>>(
-      partial, count, width, split, first, second, dtype);
-  return hipGetLastError();
+  return in_slices(width, most_groups(1024) * 64, [&](int64_t begin, int64_t columns) {
+    column_sums_kernel<<<dim3(static_cast<uint32_t>((columns + 63) / 64)), dim3(1024), 0, stream>>>(
+        partial, count, width, begin, split, first, second, dtype);
+    return hipGetLastError();
+  });
 }
 
 int norm_blocks(int dtype, int64_t rows, int64_t cols) {
@@ -430,8 +452,9 @@ hipError_t launch_norm(const NormArgs& a, int dtype, hipStream_t stream) {
   return with_type(dtype, [&](auto t) -> hipError_t {
     using T = decltype(t);
     if (nv > kMostVectors) {
-      norm_fwd_long_kernel<T><<<dim3(static_cast<uint32_t>(a.rows)), dim3(1024), 0, stream>>>(a);
-      return hipGetLastError();
+      return in_row_ranges<T>(a, 1, 1024, [&](const NormArgs& part, dim3 grid) {
+        norm_fwd_long_kernel<T><<<grid, dim3(1024), 0, stream>>>(part);
+      });
     }
     if (nv <= 64) return fwd<T, 1, 4, 1>(a, stream);
     if (nv <= 128) return fwd<T, 1, 4, 2>(a, stream);
@@ -453,7 +476,10 @@ hipError_t launch_norm_backward(const NormArgs& a, void* dweight, void* dbias, i
   hipError_t err = with_type(dtype, [&](auto t) -> hipError_t {
     using T = decltype(t);
     if (a.cols > kMostBackward) {
-      norm_bwd_long_kernel<T><<<dim3(static_cast<uint32_t>(a.rows)), dim3(1024), 0, stream>>>(a);
+      const hipError_t err = in_row_ranges<T>(a, 1, 1024, [&](const NormArgs& part, dim3 grid) {
+        norm_bwd_long_kernel<T><<<grid, dim3(1024), 0, stream>>>(part);
+      });
+      if (err != hipSuccess) return err;
       if (a.partial != nullptr)
         norm_params_long_kernel<T><<<dim3(static_cast<uint32_t>((a.cols + 1023) / 1024), blocks), dim3(1024), 0,
                                      stream>>>(a);
