@@ -50,4 +50,8 @@ auto in_slices(int64_t batch, int64_t most, F f) {
 // than 2^32 work-items in a dimension.
 constexpr int64_t most_groups(int threads) { return (int64_t{1} << 31) / threads; }
 
+// Rows of a product into n columns that one launch takes.  Its workgroups have 512 threads
+// for at least 128 x 128 results, or 256 for 64 rows of at most 32 columns.
+constexpr int64_t most_product_rows(int64_t n) { return most_groups(512) / ((n + 127) / 128) * 128; }
+
 }  // namespace fh

@@ -11,6 +11,7 @@
 // values before that rounding.
 #include <algorithm>
 
+#include "fh_plan.h"
 #include "linear.h"
 
 namespace fh {
@@ -155,15 +156,30 @@ hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols,
   return ws.dry() ? hipSuccess : launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
 }
 
-hipError_t multiply(ProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols,
+template <typename P>
+P* rows_on(P* p, int64_t bytes) {
+  return p != nullptr ? reinterpret_cast<P*>(reinterpret_cast<uintptr_t>(p) + bytes) : nullptr;
+}
+
+// The product `p` of operands a and b, in as many launches as its rows need.
+hipError_t multiply(const ProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols,
                     Workspace& ws, hipStream_t stream) {
-  p.a = a.data;
-  p.lda = a.ld;
-  p.b = b.data;
-  p.ldb = b.ld;
-  plan_product(p, dtype, a_cols, b_cols);
-  if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
-  return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream);
+  const int64_t size = dtype == F32::code ? 4 : 2;  // of the saved sums as well
+  // A in columns is a weight's gradient, with fewer than 2^22 rows.
+  return in_slices(p.m, a_cols ? p.m : most_product_rows(p.n), [&](int64_t first, int64_t count) {
+    ProductArgs part = p;
+    part.m = static_cast<int>(count);
+    part.a = rows_on(a.data, first * a.ld * size);
+    part.lda = a.ld;
+    part.b = b.data;
+    part.ldb = b.ld;
+    part.residual = rows_on(p.residual, first * p.ldr * size);
+    part.saved = rows_on(p.saved, first * p.n * size);
+    part.out = rows_on(p.out, first * p.n * size);
+    plan_product(part, dtype, a_cols, b_cols);
+    if (part.slices > 1) part.partial = ws.take<float>(static_cast<int64_t>(part.slices) * part.m * part.n);
+    return ws.dry() ? hipSuccess : launch_product(part, dtype, a_cols, b_cols, stream);
+  });
 }
 
 }  // namespace

@@ -1,4 +1,4 @@
-"""Layer norm over more rows and columns than one launch's work-items count.
+"""Layer norm and linear over more rows and columns than one launch's work-items count.
 
 A dispatch counts its work-items in 32 bits; longer calls go in several launches.
 """
@@ -31,6 +31,17 @@ def test_workgroups_of_a_launch(tmp_path):
         CHECK(status == 0 && next == rows);
       }
     }
+  }
+""")
+
+
+def test_rows_of_a_product_launch(tmp_path):
+    _run(tmp_path, """
+  for (int64_t n = 1; n < (int64_t{1} << 22); n += n < 300 ? 1 : n / 3) {
+    const int64_t rows = fh::most_product_rows(n);
+    CHECK(rows >= (int64_t{1} << 14) && rows % 128 == 0);
+    CHECK(rows / 128 * ((n + 127) / 128) * 512 < (int64_t{1} << 32));
+    if (n <= 32) CHECK(rows / 64 * 256 < (int64_t{1} << 32));
   }
 """)
 
@@ -68,3 +79,21 @@ def test_layer_norm_parameters_of_more_columns_than_a_launch():
     assert torch.equal(db, g[0])
     want = g[0].float() * n[0].detach().float()  # n is rounded to bf16, dw as well
     assert bool(((dw.float() - want).abs() <= 2 * half_ulp(dw.dtype) * want.abs() + floor(dw.dtype)).all())
+
+
+@gpu
+def test_linear_of_more_rows_than_a_launch():
+    """2^29 + 70 rows of 8 into 1: every row has the bits that it has in a shorter call."""
+    rows, part = 2**29 + 70, 2**26
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-8, 9, (rows, 8), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    w, b, res, g = _normal(1, 8, seed=2), _normal(1, seed=3), _normal(rows, 1, seed=4), _normal(rows, 1, seed=5)
+    leaf = x.requires_grad_()
+    y = fh.linear(leaf, w, b, activation="silu", residual=res)
+    (dx,) = torch.autograd.grad(y, leaf, g)
+    y = y.detach()
+    for first in range(0, rows, part):
+        piece = x[first : first + part].detach().requires_grad_()
+        want = fh.linear(piece, w, b, activation="silu", residual=res[first : first + part])
+        (want_dx,) = torch.autograd.grad(want, piece, g[first : first + part])
+        assert torch.equal(y[first : first + part], want) and torch.equal(dx[first : first + part], want_dx)
