@@ -9,7 +9,8 @@ On a gfx950 device with float32 / float16 / bfloat16 operands of one type (weigh
 the bias of the product may be float32 beside 16-bit operands) both run hand-written HIP kernels,
 forward and backward.  Rows are read in place whatever their stride, so one stream of a
 ``[tokens, streams, width]`` tensor needs no copy.  Everything else -- CPU tensors, other types,
-tensor subclasses, function transforms, forward-mode tangents -- is composed from native PyTorch
+tensor subclasses, function transforms, forward-mode tangents, 2**31 rows or 2**30 columns of a norm,
+2**30 rows or 2**22 columns or outputs of a product -- is composed from native PyTorch
 operations, float16 and bfloat16 in float32; a backward that builds a graph takes differentiable
 native pieces.
 """
@@ -32,7 +33,9 @@ _ACTIVATIONS = {
 }
 _NORM = torch.ops.flash_hypercons._layer_norm
 _LINEAR = torch.ops.flash_hypercons._linear
-_MOST = 2**22  # columns and outputs of a linear layer's kernels
+# Rows and columns that the kernels take fewer than; a linear layer's outputs as its columns.
+_NORM_ROWS, _NORM_COLS = 2**31, 2**30
+_LINEAR_ROWS, _LINEAR_COLS = 2**30, 2**22
 
 
 def _plain(t: Optional[torch.Tensor]) -> bool:
@@ -45,8 +48,8 @@ def _plain(t: Optional[torch.Tensor]) -> bool:
     )
 
 
-def _eligible(x: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
-    """Operands for the HIP kernels, which check their shapes themselves."""
+def _eligible(rows: int, cols: int, x: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """Operands for the HIP kernels, which check their shapes themselves; x has fewer rows and columns than these."""
     return (
         x is not None
         and _plain(x)
@@ -54,7 +57,8 @@ def _eligible(x: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
         and torch.version.hip is not None
         and not torch._C._are_functorch_transforms_active()
         and x.ndim >= 1
-        and x.shape[-1] >= 1
+        and 1 <= x.shape[-1] < cols
+        and x.numel() // x.shape[-1] < rows
         and _device_supported(x.device.index)
     )
 
@@ -111,7 +115,7 @@ def layer_norm(
     weight and bias are [C] or None, of x's type or float32.  Differentiable in all three; the
     parameters' gradients are summed over the rows in a fixed order.
     """
-    if _eligible(x, weight, bias):
+    if _eligible(_NORM_ROWS, _NORM_COLS, x, weight, bias):
         return _NORM(x, weight, bias, eps)
     y = torch.nn.functional.layer_norm(_wide(x), x.shape[-1:], _wide(weight), _wide(bias), eps)
     return y.to(x.dtype)
@@ -134,7 +138,12 @@ def linear(
     if activation not in _ACTIVATIONS:
         raise ValueError(f"linear: unknown activation {activation!r}; one of {', '.join(map(repr, _ACTIVATIONS))}")
     code, native = _ACTIVATIONS[activation]
-    if weight is not None and _eligible(x, weight, bias, residual) and weight.ndim == 2 and 0 < weight.shape[0] < _MOST > x.shape[-1]:
+    if (
+        weight is not None
+        and _eligible(_LINEAR_ROWS, _LINEAR_COLS, x, weight, bias, residual)
+        and weight.ndim == 2
+        and 1 <= weight.shape[0] < _LINEAR_COLS
+    ):
         return _LINEAR(x, weight, bias, residual, code)
     y = native(torch.nn.functional.linear(_wide(x), _wide(weight), _wide(bias)))
     if residual is not None:
