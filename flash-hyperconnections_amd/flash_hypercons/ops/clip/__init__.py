@@ -7,13 +7,14 @@ up to 96 tensors and two more for each further 96.
 
 On a gfx950 device with float32 / float16 / bfloat16 tensors (of one device, types mixed as they
 come) and a norm of 1, 2 or infinity, the HIP kernels run: sums are float64 and in one fixed order,
-the norm is a float32 scalar on the device, and nothing waits for it.  Everything else is composed
-from native PyTorch operations.
+the norm is a float32 scalar on the device, and nothing waits for it.  Everything else, function
+transforms and forward-mode tangents among it, is composed from native PyTorch operations.
 """
 
 from typing import Iterable, List, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from flash_hypercons import _C  # noqa: F401  (registers the flash_hypercons::* operators)
 from flash_hypercons.ops.matrix_exp import _device_supported
@@ -25,7 +26,7 @@ Tensors = Union[torch.Tensor, Iterable[torch.Tensor]]
 
 
 def _eligible(tensors: List[torch.Tensor], norm_type: float) -> bool:
-    if norm_type not in _TYPES or torch.version.hip is None:
+    if norm_type not in _TYPES or torch.version.hip is None or torch._C._are_functorch_transforms_active():
         return False
     device = tensors[0].device
     return (
@@ -35,6 +36,7 @@ def _eligible(tensors: List[torch.Tensor], norm_type: float) -> bool:
             and type(t) in (torch.Tensor, torch.nn.Parameter)
             for t in tensors
         )
+        and (forward_ad._current_level < 0 or all(forward_ad.unpack_dual(t).tangent is None for t in tensors))
         and _device_supported(device.index)
     )
 
