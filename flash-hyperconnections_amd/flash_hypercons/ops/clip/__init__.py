@@ -67,7 +67,11 @@ def _grad_norm_fake(tensors, norm_type):
 
 @torch.library.register_fake("flash_hypercons::_clip_grads")
 def _clip_grads_fake(tensors, max_norm, norm_type):
-    return [torch.empty_like(t) for t in tensors], tensors[0].new_empty((), dtype=torch.float32)
+    # Dense tensors keep their strides, and the others' results are contiguous.
+    dense = torch.ops.aten.is_non_overlapping_and_dense
+    clipped = [torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+               if not t.is_neg() and dense(t) else t.new_empty(t.shape) for t in tensors]
+    return clipped, tensors[0].new_empty((), dtype=torch.float32)
 
 
 @torch.library.register_fake("flash_hypercons::_clip_grads_")

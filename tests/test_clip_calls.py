@@ -40,3 +40,49 @@ def test_forward_mode_tangents(device):
     want = (g.double() * v.double()).sum() / g.double().norm()
     assert tangent is not None
     assert abs(tangent.double() - want) <= 2.0**-20 * (g * v).double().abs().sum() / g.double().norm()
+
+
+# ---- tracing ---------------------------------------------------------------------------
+
+
+LAYOUTS = {
+    "rows": lambda t: t,
+    "columns": lambda t: t.t(),
+    "permuted": lambda t: t.view(3, 4, 90).permute(2, 0, 1),
+    "gapped": lambda t: t[:, 1:40],
+    "gapped columns": lambda t: t[:, 1:40].t(),
+    "every second": lambda t: t[:, ::2],
+    "expanded": lambda t: t[:1].expand(5, 90),
+    "one row": lambda t: t[:1, :40],
+    "one column": lambda t: t[:, :1],
+    "empty": lambda t: t[:0, :4].t(),
+    "scalar": lambda t: t[0, 0],
+    "negated": lambda t: torch.complex(t, t).conj().imag,
+}
+
+
+@gpu
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_traced_results_have_the_real_strides(layout):
+    t = LAYOUTS[layout](torch.zeros(12, 90, device="cuda"))
+    with torch.no_grad():
+        real, _ = fh.clip_grad_norm([t], 1.0)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode() as mode:
+        fake, norm = torch.ops.flash_hypercons._clip_grads([mode.from_tensor(t)], 1.0, 2.0)
+    assert fake[0].shape == real[0].shape and fake[0].stride() == real[0].stride() and norm.shape == ()
+
+
+@gpu
+def test_compiled_clipping_matches():
+    wide, flat = _normal(12, 90, device="cuda"), _normal(33, device="cuda", seed=1, dtype=torch.bfloat16)
+    grads = [wide[:, 1:40].t(), wide[:, 50:].t(), flat]
+
+    def clip(*g):
+        clipped, norm = fh.clip_grad_norm(g, 0.5)
+        return [c.view(-1) if c.is_contiguous() else c.t() for c in clipped], norm
+
+    got, norm = torch.compile(clip, fullgraph=True, backend="aot_eager")(*grads)
+    want, want_norm = clip(*grads)
+    assert torch.equal(norm, want_norm) and all(map(torch.equal, got, want))
