@@ -267,6 +267,8 @@ struct Arrays {
         copies.push_back(flat);
         if (inplace) back.emplace_back(flat, t);
       }
+      // What is written in place has storage of its own from here on, where a lazy clone shared it.
+      data.push_back(inplace ? flat.mutable_data_ptr() : flat.const_data_ptr());
       if (inplace && t.numel() > 0) {
         const auto at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
         int64_t last = 0;
@@ -277,7 +279,6 @@ struct Arrays {
         // Gapped tensors may interleave; they are copied, and not looked at here.
         if (t.is_non_overlapping_and_dense()) spans.emplace_back(at, at + (last + 1) * t.element_size());
       }
-      data.push_back(flat.const_data_ptr());
       sizes.push_back(flat.numel());
       dtypes.push_back(dtype_code(t.scalar_type()));
     }

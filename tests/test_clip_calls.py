@@ -86,3 +86,19 @@ def test_compiled_clipping_matches():
     got, norm = torch.compile(clip, fullgraph=True, backend="aot_eager")(*grads)
     want, want_norm = clip(*grads)
     assert torch.equal(norm, want_norm) and all(map(torch.equal, got, want))
+
+
+# ---- copy-on-write ---------------------------------------------------------------------
+
+
+@gpu
+def test_lazy_clones_keep_their_own_values():
+    kept = _normal(300, device="cuda")
+    before = kept.clone()
+    params = [torch.nn.Parameter(torch.zeros_like(kept)) for _ in range(2)]
+    for p in params:
+        p.grad = torch._lazy_clone(kept)
+    want, want_norm = fh.clip_grad_norm([before, before], 0.5)
+    norm = fh.clip_grad_norm_(params, 0.5)
+    assert torch.equal(kept, before)
+    assert torch.equal(norm, want_norm) and all(torch.equal(p.grad, w) for p, w in zip(params, want))
