@@ -42,18 +42,22 @@ def _eligible(tensors: List[torch.Tensor], norm_type: float) -> bool:
 
 
 def _native_norm(tensors: List[torch.Tensor], norm_type: float) -> torch.Tensor:
+    """In float64, which the factor of float64 gradients is made from; callers get it in float32."""
     device = tensors[0].device
     parts = [torch.linalg.vector_norm(t, norm_type, dtype=torch.float64).to(device) for t in tensors if t.numel()]
-    return torch.linalg.vector_norm(torch.stack(parts), norm_type).float() if parts else torch.zeros((), device=device)
+    if not parts:
+        return torch.zeros((), device=device, dtype=torch.float64)
+    return torch.linalg.vector_norm(torch.stack(parts), norm_type)
 
 
 def _factor(norm: torch.Tensor, max_norm: float) -> torch.Tensor:
-    return (max_norm / (norm.double() + 1e-6)).clamp(max=1.0).float()
+    return (max_norm / (norm + 1e-6)).clamp(max=1.0)
 
 
 def _scaled(t: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
-    f = factor.to(t.device)
-    return (t * f) if t.dtype in (torch.float32, torch.float64) else (t.float() * f).to(t.dtype)
+    if t.dtype == torch.float64:
+        return t * factor.to(t.device)
+    return (t.float() * factor.to(t.device, torch.float32)).to(t.dtype)
 
 
 def _listed(tensors: Tensors) -> List[torch.Tensor]:
@@ -85,7 +89,7 @@ def grad_norm(tensors: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     listed, norm_type = _listed(tensors), float(norm_type)
     if not listed:
         return torch.zeros(())
-    return _OPS._grad_norm(listed, norm_type) if _eligible(listed, norm_type) else _native_norm(listed, norm_type)
+    return _OPS._grad_norm(listed, norm_type) if _eligible(listed, norm_type) else _native_norm(listed, norm_type).float()
 
 
 @torch.no_grad()
@@ -100,7 +104,7 @@ def clip_grad_norm(
         return _OPS._clip_grads(listed, max_norm, norm_type)
     norm = _native_norm(listed, norm_type)
     factor = _factor(norm, max_norm)
-    return [_scaled(t, factor) for t in listed], norm
+    return [_scaled(t, factor) for t in listed], norm.float()
 
 
 @torch.no_grad()
@@ -126,7 +130,7 @@ def clip_grad_norm_(
     factor = _factor(norm, max_norm)
     for g in grads:
         g.copy_(_scaled(g, factor))
-    return norm
+    return norm.float()
 
 
 __all__ = ["clip_grad_norm", "clip_grad_norm_", "grad_norm"]

@@ -102,3 +102,22 @@ def test_lazy_clones_keep_their_own_values():
     norm = fh.clip_grad_norm_(params, 0.5)
     assert torch.equal(kept, before)
     assert torch.equal(norm, want_norm) and all(torch.equal(p.grad, w) for p, w in zip(params, want))
+
+
+# ---- wide types, which go native -------------------------------------------------------
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e60, 1e-60])
+@pytest.mark.parametrize("device", DEVICES)
+def test_float64_gradients_are_scaled_in_float64(device, scale):
+    """The norm and the factor are a few FP64 roundings off, 2^-53 each, and sums of 58 squares."""
+    grads = [_normal(40, device=device, dtype=torch.float64) * scale,
+             _normal(2, 9, device=device, seed=1, dtype=torch.float64) * scale]
+    norm = torch.cat([g.reshape(-1) for g in grads]).norm()
+    limit = 0.25 * float(norm)
+    factor = limit / (norm + 1e-6) if scale >= 1.0 else torch.ones_like(norm)
+    clipped, got = fh.clip_grad_norm(grads, limit if scale >= 1.0 else 1.0)
+    assert got.dtype == torch.float32 and torch.equal(got, norm.float())
+    for c, g in zip(clipped, grads):
+        assert c.dtype == torch.float64
+        torch.testing.assert_close(c, g * factor, rtol=2.0**-45, atol=0)
