@@ -44,7 +44,10 @@ def _eligible(tensors: List[torch.Tensor], norm_type: float) -> bool:
 def _native_norm(tensors: List[torch.Tensor], norm_type: float) -> torch.Tensor:
     """In float64, which the factor of float64 gradients is made from; callers get it in float32."""
     device = tensors[0].device
-    parts = [torch.linalg.vector_norm(t, norm_type, dtype=torch.float64).to(device) for t in tensors if t.numel()]
+    parts = [
+        torch.linalg.vector_norm(t, norm_type, dtype=torch.complex128 if t.is_complex() else torch.float64).to(device)
+        for t in tensors if t.numel()
+    ]  # fmt: skip
     if not parts:
         return torch.zeros((), device=device, dtype=torch.float64)
     return torch.linalg.vector_norm(torch.stack(parts), norm_type)
@@ -55,9 +58,10 @@ def _factor(norm: torch.Tensor, max_norm: float) -> torch.Tensor:
 
 
 def _scaled(t: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
-    if t.dtype == torch.float64:
+    if t.dtype in (torch.float64, torch.complex128):
         return t * factor.to(t.device)
-    return (t.float() * factor.to(t.device, torch.float32)).to(t.dtype)
+    factor = factor.to(t.device, torch.float32)
+    return t * factor if t.is_complex() else (t.float() * factor).to(t.dtype)
 
 
 def _listed(tensors: Tensors) -> List[torch.Tensor]:

@@ -121,3 +121,18 @@ def test_float64_gradients_are_scaled_in_float64(device, scale):
     for c, g in zip(clipped, grads):
         assert c.dtype == torch.float64
         torch.testing.assert_close(c, g * factor, rtol=2.0**-45, atol=0)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, 3.0, float("inf")])
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128], ids=str)
+def test_complex_gradients_are_scaled_whole(dtype, p):
+    real, imag = _normal(40), _normal(40, seed=1)
+    g = torch.complex(real, imag).to(dtype)
+    norm = torch.linalg.vector_norm(g.to(torch.complex128), p)
+    clipped, got = fh.clip_grad_norm([g], 0.25 * float(norm), p)
+    torch.testing.assert_close(got.double(), norm, rtol=2.0**-22, atol=0)
+    torch.testing.assert_close(clipped[0], (g.to(torch.complex128) * 0.25).to(dtype), rtol=1e-5, atol=0)
+    param = torch.nn.Parameter(torch.zeros_like(g))
+    param.grad = g.clone()
+    fh.clip_grad_norm_([param], 0.25 * float(norm), p)
+    assert torch.equal(param.grad, clipped[0])
