@@ -49,9 +49,12 @@ __device__ __forceinline__ float clamp_saved(float z) {
 }
 
 // Phi(z) and the normal density at z, by formula 7.1.26 of Abramowitz and Stegun's
-// handbook, whose error of 1.5e-7 is far below the last bit of a 16-bit result.  The
-// exponential it needs is the density's as well.  A gelu adds 74 us to 16384 x 4096
-// x 16384 bf16 so, and 169 with the library's erff.
+// handbook: Phi is off by 7e-8 at most, about the rounding of 1 + erf in FP32.  Far out on
+// the negative side that is no longer small beside gelu itself: relative to it the formula
+// errs by 5e-4 at z = -4, where gelu is -1e-4, by 4e-3 at -6 (-6e-9) and 4e-2 at -13, where
+// 1 + erf in FP32 has lost every digit from -5.5 on.  The exponential it needs is the
+// density's as well.  A gelu adds 74 us to 16384 x 4096 x 16384 bf16 so, and 169 with
+// the library's erff.
 struct Normal {
   float phi, density;
 };
