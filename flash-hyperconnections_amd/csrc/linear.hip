@@ -8,7 +8,10 @@
 //
 // dz is formed by the same kernel, together with the column sums that make db.  It is
 // rounded to the storage type, as operands of 16-bit products have to be; db adds the
-// values before that rounding.
+// values before that rounding.  With an activation this doubles the variance of dx's and
+// dW's errors: 0.0024 of their size in bf16 and 0.0003 in FP16 (root mean square, against 64
+// bits, gelu and normal operands), where the results' own rounding makes 0.0017 and 0.0002.
+// Without one dz is the upstream gradient itself and loses nothing.
 #include <algorithm>
 
 #include "fh_plan.h"

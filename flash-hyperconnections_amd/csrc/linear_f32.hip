@@ -10,12 +10,14 @@
 // they are, four bytes an element at any alignment, and half as many panels go through
 // LDS as if each product of parts read its own.
 //
-// What bounds it are the matrix instructions and the splitting together, which share
-// the SIMDs' time: a step of 32 of the sum's terms takes a wavefront of the smaller tile
-// 24 matrix instructions and 150 others, 1.3 to 1.6 us; the larger tile's does twice
-// the products for 1.6 times the splitting in 2.1 to 2.7 us.  2048 x 4096 x 4096
-// took 405 us in the one and 352 in the other, and takes 337 (204 TFLOP/s) since results
-// leave in whole lines.
+// A step of 32 of the sum's terms takes a wavefront of the smaller tile 24 matrix
+// instructions and 150 others, 1.3 to 1.6 us; the larger tile's does twice the products for
+// 1.6 times the splitting in 2.1 to 2.7 us.  2048 x 4096 x 4096 took 405 us in the one and
+// 352 in the other, and takes 337 (204 TFLOP/s) since results leave in whole lines.  Smaller
+// products stay well below that: in the three of 1500 x 1027 x 771, 63 to 108 tiles in 2 to
+// 4 slices, a compute unit has one workgroup of 11 to 13 steps, and the matrix cores are busy
+// 36 to 38% of the time.  What of splitting, LDS writes, barriers and the joins of slices
+// takes the rest was not separated.
 #include <algorithm>
 
 #include "linear_parts.h"

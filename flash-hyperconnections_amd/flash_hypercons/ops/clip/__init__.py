@@ -118,6 +118,9 @@ def clip_grad_norm_(
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)); returns the norm.
 
     Parameters without a gradient are left out; gradients that the norm allows stay as they are.
+    Where the HIP kernels run, dense gradients that share memory (one listed twice among them) raise
+    before anything is scaled; composed natively, as in torch, each mention scales the memory again.
+    Gradients with gaps are copied and not compared.
     ``error_if_nonfinite`` raises before anything is scaled, and waits for the norm to do so.
     """
     grads = [p.grad for p in _listed(parameters) if p.grad is not None]
