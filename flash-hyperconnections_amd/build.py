@@ -49,10 +49,12 @@ KERNEL_SOURCES = [
     "linear_narrow.hip",
     "linear_f32.hip",
     "grad_clip.hip",
+    "embedding.hip",
+    "cross_entropy.hip",
     "fh_capi.cpp",
 ]
 
-EXTENSION_SOURCES = ["register.cpp", "register_block.cpp"]
+EXTENSION_SOURCES = ["register.cpp", "register_block.cpp", "register_ends.cpp"]
 
 # -ffp-contract=off: every fused multiply-add in the kernels is written out.
 # The packed-FP32 feature is switched off (no packed FP32 instructions are

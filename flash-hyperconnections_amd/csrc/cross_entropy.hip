@@ -1,0 +1,480 @@
+// Softmax cross entropy of a linear layer's results, which are never kept:
+//   z_i = W x_i + b,  lse_i = log(sum over v of exp(z_iv)),  loss_i = lse_i - z_i[t_i];
+//   dz_iv = f_i (exp(z_iv - lse_i) - [v = t_i]),  dx = dz W,  dW = dz^T x,  db = sum over i of dz_i,
+// where f_i is the upstream gradient of loss_i.
+//
+// Rows without a target take part in nothing, so the others are gathered first
+// (rows_kernel, gather_kernel), and the products after that have as many rows as there
+// are targets; what they cost goes by the targets and not by the batch.  How many there are
+// stays on the device: launches are sized for all, and workgroups past the last row end.
+//
+// Forward: the products' workgroups reduce every 64 logits of a row to their maximum and
+// the sum of exponentials beside it, and pick the target's; lse_kernel joins these.
+// Backward: the vocabulary goes in pieces.  A piece's logits are formed again, turned into
+// dz on their way out, and multiplied into dx, a running FP32 sum over the pieces, and dW,
+// whose rows the piece completes.  The logits' second product is what not keeping them
+// costs: 8 operations a weight and row where 6 would do.
+//
+// In FP16 dz is held times a power of two that puts the largest |f_i| between 2^14 and 2^15:
+// probabilities down to 2^-39 of the largest factor stay above zero then.  The results' last
+// step divides by it, exactly.  The other types have the range without.
+#include <algorithm>
+
+#include "fh_plan.h"
+#include "linear.h"
+
+namespace fh {
+namespace {
+
+constexpr int kRowThreads = 1024;
+
+struct RowsArgs {
+  const int64_t* targets;
+  int64_t ignore;
+  int rows, vocab;
+  int* live;          // how many rows have a target
+  int* index;         // [rows] which ones, in their order
+  int* label;         // [rows] their targets; -1 for one that is out of range
+  float* losses;      // forward: [rows] zeroed where there is no target, or null
+  // backward
+  const float* grad;  // of the loss, or of each row's
+  int per_row, mean, scaled;
+  const float* lse;   // [rows] in the order of `index`
+  float2* row;        // [rows] lse and the factor
+  float* scale;       // what undoes the factors' power of two
+};
+
+// Sum over the workgroup of a count for each thread, and of those before it.
+__device__ __forceinline__ int before(bool mine, int& total, int (&area)[2][kRowThreads / 64], int& turn) {
+  const uint64_t mask = __ballot(mine);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* counts = area[turn];
+  turn ^= 1;  // what the others may still read stays
+  if (lane == 0) counts[wave] = __popcll(mask);
+  __syncthreads();
+  int sum = 0, mine_before = 0;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) {
+    if (w == wave) mine_before = sum;
+    sum += counts[w];
+  }
+  total = sum;
+  return mine_before + lanes_below(mask);
+}
+
+// One workgroup: targets are few beside anything else here.
+template <bool Backward>
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
+  __shared__ int area[2][kRowThreads / 64];
+  __shared__ float most[kRowThreads / 64];
+  int turn = 0, done = 0, total;
+  float power = 1.f, mean = 1.f;
+  if constexpr (Backward) {
+    // The largest finite factor's size, and how many factors there are.
+    float largest = 0.f;
+    int count = 0;
+    for (int64_t r = threadIdx.x; r < a.rows; r += kRowThreads) {
+      if (a.targets[r] == a.ignore) continue;
+      ++count;
+      const float g = __builtin_fabsf(a.grad[a.per_row ? r : 0]);
+      if (g < __builtin_inff()) largest = __builtin_fmaxf(largest, g);
+    }
+    __shared__ int counts[kRowThreads / 64];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      largest = __builtin_fmaxf(largest, __shfl_xor(largest, d));
+      count += __shfl_xor(count, d);
+    }
+    if ((threadIdx.x & 63) == 0) {
+      most[threadIdx.x >> 6] = largest;
+      counts[threadIdx.x >> 6] = count;
+    }
+    __syncthreads();
+    count = 0;
+    for (int w = 0; w < kRowThreads / 64; ++w) {
+      largest = __builtin_fmaxf(largest, most[w]);
+      count += counts[w];
+    }
+    mean = a.mean ? static_cast<float>(count) : 1.f;
+    largest /= mean;
+    if (a.scaled && largest > 0.f) {
+      const int e = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
+      power = __builtin_ldexpf(1.f, e < -112 ? -112 : e > 126 ? 126 : e);
+    }
+    if (threadIdx.x == 0) *a.scale = 1.f / power;
+  }
+  for (int64_t first = 0; first < a.rows; first += kRowThreads) {
+    const int64_t r = first + threadIdx.x;
+    const int64_t t = r < a.rows ? a.targets[r] : a.ignore;
+    const bool mine = r < a.rows && t != a.ignore;
+    const int at = done + before(mine, total, area, turn);
+    done += total;
+    if (mine) {
+      const bool valid = t >= 0 && t < a.vocab;
+      a.index[at] = static_cast<int>(r);
+      a.label[at] = valid ? static_cast<int>(t) : -1;
+      if constexpr (Backward) {
+        const float f = valid ? a.grad[a.per_row ? r : 0] / mean * power : __builtin_nanf("");
+        a.row[at] = make_float2(a.lse[at], f);
+      }
+    } else if (!Backward && r < a.rows && a.losses != nullptr) {
+      a.losses[r] = 0.f;
+    }
+  }
+  if (threadIdx.x == 0) *a.live = done;
+}
+
+struct GatherArgs {
+  const void* src;    // [rows, cols], rows src_stride elements apart
+  int64_t src_stride;
+  const int* live;
+  const int* index;
+  void* out;          // [rows, ld], zero past cols
+  int64_t ld;
+  int cols;
+};
+
+// A wavefront to each row that has a target.
+template <typename T>
+__global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
+  using S = typename T::storage;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= *a.live) return;
+  const S* from = static_cast<const S*>(a.src) + a.index[row] * a.src_stride;
+  S* to = static_cast<S*>(a.out) + row * a.ld;
+  for (int c = (threadIdx.x & 63) * kVec<T>; c < a.ld; c += 64 * kVec<T>) {
+    const U32x4 w = load_row<T>(from, c, a.cols);
+    __builtin_memcpy(to + c, &w, 16);
+  }
+}
+
+// Zeros for the rows without a target, a wavefront to each.
+template <typename T>
+__global__ __launch_bounds__(256) void zero_rows_kernel(const int64_t* targets, int64_t ignore, int64_t rows, int cols,
+                                                        void* out) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows || targets[row] != ignore) return;
+  auto* to = static_cast<typename T::storage*>(out) + row * cols;
+  for (int c = (threadIdx.x & 63) * kVec<T>; c < cols; c += 64 * kVec<T>) store_row<T>(U32x4{0, 0, 0, 0}, to, c, cols);
+}
+
+struct LseArgs {
+  const float2* stats;  // [groups, ld]
+  int64_t ld;
+  int groups, rows;
+  const int* live;
+  int row0;
+  const int* label;
+  const int* index;
+  const float* chosen;
+  float* lse;           // [rows] in the order of `index`
+  float* losses;        // likewise, or by their rows
+  int by_row;
+};
+
+// Joins two pairs of a maximum and a sum of exponentials beside it.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float m = __builtin_fmaxf(a.x, b.x), from = m == -__builtin_inff() ? 0.f : m;
+  return make_float2(m, a.y * expf(a.x - from) + b.y * expf(b.x - from));
+}
+
+// Sixteen wavefronts, `across` rows (a power of two, up to 64) by 1024 / across groups.
+__global__ __launch_bounds__(1024) void lse_kernel(LseArgs a, int across) {
+  __shared__ float2 area[1024];
+  const int live = *a.live - a.row0, rows = live < a.rows ? live : a.rows;
+  const int row = static_cast<int>(blockIdx.x) * across + (threadIdx.x & (across - 1));
+  if (static_cast<int>(blockIdx.x) * across >= rows) return;  // the whole workgroup
+  float2 sum = make_float2(-__builtin_inff(), 0.f);
+  if (row < rows) {
+    for (int g = threadIdx.x / across; g < a.groups; g += 1024 / across)
+      sum = join(sum, a.stats[static_cast<int64_t>(g) * a.ld + row]);
+  }
+  area[threadIdx.x] = sum;
+  for (int d = 512; d >= across; d >>= 1) {
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < d) area[threadIdx.x] = sum = join(sum, area[threadIdx.x + d]);
+  }
+  if (static_cast<int>(threadIdx.x) < across && row < rows) {
+    const float log_sum = logf(sum.y);
+    a.lse[row] = sum.x + log_sum;
+    // In this order a loss close to zero keeps its digits: the target is then the maximum.
+    const float loss = a.label[row] >= 0 ? (sum.x - a.chosen[row]) + log_sum : __builtin_nanf("");
+    a.losses[a.by_row ? a.index[row] : row] = loss;
+  }
+}
+
+// The sum of the losses, or their mean, by one workgroup in FP64.
+__global__ __launch_bounds__(1024) void loss_kernel(const float* losses, const int* live, int mean, float* out) {
+  __shared__ double area[1024];
+  const int count = *live;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < count; i += 1024) sum += losses[i];
+  area[threadIdx.x] = sum;
+  for (int d = 512; d > 0; d >>= 1) {
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < d) area[threadIdx.x] = sum = sum + area[threadIdx.x + d];
+  }
+  if (threadIdx.x == 0) *out = static_cast<float>(mean ? sum / count : sum);
+}
+
+// Column sums of dz [rows, ld]: 64 V columns and every gridDim.y-th four rows a workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void bias_kernel(const void* dz, int64_t ld, int cols, int most, const int* live,
+                                                   int row0, float* partial) {
+  using S = typename T::storage;
+  constexpr int V = kVec<T>;
+  __shared__ float area[4][V][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (static_cast<int>(blockIdx.x) * 64 + lane) * V;
+  const int more = *live - row0, rows = more < most ? more : most;
+  float sums[V] = {};
+  for (int row = blockIdx.y * 4 + wave; row < rows; row += gridDim.y * 4) {
+    float f[V];
+    to_floats<T>(load_row<T>(static_cast<const S*>(dz) + row * ld, c, cols), f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[i] += f[i];
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) area[wave][i][lane] = sums[i];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (c + i < cols)
+      partial[static_cast<int64_t>(blockIdx.y) * cols + c + i] =
+          ((area[0][i][lane] + area[1][i][lane]) + area[2][i][lane]) + area[3][i][lane];
+}
+
+// db from `count` partial sums.
+template <typename T>
+__global__ __launch_bounds__(256) void join_bias_kernel(const float* partial, int count, int cols, const float* scale,
+                                                        void* out) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float sum = 0.f;
+  for (int i = 0; i < count; ++i) sum += partial[static_cast<int64_t>(i) * cols + c];
+  static_cast<typename T::storage*>(out)[c] = from_f32<T>(sum * *scale);
+}
+
+int element(int dtype) { return dtype == F32::code ? 4 : 2; }
+
+char* bytes_on(const void* p, int64_t bytes) {
+  return p != nullptr ? reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(p) + bytes) : nullptr;
+}
+
+dim3 blocks_of(int64_t items, int each) { return dim3(static_cast<uint32_t>((items + each - 1) / each)); }
+
+// The rows with a target and x's rows of them.
+struct Rows {
+  int *live, *index, *label;
+  Laid x;
+};
+
+hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, Workspace& ws, Rows& got, hipStream_t stream) {
+  const int64_t v = a.dtype == F32::code ? 4 : 8, ld = (a.cols + v - 1) / v * v;
+  r.targets = a.targets;
+  r.ignore = a.ignore;
+  r.rows = static_cast<int>(a.rows);
+  r.vocab = static_cast<int>(a.vocab);
+  r.live = got.live = ws.take<int>(1);
+  r.index = got.index = ws.take<int>(a.rows);
+  r.label = got.label = ws.take<int>(a.rows);
+  GatherArgs g{a.x, a.x_stride, got.live, got.index, ws.take<char>(a.rows * ld * element(a.dtype)), ld,
+               static_cast<int>(a.cols)};
+  got.x = {g.out, ld};
+  if (ws.dry()) return hipSuccess;
+  if (backward) rows_kernel<true><<<dim3(1), dim3(kRowThreads), 0, stream>>>(r);
+  else rows_kernel<false><<<dim3(1), dim3(kRowThreads), 0, stream>>>(r);
+  return with_type(a.dtype, [&](auto t) {
+    gather_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(g);
+    return hipGetLastError();
+  });
+}
+
+// A product of the loss; a sum over few results may go in slices.
+hipError_t multiply(ProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols, Finish finish,
+                    Workspace& ws, hipStream_t stream) {
+  p.a = a.data;
+  p.lda = a.ld;
+  p.b = b.data;
+  p.ldb = b.ld;
+  plan_product(p, dtype, a_cols, b_cols, finish);
+  if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
+  return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream, finish);
+}
+
+// z = x W^T + b of `count` rows and `outs` of the vocabulary.
+ProductArgs logits(const LossArgs& a, const Rows& rows, int64_t row0, int64_t count, int64_t col0, int64_t outs) {
+  ProductArgs p{};
+  p.m = static_cast<int>(count);
+  p.n = static_cast<int>(outs);
+  p.k = static_cast<int>(a.cols);
+  p.bias = bytes_on(a.bias, col0 * element(a.bias_dtype));
+  p.bias_f32 = a.bias_dtype == F32::code;
+  p.loss.live = rows.live;
+  p.loss.row0 = static_cast<int>(row0);
+  p.loss.label = rows.label + row0;
+  p.loss.col0 = static_cast<int>(col0);
+  return p;
+}
+
+Laid rows_from(const Laid& a, int64_t row, int dtype) { return {bytes_on(a.data, row * a.ld * element(dtype)), a.ld}; }
+
+constexpr int64_t kStats = int64_t{1} << 25;  // maxima and sums at a time: 256 MB
+constexpr int64_t kPiece = int64_t{1} << 30;  // bytes of dz at a time
+
+}  // namespace
+
+hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
+  Workspace ws(workspace);
+  const bool by_row = a.reduction == FH_REDUCE_NONE;
+  RowsArgs r{};
+  r.losses = by_row ? a.loss : nullptr;
+  Rows rows;
+  hipError_t err = gather(a, r, false, ws, rows, stream);
+  Laid w;
+  if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
+  const int64_t groups = (a.vocab + 63) / 64;
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(a.rows, most_product_rows(a.vocab)),
+                                         std::max<int64_t>(256, kStats / groups / 256 * 256));
+  auto* stats = ws.take<float2>(groups * most);
+  auto* chosen = ws.take<float>(most);
+  float* losses = by_row ? a.loss : ws.take<float>(a.rows);
+  int across = 64;  // rows of a workgroup that joins them
+  while (across > a.rows || (across > 4 && a.rows / across < compute_units())) across >>= 1;
+  if (err == hipSuccess) {
+    err = in_slices(a.rows, most, [&](int64_t row0, int64_t count) {
+      ProductArgs p = logits(a, rows, row0, count, 0, a.vocab);
+      p.loss.stats = stats;
+      p.loss.ld = most;
+      p.loss.chosen = chosen;
+      const hipError_t e = multiply(p, rows_from(rows.x, row0, a.dtype), w, a.dtype, false, false, Finish::kStats, ws, stream);
+      if (e != hipSuccess || ws.dry()) return e;
+      const LseArgs l{stats, most, static_cast<int>(groups), static_cast<int>(count), rows.live, static_cast<int>(row0),
+                      rows.label + row0, rows.index + row0, chosen, a.lse + row0, by_row ? losses : losses + row0, by_row};
+      lse_kernel<<<blocks_of(count, across), dim3(1024), 0, stream>>>(l, across);
+      return hipGetLastError();
+    });
+  }
+  if (err == hipSuccess && !by_row && !ws.dry()) {
+    loss_kernel<<<dim3(1), dim3(1024), 0, stream>>>(losses, rows.live, a.reduction == FH_REDUCE_MEAN, a.loss);
+    err = hipGetLastError();
+  }
+  if (bytes != nullptr) *bytes = ws.used();
+  return err;
+}
+
+hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
+  Workspace ws(workspace);
+  RowsArgs r{};
+  r.grad = a.grad;
+  r.per_row = a.reduction == FH_REDUCE_NONE;
+  r.mean = a.reduction == FH_REDUCE_MEAN;
+  r.scaled = a.dtype == F16::code;
+  r.lse = a.lse;
+  r.row = ws.take<float2>(a.rows);
+  r.scale = ws.take<float>(1);
+  Rows rows;
+  hipError_t err = gather(a, r, true, ws, rows, stream);
+  Laid w;
+  if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
+  if (err != hipSuccess) return err;
+  const int es = element(a.dtype);
+  // Pieces of the vocabulary, as even as whole tiles allow, of as many rows as 32-bit offsets into them do.
+  const int64_t most_rows = std::min<int64_t>(std::min<int64_t>(a.rows, 1 << 16), most_product_rows(a.cols));
+  int64_t piece = std::min<int64_t>(std::min<int64_t>(a.vocab, std::max<int64_t>(1024, kPiece / (most_rows * es))),
+                                    most_product_rows(std::max(a.cols, most_rows)));
+  const int64_t pieces = (a.vocab + piece - 1) / piece;
+  piece = std::min<int64_t>(a.vocab, ((a.vocab + pieces - 1) / pieces + 255) / 256 * 256);
+  const int64_t ld = (piece + 7) / 8 * 8, chunks = (a.rows + most_rows - 1) / most_rows;
+  const Laid dz{ws.take<char>(most_rows * ld * es), ld};
+  auto* dx_sums = a.dx != nullptr && piece < a.vocab ? ws.take<float>(a.rows * a.cols) : nullptr;
+  auto* dw_sums = a.dweight != nullptr && chunks > 1 ? ws.take<float>(piece * a.cols) : nullptr;
+  const int down = static_cast<int>(std::min<int64_t>((most_rows + 15) / 16, 64));  // partial sums of db for each chunk
+  auto* db_sums = a.dbias != nullptr ? ws.take<float>(chunks * down * piece) : nullptr;
+  if (a.dx != nullptr && !ws.dry()) {
+    err = with_type(a.dtype, [&](auto t) {
+      zero_rows_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(
+          a.targets, a.ignore, a.rows, static_cast<int>(a.cols), a.dx);
+      return hipGetLastError();
+    });
+  }
+  // Products follow one another on the stream, and share the space for what their slices add up to.
+  const int64_t before = ws.used();
+  int64_t most_used = before;
+  const auto shared = [&](auto call) {
+    Workspace part(bytes_on(workspace, before));
+    const hipError_t e = call(part);
+    most_used = std::max(most_used, before + part.used());
+    return e;
+  };
+  if (err == hipSuccess) {
+    err = in_slices(a.vocab, piece, [&](int64_t col0, int64_t outs) {
+      const Laid wp = rows_from(w, col0, a.dtype);
+      const hipError_t all = in_slices(a.rows, most_rows, [&](int64_t row0, int64_t count) {
+        const Laid xp = rows_from(rows.x, row0, a.dtype);
+        hipError_t e = shared([&](Workspace& part) {
+          ProductArgs p = logits(a, rows, row0, count, col0, outs);
+          p.loss.row = r.row + row0;
+          p.loss.ld = (outs + 7) / 8 * 8;
+          p.out = const_cast<void*>(dz.data);
+          return multiply(p, xp, wp, a.dtype, false, false, Finish::kSlope, part, stream);
+        });
+        const Laid d{dz.data, (outs + 7) / 8 * 8};
+        ProductArgs s{};
+        s.loss.live = rows.live;
+        s.loss.row0 = static_cast<int>(row0);
+        s.loss.scale = r.scale;
+        if (e == hipSuccess && a.dx != nullptr) {
+          e = shared([&](Workspace& part) {
+            ProductArgs p = s;
+            p.m = static_cast<int>(count);
+            p.n = static_cast<int>(a.cols);
+            p.k = static_cast<int>(outs);
+            p.loss.sums = dx_sums != nullptr ? dx_sums + row0 * a.cols : nullptr;
+            p.loss.first = col0 == 0;
+            p.loss.last = col0 + outs == a.vocab;
+            p.loss.index = rows.index + row0;
+            p.out = a.dx;
+            return multiply(p, d, wp, a.dtype, false, true, Finish::kSum, part, stream);
+          });
+        }
+        if (e == hipSuccess && a.dweight != nullptr) {
+          e = shared([&](Workspace& part) {
+            ProductArgs p = s;
+            p.m = static_cast<int>(outs);
+            p.n = static_cast<int>(a.cols);
+            p.k = static_cast<int>(count);
+            p.loss.sums = dw_sums;
+            p.loss.first = row0 == 0;
+            p.loss.last = row0 + count == a.rows;
+            p.out = bytes_on(a.dweight, col0 * a.cols * es);
+            return multiply(p, d, xp, a.dtype, true, true, Finish::kSum, part, stream);
+          });
+        }
+        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) {
+          e = with_type(a.dtype, [&](auto t) {
+            using T = decltype(t);
+            const dim3 grid(static_cast<uint32_t>((outs + 64 * kVec<T> - 1) / (64 * kVec<T>)), static_cast<uint32_t>(down));
+            bias_kernel<T><<<grid, dim3(256), 0, stream>>>(d.data, d.ld, static_cast<int>(outs), static_cast<int>(count),
+                                                           rows.live, static_cast<int>(row0),
+                                                           db_sums + row0 / most_rows * down * outs);
+            return hipGetLastError();
+          });
+        }
+        return e;
+      });
+      if (all != hipSuccess || a.dbias == nullptr || ws.dry()) return all;
+      return with_type(a.bias_dtype, [&](auto t) {
+        join_bias_kernel<decltype(t)><<<blocks_of(outs, 256), dim3(256), 0, stream>>>(
+            db_sums, static_cast<int>(chunks) * down, static_cast<int>(outs), r.scale,
+            bytes_on(a.dbias, col0 * element(a.bias_dtype)));
+        return hipGetLastError();
+      });
+    });
+  }
+  if (bytes != nullptr) *bytes = most_used;
+  return err;
+}
+
+}  // namespace fh

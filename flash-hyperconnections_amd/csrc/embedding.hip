@@ -1,0 +1,476 @@
+// Rows of a table, scaled and copied into the residual streams, and the table's gradient:
+//   y[i, s] = scale W[t_i],   dW[v] = scale (sum over i with t_i = v, in their order, over s of g[i, s]).
+//
+// Both move memory and nothing else.  The forward reads a row once for all streams.
+//
+// The gradient sorts the tokens (stably, by radix; a tile of up to 16384 in one workgroup's
+// LDS, several tiles through memory), so that a row's terms are neighbours.  The sorted
+// places go in chunks, a wavefront to a chunk and a strip of columns, which adds up the runs of
+// equal tokens.  A run that lies in one chunk is written at once; the parts of one that goes
+// over several, FP32, are joined by another kernel in their order.  Rows whose token does not
+// occur are zeros, written beside that.  Nothing depends on the order in which workgroups run.
+#include <algorithm>
+
+#include "fh_plan.h"
+#include "fh_kernels.h"
+#include "fh_vec.h"
+#include "workspace.h"
+
+namespace fh {
+namespace {
+
+// Four tokens a workgroup, a wavefront and Vectors vectors a lane to each; blockIdx.y strips of columns.
+constexpr int kVectors = 2;
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_kernel(EmbeddingArgs a) {
+  using S = typename T::storage;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (i >= a.count) return;
+  const int cols = static_cast<int>(a.cols);
+  const int c = (static_cast<int>(blockIdx.y) * kVectors * 64 + (threadIdx.x & 63)) * kVec<T>;
+  const int64_t token = a.tokens[i];
+  // A token out of range, which only a wait for the device could report, gives NaN.
+  const bool valid = token >= 0 && token < a.vocab;
+  const S* from = static_cast<const S*>(a.weight) + (valid ? token : 0) * a.w_stride;
+  U32x4 w[kVectors];
+#pragma unroll
+  for (int u = 0; u < kVectors; ++u) w[u] = load_row<T>(from, c + u * 64 * kVec<T>, cols);
+  if (a.scale != 1.f || !valid) {
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) {
+      float f[kVec<T>];
+      to_floats<T>(w[u], f);
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) f[k] = valid ? f[k] * a.scale : __builtin_nanf("");
+      w[u] = from_floats<T>(f);
+    }
+  }
+  S* to = static_cast<S*>(a.out) + i * a.streams * a.cols;
+  for (int s = 0; s < a.streams; ++s, to += a.cols) {
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) store_row<T>(w[u], to, c + u * 64 * kVec<T>, cols);
+  }
+}
+
+// ---- sorting -------------------------------------------------------------------------
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kMostTile = 16 * kThreads;
+
+// A token's key: itself, or the first number past the vocabulary where it has no gradient.
+__device__ __forceinline__ uint32_t key_of(const EmbeddingArgs& a, int64_t i) {
+  const int64_t t = a.tokens[i];
+  return static_cast<uint32_t>(t >= 0 && t < a.vocab && t != a.padding ? t : a.vocab);
+}
+
+// Exclusive sums of `Each` counts a thread, in the threads' order.
+template <int Each>
+__device__ __forceinline__ void scan(uint32_t (&v)[Each], uint32_t (&area)[kWaves]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t sum = 0;
+#pragma unroll
+  for (int e = 0; e < Each; ++e) {
+    const uint32_t mine = v[e];
+    v[e] = sum;
+    sum += mine;
+  }
+  uint32_t upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t other = __shfl_up(upto, d);
+    if (lane >= d) upto += other;
+  }
+  if (lane == 63) area[wave] = upto;
+  __syncthreads();
+  uint32_t base = upto - sum;
+  for (int w = 0; w < wave; ++w) base += area[w];
+#pragma unroll
+  for (int e = 0; e < Each; ++e) v[e] += base;
+}
+
+// A tile's places in the order of Bits bits of its keys, equal ones as they were.  Wavefront
+// w holds keys 64 P w .. 64 P (w + 1) - 1, 64 at a time.  Afterwards counts[digit][wave] is the
+// place of that wavefront's first key with that digit.
+template <int P, int Bits>
+__device__ __forceinline__ void rank(const uint32_t (&key)[P], int shift, uint32_t (&place)[P],
+                                     uint32_t (&counts)[kWaves << Bits], uint32_t (&area)[kWaves]) {
+  constexpr int each = (kWaves << Bits) / kThreads;
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int e = 0; e < each; ++e) counts[e * kThreads + threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const uint32_t digit = key[i] >> shift & ((1u << Bits) - 1);
+    uint64_t peers = ~uint64_t{0};
+#pragma unroll
+    for (int b = 0; b < Bits; ++b) {
+      const bool set = digit >> b & 1;
+      const uint64_t those = __ballot(set);
+      peers &= set ? those : ~those;
+    }
+    uint32_t* count = counts + digit * kWaves + wave;
+    const uint32_t before = *reinterpret_cast<volatile uint32_t*>(count);
+    const int below = lanes_below(peers);
+    place[i] = before + below;
+    if (below == 0) *reinterpret_cast<volatile uint32_t*>(count) = before + __popcll(peers);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  uint32_t v[each];
+#pragma unroll
+  for (int e = 0; e < each; ++e) v[e] = counts[threadIdx.x * each + e];
+  scan<each>(v, area);
+#pragma unroll
+  for (int e = 0; e < each; ++e) counts[threadIdx.x * each + e] = v[e];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < P; ++i) place[i] += counts[(key[i] >> shift & ((1u << Bits) - 1)) * kWaves + wave];
+}
+
+// Up to 1024 P tokens, in one workgroup.  Three passes for 2^18 words; 16384 tokens in 18 us.
+template <int P>
+__global__ __launch_bounds__(kThreads) void sort_tile_kernel(EmbeddingArgs a, int bits, uint32_t* keys, int* order) {
+  constexpr int kBits = 6;
+  __shared__ uint32_t counts[kWaves << kBits], area[kWaves], moved[P * kThreads];
+  __shared__ uint16_t from[P * kThreads];
+  const int first = (threadIdx.x >> 6) * 64 * P + (threadIdx.x & 63), count = static_cast<int>(a.count);
+  uint32_t key[P], at[P], place[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    at[i] = first + 64 * i;
+    key[i] = first + 64 * i < count ? key_of(a, first + 64 * i) : ~0u;  // past the last: they stay behind
+  }
+  for (int shift = 0; shift < bits; shift += kBits) {
+    rank<P, kBits>(key, shift, place, counts, area);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      moved[place[i]] = key[i];
+      from[place[i]] = static_cast<uint16_t>(at[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      key[i] = moved[first + 64 * i];
+      at[i] = from[first + 64 * i];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (first + 64 * i >= count) continue;
+    keys[first + 64 * i] = key[i];
+    order[first + 64 * i] = static_cast<int>(at[i]);
+  }
+}
+
+constexpr int kDigit = 9;  // bits of a pass over several tiles
+
+// keys null: the tokens themselves.
+__device__ __forceinline__ uint32_t key_at(const EmbeddingArgs& a, const uint32_t* keys, int64_t i) {
+  return keys != nullptr ? keys[i] : key_of(a, i);
+}
+
+// How often each digit occurs in each tile: table[tile][digit].
+__global__ __launch_bounds__(kThreads) void count_kernel(EmbeddingArgs a, const uint32_t* keys, int shift,
+                                                         uint32_t* table) {
+  __shared__ uint32_t counts[1 << kDigit];
+  for (int d = threadIdx.x; d < 1 << kDigit; d += kThreads) counts[d] = 0;
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kMostTile;
+  for (int i = threadIdx.x; i < kMostTile && first + i < a.count; i += kThreads)
+    atomicAdd(counts + (key_at(a, keys, first + i) >> shift & ((1u << kDigit) - 1)), 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < 1 << kDigit; d += kThreads) table[(static_cast<int64_t>(blockIdx.x) << kDigit) + d] = counts[d];
+}
+
+// Moves a tile's keys to their places in the whole.
+__global__ __launch_bounds__(kThreads) void move_kernel(EmbeddingArgs a, const uint32_t* keys, const int* order,
+                                                        int shift, const uint32_t* table, uint32_t* to_keys,
+                                                        int* to_order) {
+  constexpr int P = kMostTile / kThreads, kDigits = 1 << kDigit;
+  __shared__ uint32_t counts[kWaves << kDigit], area[kWaves], base[kDigits], other[kWaves];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kMostTile;
+  const int at = (threadIdx.x >> 6) * 64 * P + (threadIdx.x & 63);
+  // A digit's place: after the smaller digits of all tiles and this one of the tiles before.
+  uint32_t all[1] = {0}, before = 0;
+  if (threadIdx.x < kDigits) {
+    for (uint32_t tile = 0; tile < gridDim.x; ++tile) {
+      const uint32_t n = table[(static_cast<int64_t>(tile) << kDigit) + threadIdx.x];
+      before += tile < blockIdx.x ? n : 0;
+      all[0] += n;
+    }
+  }
+  scan<1>(all, other);
+  if (threadIdx.x < kDigits) base[threadIdx.x] = all[0] + before;
+  uint32_t key[P], place[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) key[i] = first + at + 64 * i < a.count ? key_at(a, keys, first + at + 64 * i) : ~0u;
+  rank<P, kDigit>(key, shift, place, counts, area);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int64_t from = first + at + 64 * i;
+    if (from >= a.count) continue;
+    const uint32_t digit = key[i] >> shift & (kDigits - 1);
+    const uint32_t to = base[digit] + place[i] - counts[digit * kWaves];
+    to_keys[to] = key[i];
+    to_order[to] = order != nullptr ? order[from] : static_cast<int>(from);
+  }
+}
+
+// ---- sums ----------------------------------------------------------------------------
+
+struct SumArgs {
+  EmbeddingArgs a;
+  const uint32_t* keys;  // [count], sorted
+  const int* order;      // [count]
+  float* partial;        // [chunks, 2, cols]: of the run that goes on from the chunk before, and that goes on after
+  int chunk, chunks, strips, summing;  // summing: workgroups that do not write zeros
+};
+
+template <typename T>
+__device__ __forceinline__ void put(const SumArgs& p, float (&f)[kVec<T>], uint32_t key, int c) {
+#pragma unroll
+  for (int k = 0; k < kVec<T>; ++k) f[k] *= p.a.scale;
+  store_row<T>(from_floats<T>(f), static_cast<typename T::storage*>(p.a.out) + key * p.a.cols, c,
+               static_cast<int>(p.a.cols));
+}
+
+template <int V>
+__device__ __forceinline__ void keep(const SumArgs& p, const float (&f)[V], int64_t chunk, int which, int c) {
+  float* to = p.partial + (chunk * 2 + which) * p.a.cols;
+  if (c + V <= p.a.cols) {
+    __builtin_memcpy(to + c, f, sizeof(f));
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (c + k < p.a.cols) to[c + k] = f[k];
+  }
+}
+
+// A row of the table whose token does not occur: 64 rows a workgroup.
+template <typename T>
+__device__ __forceinline__ void write_zeros(const SumArgs& p, int64_t first) {
+  const int lane = threadIdx.x & 63, cols = static_cast<int>(p.a.cols);
+  const int64_t row = first + lane;
+  int64_t low = 0, high = p.a.count;
+  while (low < high) {
+    const int64_t mid = (low + high) / 2;
+    if (p.keys[mid] < static_cast<uint32_t>(row)) low = mid + 1;
+    else high = mid;
+  }
+  const bool here = row >= p.a.vocab || (low < p.a.count && p.keys[low] == static_cast<uint32_t>(row));
+  for (uint64_t left = ~__ballot(here) >> (threadIdx.x >> 6) & 0x1111111111111111ull; left != 0; left &= left - 1) {
+    auto* to = static_cast<typename T::storage*>(p.a.out) +
+               (first + (threadIdx.x >> 6) + __ffsll(static_cast<unsigned long long>(left)) - 1) * p.a.cols;
+    for (int c = lane * kVec<T>; c < cols; c += 64 * kVec<T>) store_row<T>(U32x4{0, 0, 0, 0}, to, c, cols);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void sum_kernel(SumArgs p) {
+  using S = typename T::storage;
+  constexpr int V = kVec<T>, kAhead = 8;
+  if (static_cast<int>(blockIdx.x) >= p.summing) {
+    write_zeros<T>(p, (static_cast<int64_t>(blockIdx.x) - p.summing) * 64);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6));
+  const int64_t chunk = unit / p.strips;
+  if (chunk >= p.chunks) return;
+  const int c = (unit % p.strips * 64 + lane) * V, cols = static_cast<int>(p.a.cols);
+  const int64_t first = chunk * p.chunk;
+  const int count = static_cast<int>(p.a.count - first < p.chunk ? p.a.count - first : p.chunk);
+  const uint32_t none = static_cast<uint32_t>(p.a.vocab);
+  // The chunk's keys and rows, one a lane.
+  const uint32_t my_key = lane < count ? p.keys[first + lane] : none;
+  const int my_row = lane < count ? p.order[first + lane] : 0;
+  const uint32_t before = first > 0 ? p.keys[first - 1] : none, after = first + count < p.a.count ? p.keys[first + count] : none;
+  const int valid = __popcll(__ballot(my_key != none));  // those without a gradient come last
+  if (valid == 0) return;
+  uint32_t key = __builtin_amdgcn_readlane(my_key, 0);
+  bool goes_on = key == before;
+  float sum[V] = {};
+  const int streams = p.a.streams, items = valid * streams;
+  int place = 0, stream = 0;  // of the next load
+  int at = 0, step = 0;       // of the next addition
+  for (int i = 0; i < items; i += kAhead) {
+    U32x4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u >= items) break;
+      const int64_t row = static_cast<int64_t>(__builtin_amdgcn_readlane(my_row, place)) * streams + stream;
+      raw[u] = load_row<T>(static_cast<const S*>(p.a.grad) + row * p.a.g_stride, c, cols);
+      if (++stream == streams) {
+        stream = 0;
+        ++place;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u >= items) break;
+      if (step == 0) {
+        const uint32_t next = __builtin_amdgcn_readlane(my_key, at);
+        if (next != key) {
+          if (goes_on) keep(p, sum, chunk, 0, c);
+          else put<T>(p, sum, key, c);
+          goes_on = false;
+          key = next;
+#pragma unroll
+          for (int k = 0; k < V; ++k) sum[k] = 0.f;
+        }
+      }
+      float f[V];
+      to_floats<T>(raw[u], f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] += f[k];
+      if (++step == streams) {
+        step = 0;
+        ++at;
+      }
+    }
+  }
+  if (goes_on) keep(p, sum, chunk, 0, c);
+  else if (valid == count && after == key) keep(p, sum, chunk, 1, c);
+  else put<T>(p, sum, key, c);
+}
+
+// Runs over several chunks, by the chunk in which they begin: its part and those of the chunks after it, in
+// order, a quarter of them a wavefront.
+template <typename T>
+__global__ __launch_bounds__(256) void join_runs_kernel(SumArgs p) {
+  constexpr int V = kVec<T>;
+  __shared__ float area[4][V][64];
+  const int64_t chunk = blockIdx.x / p.strips, first = chunk * p.chunk, end = first + p.chunk;
+  if (end >= p.a.count) return;
+  const uint32_t key = p.keys[end - 1];
+  if (key >= static_cast<uint32_t>(p.a.vocab) || p.keys[end] != key || (first > 0 && p.keys[first - 1] == key)) return;
+  // The first place past the run.
+  int64_t low = end, high = p.a.count;
+  while (low < high) {
+    const int64_t mid = (low + high) / 2;
+    if (p.keys[mid] <= key) low = mid + 1;
+    else high = mid;
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = (static_cast<int>(blockIdx.x) % p.strips * 64 + lane) * V, cols = static_cast<int>(p.a.cols);
+  const int64_t parts = (low - 1) / p.chunk - chunk + 1, from = parts * wave / 4, to = parts * (wave + 1) / 4;
+  float sum[V] = {};
+  const auto load = [&](int64_t part, float (&f)[V]) {
+    const float* row = p.partial + ((chunk + part) * 2 + (part == 0 ? 1 : 0)) * p.a.cols;
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = 0.f;
+    if (c + V <= cols) {
+      __builtin_memcpy(f, row + c, sizeof(f));
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (c + k < cols) f[k] = row[c + k];
+    }
+  };
+  int64_t i = from;
+  for (; i + 4 <= to; i += 4) {
+    float f[4][V];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load(i + u, f[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] += f[u][k];
+  }
+  for (; i < to; ++i) {
+    float f[V];
+    load(i, f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] += f[k];
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) area[wave][k][lane] = sum[k];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int k = 0; k < V; ++k) sum[k] = ((area[0][k][lane] + area[1][k][lane]) + area[2][k][lane]) + area[3][k][lane];
+  put<T>(p, sum, key, c);
+}
+
+dim3 blocks_of(int64_t items, int64_t each) { return dim3(static_cast<uint32_t>((items + each - 1) / each)); }
+
+// The keys in `keys` and `order` afterwards, through another pair.
+hipError_t sort_tokens(const EmbeddingArgs& a, Workspace& ws, uint32_t*& keys, int*& order, hipStream_t stream) {
+  keys = ws.take<uint32_t>(a.count);
+  order = ws.take<int>(a.count);
+  int bits = 1;
+  while (a.vocab >> bits != 0) ++bits;  // of the vocabulary's size, the last key
+  if (a.count <= kMostTile) {
+    if (ws.dry()) return hipSuccess;
+    if (a.count <= kThreads) sort_tile_kernel<1><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
+    else if (a.count <= 4 * kThreads) sort_tile_kernel<4><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
+    else sort_tile_kernel<16><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
+    return hipGetLastError();
+  }
+  auto* other_keys = ws.take<uint32_t>(a.count);
+  auto* other_order = ws.take<int>(a.count);
+  const dim3 tiles = blocks_of(a.count, kMostTile);
+  auto* table = ws.take<uint32_t>(static_cast<int64_t>(tiles.x) << kDigit);
+  if (ws.dry()) return hipSuccess;
+  for (int shift = 0; shift < bits; shift += kDigit) {
+    const uint32_t* from = shift > 0 ? keys : nullptr;
+    count_kernel<<<tiles, dim3(kThreads), 0, stream>>>(a, from, shift, table);
+    move_kernel<<<tiles, dim3(kThreads), 0, stream>>>(a, from, shift > 0 ? order : nullptr, shift, table, other_keys,
+                                                      other_order);
+    std::swap(keys, other_keys);
+    std::swap(order, other_order);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream) {
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const int64_t across = kVectors * 64 * kVec<T>;
+    return in_slices(a.count, most_groups(256) * 4, [&](int64_t first, int64_t count) {
+      EmbeddingArgs part = a;
+      part.count = count;
+      part.tokens = a.tokens + first;
+      part.out = static_cast<typename T::storage*>(a.out) + first * a.streams * a.cols;
+      const dim3 grid(static_cast<uint32_t>((count + 3) / 4), static_cast<uint32_t>((a.cols + across - 1) / across));
+      embedding_kernel<T><<<grid, dim3(256), 0, stream>>>(part);
+      return hipGetLastError();
+    });
+  });
+}
+
+hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* workspace, int64_t* bytes,
+                                     hipStream_t stream) {
+  Workspace ws(workspace);
+  SumArgs p{};
+  p.a = a;
+  uint32_t* keys = nullptr;
+  int* order = nullptr;
+  hipError_t err = a.count > 0 ? sort_tokens(a, ws, keys, order, stream) : hipSuccess;
+  if (err != hipSuccess) return err;
+  p.keys = keys;
+  p.order = order;
+  const int64_t strip = 64 * (dtype == F32::code ? 4 : 8);
+  p.strips = static_cast<int>((a.cols + strip - 1) / strip);
+  // Chunks for about eight wavefronts a compute unit, of 16 to 64 places.
+  p.chunk = 64;
+  while (p.chunk > 16 && a.count / p.chunk * p.strips < 8 * compute_units()) p.chunk /= 2;
+  p.chunks = static_cast<int>((a.count + p.chunk - 1) / p.chunk);
+  p.partial = ws.take<float>(static_cast<int64_t>(p.chunks) * 2 * a.cols);
+  if (bytes != nullptr) *bytes = ws.used();
+  if (ws.dry()) return hipSuccess;
+  const int64_t units = static_cast<int64_t>(p.chunks) * p.strips;
+  p.summing = static_cast<int>((units + 3) / 4);
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    sum_kernel<T><<<dim3(static_cast<uint32_t>(p.summing + (a.vocab + 63) / 64)), dim3(256), 0, stream>>>(p);
+    if (p.chunks > 1) join_runs_kernel<T><<<dim3(static_cast<uint32_t>(units)), dim3(256), 0, stream>>>(p);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace fh

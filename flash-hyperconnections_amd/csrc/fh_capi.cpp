@@ -245,6 +245,56 @@ int validate_linear(const fh::LinearArgs& a) {
   return FH_OK;
 }
 
+int validate_embedding(const int64_t* tokens, const void* rows, int64_t stride, int streams, int dtype, int64_t count,
+                       int64_t vocab, int64_t cols) {
+  constexpr int64_t most = int64_t{1} << 28;
+  if (!known_dtype(dtype) || count < 0 || count >= most || vocab < 1 || vocab >= most || cols < 1 ||
+      cols >= int64_t{1} << 24 || streams < 1 || streams >= 1 << 16)
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "embedding: expected weight [vocab, cols] in float32, float16, or bfloat16 with 1 <= vocab < 2^28 and "
+                "1 <= cols < 2^24, fewer than 2^28 tokens and 1 <= streams < 2^16");
+  if (count > 0 && (tokens == nullptr || !aligned(tokens, 8) || !rows_ok(rows, stride, dtype)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "embedding: null or misaligned pointer, or negative stride");
+  return FH_OK;
+}
+
+int validate_loss(const fh::LossArgs& a) {
+  constexpr int64_t most = int64_t{1} << 22;
+  if (!known_dtype(a.dtype) || (a.bias_dtype != a.dtype && a.bias_dtype != FH_DTYPE_F32) || a.rows < 0 ||
+      a.rows >= (int64_t{1} << 24) || a.cols < 1 || a.cols >= most || a.vocab < 1 || a.vocab >= most)
+    return fail(FH_ERR_INVALID_ARGUMENT,
+                "linear_cross_entropy: expected x [rows, cols] and weight [vocab, cols] in float32, float16, or bfloat16 "
+                "with fewer than 2^24 rows and 1 <= cols, vocab < 2^22, and a bias of their type or float32");
+  if (a.reduction < FH_REDUCE_NONE || a.reduction > FH_REDUCE_MEAN)
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: unknown reduction");
+  if (a.rows > 0 && (!rows_ok(a.x, a.x_stride, a.dtype) || !rows_ok(a.weight, a.w_stride, a.dtype) ||
+                     a.targets == nullptr || !aligned(a.targets, 8) || a.lse == nullptr || !aligned(a.lse, 4) ||
+                     (a.bias != nullptr && !aligned(a.bias, element_size(a.bias_dtype)))))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
+  return FH_OK;
+}
+
+fh::LossArgs loss_args(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
+                       int bias_dtype, const int64_t* targets, int64_t ignore, int reduction, const float* lse,
+                       int dtype, int64_t rows, int64_t cols, int64_t vocab) {
+  fh::LossArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.weight = weight;
+  a.w_stride = weight_stride;
+  a.bias = bias;
+  a.bias_dtype = bias_dtype;
+  a.targets = targets;
+  a.ignore = ignore;
+  a.reduction = reduction;
+  a.lse = const_cast<float*>(lse);
+  a.dtype = dtype;
+  a.rows = rows;
+  a.cols = cols;
+  a.vocab = vocab;
+  return a;
+}
+
 int validate_clip(const char* op, int count, const void* const* grads, void* const* out, const int64_t* sizes,
                   const int* dtypes, double norm_type, const float* norm, int* power) {
   if (norm_type != 1.0 && norm_type != 2.0 && !(std::isinf(norm_type) && norm_type > 0))
@@ -553,6 +603,97 @@ int fh_clip_gradients(int count, const void* const* grads, void* const* out, con
   rc = check_workspace("clip_gradients", workspace, workspace_bytes, fh::clip_partials(list) * 8, &query);
   if (rc != FH_OK || query) return rc;
   return launched(fh::launch_clip(list, power, max_norm, true, norm, static_cast<double*>(workspace), stream));
+}
+
+int fh_embedding(const int64_t* tokens, const void* weight, int64_t weight_stride, double scale, int streams, void* y,
+                 int dtype, int64_t count, int64_t vocab, int64_t cols, hipStream_t stream) {
+  const int rc = validate_embedding(tokens, weight, weight_stride, streams, dtype, count, vocab, cols);
+  if (rc != FH_OK) return rc;
+  if (count == 0) return launched(hipSuccess);
+  if (!rows_ok(y, 0, dtype)) return fail(FH_ERR_INVALID_ARGUMENT, "embedding: null or misaligned pointer, or negative stride");
+  fh::EmbeddingArgs a{};
+  a.tokens = tokens;
+  a.weight = weight;
+  a.w_stride = weight_stride;
+  a.scale = static_cast<float>(scale);
+  a.out = y;
+  a.count = count;
+  a.vocab = vocab;
+  a.cols = cols;
+  a.streams = streams;
+  return launched(fh::launch_embedding(a, dtype, stream));
+}
+
+int fh_embedding_backward(const int64_t* tokens, const void* grad, int64_t grad_stride, double scale, int streams,
+                          int64_t padding, void* dweight, void* workspace, int64_t* workspace_bytes, int dtype,
+                          int64_t count, int64_t vocab, int64_t cols, hipStream_t stream) {
+  int rc = validate_embedding(tokens, grad, grad_stride, streams, dtype, count, vocab, cols);
+  if (rc != FH_OK) return rc;
+  if (!rows_ok(dweight, 0, dtype))
+    return fail(FH_ERR_INVALID_ARGUMENT, "embedding: null or misaligned pointer, or negative stride");
+  fh::EmbeddingArgs a{};
+  a.tokens = tokens;
+  a.grad = grad;
+  a.g_stride = grad_stride;
+  a.scale = static_cast<float>(scale);
+  a.padding = padding;
+  a.out = dweight;
+  a.count = count;
+  a.vocab = vocab;
+  a.cols = cols;
+  a.streams = streams;
+  int64_t need = 0;
+  bool query = false;
+  (void)fh::launch_embedding_backward(a, dtype, nullptr, &need, stream);
+  rc = check_workspace("embedding", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_embedding_backward(a, dtype, workspace, nullptr, stream));
+}
+
+int fh_linear_cross_entropy(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                            const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore, int reduction,
+                            float* loss, float* lse, void* workspace, int64_t* workspace_bytes, int dtype,
+                            int64_t rows, int64_t cols, int64_t vocab, hipStream_t stream) {
+  fh::LossArgs a = loss_args(x, x_stride, weight, weight_stride, bias, bias_dtype, targets, ignore, reduction, lse,
+                             dtype, rows, cols, vocab);
+  a.loss = loss;
+  int rc = validate_loss(a);
+  if (rc != FH_OK) return rc;
+  if (rows == 0) return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: no rows, whose loss is the caller's");
+  if (loss == nullptr || !aligned(loss, 4))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
+  int64_t need = 0;
+  bool query = false;
+  (void)fh::launch_cross_entropy(a, nullptr, &need, stream);
+  rc = check_workspace("linear_cross_entropy", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_cross_entropy(a, workspace, nullptr, stream));
+}
+
+int fh_linear_cross_entropy_backward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                     const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore,
+                                     int reduction, const float* lse, const float* grad, void* dx, void* dweight,
+                                     void* dbias, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                                     int64_t cols, int64_t vocab, hipStream_t stream) {
+  fh::LossArgs a = loss_args(x, x_stride, weight, weight_stride, bias, bias_dtype, targets, ignore, reduction, lse,
+                             dtype, rows, cols, vocab);
+  a.grad = grad;
+  a.dx = dx;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  int rc = validate_loss(a);
+  if (rc != FH_OK) return rc;
+  if (rows == 0)
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: no rows, whose gradients are zeros of the caller's");
+  if (grad == nullptr || !aligned(grad, 4) || (dx != nullptr && !rows_ok(dx, 0, dtype)) ||
+      (dweight != nullptr && !rows_ok(dweight, 0, dtype)) || (dbias != nullptr && !rows_ok(dbias, 0, bias_dtype)))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
+  int64_t need = 0;
+  bool query = false;
+  (void)fh::launch_cross_entropy_backward(a, nullptr, &need, stream);
+  rc = check_workspace("linear_cross_entropy", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_cross_entropy_backward(a, workspace, nullptr, stream));
 }
 
 const char* fh_last_error(void) { return g_error.c_str(); }

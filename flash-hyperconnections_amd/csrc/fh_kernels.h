@@ -102,4 +102,41 @@ struct LinearArgs {
 hipError_t launch_linear(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
 hipError_t launch_linear_backward(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
 
+// ---- the two ends of a network: embedding, and the linear layer with its cross entropy -------
+
+struct EmbeddingArgs {
+  const int64_t* tokens;  // [count]
+  const void* weight;     // [vocab, cols], rows w_stride elements apart
+  const void* grad;       // backward: [count * streams, cols], rows g_stride elements apart
+  int64_t w_stride, g_stride;
+  float scale;
+  int64_t padding;        // backward: a token without a gradient, or -1
+  void* out;              // [count, streams, cols], or the gradient [vocab, cols]
+  int64_t count, vocab, cols;
+  int streams;
+};
+hipError_t launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream);
+// Also gives the bytes of workspace it needs, with `workspace` null: nothing is launched then.
+hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* workspace, int64_t* bytes,
+                                     hipStream_t stream);
+
+struct LossArgs {
+  const void* x;          // [rows, cols], rows x_stride elements apart
+  const void* weight;     // [vocab, cols]
+  const void* bias;       // [vocab] or null
+  int64_t x_stride, w_stride;
+  int bias_dtype, dtype;
+  const int64_t* targets; // [rows]
+  int64_t ignore;
+  int reduction;
+  float* loss;            // forward: one, or [rows]
+  float* lse;             // [rows], for the backward
+  const float* grad;      // backward: one, or [rows]
+  void *dx, *dweight, *dbias;  // contiguous; each may be null
+  int64_t rows, cols, vocab;
+};
+// As launch_linear and launch_linear_backward.
+hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
+hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
+
 }  // namespace fh

@@ -7,10 +7,33 @@
 #include "fh_kernels.h"
 #include "fh_vec.h"
 #include "flash_hypercons.h"
+#include "workspace.h"
 
 namespace fh {
 
 typedef float Floats4 __attribute__((ext_vector_type(4)));
+
+// What becomes of a product's results: the linear layer's epilogue; the softmax
+// statistics of logits, which are not kept; the logits' gradients; or a sum that goes on
+// from another product's and is scaled at its end.
+enum class Finish { kLinear, kStats, kSlope, kSum };
+
+// What the last three need beside the product.  Their rows are the first *live ones from
+// row0 on (of the sum where A is in columns), as many as there are targets.
+struct LossParts {
+  const int* live;
+  int row0;
+  const int* label;      // [rows] targets, negative where out of range
+  int col0;              // the vocabulary's entry of column 0
+  float2* stats;         // kStats: [columns / 64, rows] maximum and sum of exponentials, groups ld apart
+  float* chosen;         // kStats: [rows] logits of the targets
+  const float2* row;     // kSlope: [rows] the logarithm of the row's sum, and the factor of its gradient
+  int64_t ld;            // kStats: groups; kSlope: rows of out, whole vectors, zero past n
+  float* sums;           // kSum: [m, n] of the sum so far
+  int first, last;       // kSum: whether sums is not read, or not written but scaled into out
+  const float* scale;    // kSum
+  const int* index;      // kSum: [rows] rows of out, or null
+};
 
 // D[m][n] = sum over k of A[m][k] B[n][k] and what follows it.  An operand is in
 // rows (k contiguous, rows ld elements apart) or in columns (m or n contiguous, a
@@ -31,7 +54,30 @@ struct ProductArgs {
   int act;
   void* saved;           // receives the sum with its bias, or null
   void* out;             // [m, n] contiguous
+  LossParts loss;
 };
+
+// Fits a product's rows, or its sum where A is in columns, to what is live.
+template <Finish F, bool ACols>
+__device__ __forceinline__ void fit_live(ProductArgs& p) {
+  if constexpr (F != Finish::kLinear) {
+    const int more = *p.loss.live - p.loss.row0, live = more > 0 ? more : 0;
+    int& rows = ACols ? p.k : p.m;
+    rows = live < rows ? live : rows;
+  }
+}
+// The same and its tiles; false for a workgroup past them.
+template <Finish F, bool ACols>
+__device__ __forceinline__ bool fit(ProductArgs& p) {
+  if constexpr (F != Finish::kLinear) {
+    fit_live<F, ACols>(p);
+    if constexpr (!ACols) {
+      p.tiles_m = (p.m + p.side_m - 1) / p.side_m;
+      return blockIdx.x < static_cast<uint32_t>(p.tiles_m * p.tiles_n);
+    }
+  }
+  return true;
+}
 
 // What the backward needs of the sum z = x W^T + b: FP32 for FP32 results, and
 // FP16 for 16-bit ones, whatever they are.  Every activation's slope is 0 or 1 to
@@ -188,12 +234,136 @@ __device__ __forceinline__ void round_some(const float (&f)[V], typename T::stor
   }
 }
 
-// V neighbouring results (row i, columns j .. j + V - 1) on their way out: bias,
-// activation, residual; or into the slice's partial sums.
 template <typename T, int V>
+__device__ __forceinline__ void add_bias(const ProductArgs& p, int j, int left, float (&v)[V]) {
+  using S = typename T::storage;
+  if (p.bias == nullptr) return;
+  float b[V];
+  if (p.bias_f32) {
+    load_some(static_cast<const float*>(p.bias) + j, left, b);
+  } else {
+    S e[V];
+    load_some(static_cast<const S*>(p.bias) + j, left, e);
+#pragma unroll
+    for (int k = 0; k < V; ++k) b[k] = to_f32<T>(e[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] += b[k];
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp(v): the hardware's exp2 where the argument is small in size or the result is rounded
+// to 16 bits; its argument's rounding is worth |v| 2^-24 of the result.
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
+
+// A value of the lane that the quad's permutation or the mirror of 8 or 16 lanes gives.
+template <int Control>
+__device__ __forceinline__ float from_lane(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), Control, 0xF, 0xF, true));
+}
+// f over the values of Lanes neighbouring lanes, the same bits in each.
+template <int Lanes, typename F>
+__device__ __forceinline__ float over_lanes(float v, F f) {
+  v = f(v, from_lane<0xB1>(v));
+  v = f(v, from_lane<0x4E>(v));
+  if constexpr (Lanes >= 8) v = f(v, from_lane<0x141>(v));
+  if constexpr (Lanes >= 16) v = f(v, from_lane<0x140>(v));
+  return v;
+}
+
+// Logits of Lanes V neighbouring columns of row i, V a lane: their maximum m and the sum
+// of exp(z - m), as far as columns are valid, and the target's logit.  -inf alone gives
+// m = -inf and a sum of zero; a NaN or +inf makes the sum NaN.
+template <typename T, int Lanes, int V>
+__device__ __forceinline__ void stats_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+  if (i >= p.m) return;  // the same in all of these lanes
+  const int left = p.n - j;
+  if (left > 0) add_bias<T>(p, j, left, v);
+  const float none = -__builtin_inff();
+  float m = none;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    if (k >= left) v[k] = none;
+    m = __builtin_fmaxf(m, v[k]);
+  }
+  m = over_lanes<Lanes>(m, [](float a, float b) { return __builtin_fmaxf(a, b); });
+  const int at = p.loss.label[i] - p.loss.col0 - j;
+  const float from = m == none ? 0.f : m;
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    if (k == at && k < left) p.loss.chosen[i] = v[k];
+    s += exp_of(v[k] - from);
+  }
+  s = over_lanes<Lanes>(s, [](float a, float b) { return a + b; });
+  if (j % 64 == 0 && left > 0) p.loss.stats[static_cast<int64_t>(j / 64) * p.loss.ld + i] = make_float2(m, s);
+}
+
+// Logits on their way to the gradients of z: (exp(z - lse) - [target]) times the row's
+// factor, rounded to the storage type, which the products that follow take.  (Root mean
+// square 0.0017 of a term in bf16, beside as much for their results' own rounding.)  A
+// factor of zero gives zeros whatever z is.
+template <typename T, int V>
+__device__ __forceinline__ void slope_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+  using S = typename T::storage;
+  if (i >= p.m || j >= p.loss.ld) return;
+  const int left = p.n - j;
+  const float2 row = p.loss.row[i];
+  const int at = p.loss.label[i] - p.loss.col0 - j;
+  if (left > 0) add_bias<T>(p, j, left, v);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    float e;
+    if constexpr (T::code == F32::code) e = expf(v[k] - row.x);
+    else e = exp_of(v[k] - row.x);
+    if (k == at) e -= 1.f;
+    v[k] = k < left && row.y != 0.f ? e * row.y : 0.f;
+  }
+  S e[V];
+  round_some<T>(v, e);
+  __builtin_memcpy(static_cast<S*>(p.out) + static_cast<int64_t>(i) * p.loss.ld + j, e, sizeof(e));
+}
+
+// V results of a sum on their way into the sum so far, or at its end scaled and out.
+template <typename T, int V>
+__device__ __forceinline__ void sum_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+  using S = typename T::storage;
+  const int64_t at = static_cast<int64_t>(i) * p.n + j;
+  const int left = p.n - j;
+  if (!p.loss.first) {
+    float before[V];
+    load_some(p.loss.sums + at, left, before);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] += before[k];
+  }
+  if (!p.loss.last) {
+    store_some<true>(v, p.loss.sums + at, left);
+    return;
+  }
+  const float scale = *p.loss.scale;
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] *= scale;
+  S e[V];
+  round_some<T>(v, e);
+  const int64_t row = p.loss.index != nullptr ? p.loss.index[i] : i;
+  store_some(e, static_cast<S*>(p.out) + row * p.n + j, left);
+}
+
+// V neighbouring results (row i, columns j .. j + V - 1) on their way out: bias,
+// activation, residual; or into the slice's partial sums.  Lanes neighbouring lanes have
+// the results beside these.
+template <typename T, Finish F, int Lanes, int V>
 __device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int i, int j, float (&v)[V]) {
   using S = typename T::storage;
   using Z = Saved<T>;
+  if constexpr (F == Finish::kStats) {
+    stats_some<T, Lanes>(p, i, j, v);
+    return;
+  } else if constexpr (F == Finish::kSlope) {
+    slope_some<T>(p, i, j, v);
+    return;
+  }
   if (i >= p.m || j >= p.n) return;
   const int64_t at = static_cast<int64_t>(i) * p.n + j;
   const int left = p.n - j;
@@ -201,19 +371,11 @@ __device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int
     store_some<true>(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
     return;
   }
-  if (p.bias != nullptr) {
-    float b[V];
-    if (p.bias_f32) {
-      load_some(static_cast<const float*>(p.bias) + j, left, b);
-    } else {
-      S e[V];
-      load_some(static_cast<const S*>(p.bias) + j, left, e);
-#pragma unroll
-      for (int k = 0; k < V; ++k) b[k] = to_f32<T>(e[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] += b[k];
+  if constexpr (F == Finish::kSum) {
+    sum_some<T>(p, i, j, v);
+    return;
   }
+  add_bias<T>(p, j, left, v);
   if (p.saved != nullptr) {
     float z[V];
     typename Z::storage e[V];
@@ -242,7 +404,7 @@ __device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int
 __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
   *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;
 }
-template <typename T, int Rows>
+template <typename T, Finish F, int Rows>
 __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
                                               int lane) {
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
@@ -252,7 +414,7 @@ __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, c
       const int r = 4 * it + (lane >> 4), c = lane & 15;
       float v[4];
       __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
-      finish_some<T>(p, slice, row + r, col + 4 * c, v);
+      finish_some<T, F, 16>(p, slice, row + r, col + 4 * c, v);
     }
   } else {
 #pragma unroll 2
@@ -261,7 +423,7 @@ __device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, c
       float v[8];
       __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
       __builtin_memcpy(v + 4, area + r * 256 + (((c + 1) ^ (r & 15)) << 4), 16);
-      finish_some<T>(p, slice, row + r, col + 8 * (lane & 7), v);
+      finish_some<T, F, 8>(p, slice, row + r, col + 8 * (lane & 7), v);
     }
   }
   asm volatile("" ::: "memory");
@@ -330,15 +492,50 @@ __device__ __forceinline__ void wait_loads() {
 constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16-bit tile within 2^31 bytes
 
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
-// floats.  `dtype` is the operands' and the output's.
-void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
+// floats.  `dtype` is the operands' and the output's; Finish::kStats and kSlope need whole
+// sums, in one slice.
+void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
 // vectors; false for others.
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
-hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
-hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream);
-hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices);
+hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
+                          Finish finish = Finish::kLinear);
+hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream);
+hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
+                                 hipStream_t stream);
 // 16-bit types.
-hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream);
+hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
+                               hipStream_t stream);
+
+// Calls f with the operands' layouts and the finish as types, where there is such a product:
+// of rows by rows (logits and their gradients too), rows by columns, columns by columns.
+template <bool B>
+using Flag = std::integral_constant<bool, B>;
+template <Finish F>
+using FinishType = std::integral_constant<Finish, F>;
+template <typename Call>
+hipError_t with_layout(bool a_cols, bool b_cols, Finish finish, Call call) {
+  if (!a_cols && !b_cols) {
+    if (finish == Finish::kLinear) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kLinear>{});
+    if (finish == Finish::kStats) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kStats>{});
+    if (finish == Finish::kSlope) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kSlope>{});
+  } else if (b_cols) {
+    if (finish == Finish::kLinear && !a_cols) return call(Flag<false>{}, Flag<true>{}, FinishType<Finish::kLinear>{});
+    if (finish == Finish::kLinear) return call(Flag<true>{}, Flag<true>{}, FinishType<Finish::kLinear>{});
+    if (finish == Finish::kSum && !a_cols) return call(Flag<false>{}, Flag<true>{}, FinishType<Finish::kSum>{});
+    if (finish == Finish::kSum) return call(Flag<true>{}, Flag<true>{}, FinishType<Finish::kSum>{});
+  }
+  return hipErrorInvalidValue;  // no such product
+}
+
+// An operand as the products read it.
+struct Laid {
+  const void* data;
+  int64_t ld;
+};
+
+// `data` [rows, cols] as it is where the products read it so, or laid out anew in the workspace.
+hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws, Laid& got,
+                   hipStream_t stream);
 
 }  // namespace fh

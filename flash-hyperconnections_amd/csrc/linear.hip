@@ -111,52 +111,10 @@ hipError_t launch_prepare(const PrepareArgs& a, int dtype, int blocks, hipStream
   });
 }
 
-// Takes pieces of a workspace; without one it only adds up their sizes.
-class Workspace {
- public:
-  explicit Workspace(void* base) : base_(static_cast<char*>(base)) {}
-  template <typename E>
-  E* take(int64_t count) {
-    const int64_t at = used_;
-    used_ += (count * static_cast<int64_t>(sizeof(E)) + 255) / 256 * 256;
-    return base_ != nullptr ? reinterpret_cast<E*>(base_ + at) : nullptr;
-  }
-  bool dry() const { return base_ == nullptr; }
-  int64_t used() const { return used_; }
-
- private:
-  char* base_;
-  int64_t used_ = 0;
-};
-
-// An operand as the products read it.
-struct Laid {
-  const void* data;
-  int64_t ld;
-};
-
 // Whether the products read [rows, cols] as it is.
 bool as_it_is(const void* data, int64_t stride, int64_t cols, int dtype) {
   if (dtype == F32::code) return true;
   return reinterpret_cast<uintptr_t>(data) % 16 == 0 && cols % 8 == 0 && stride % 8 == 0 && stride < kMostStride;
-}
-
-// `data` as it is, or laid out anew in the workspace.
-hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws, Laid& got,
-                   hipStream_t stream) {
-  if (as_it_is(data, stride, cols, dtype)) {
-    got = {data, stride};
-    return hipSuccess;
-  }
-  PrepareArgs p{};
-  p.src = data;
-  p.src_stride = stride;
-  p.ld = padded(cols);
-  p.out = ws.take<uint16_t>(rows * p.ld);
-  p.rows = rows;
-  p.cols = static_cast<int>(cols);
-  got = {p.out, p.ld};
-  return ws.dry() ? hipSuccess : launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
 }
 
 template <typename P>
@@ -186,6 +144,23 @@ hipError_t multiply(const ProductArgs& p, const Laid& a, const Laid& b, int dtyp
 }
 
 }  // namespace
+
+hipError_t lay_out(const void* data, int64_t stride, int64_t rows, int64_t cols, int dtype, Workspace& ws, Laid& got,
+                   hipStream_t stream) {
+  if (as_it_is(data, stride, cols, dtype)) {
+    got = {data, stride};
+    return hipSuccess;
+  }
+  PrepareArgs p{};
+  p.src = data;
+  p.src_stride = stride;
+  p.ld = padded(cols);
+  p.out = ws.take<uint16_t>(rows * p.ld);
+  p.rows = rows;
+  p.cols = static_cast<int>(cols);
+  got = {p.out, p.ld};
+  return ws.dry() ? hipSuccess : launch_prepare(p, dtype, prepare_blocks(dtype, rows, cols), stream);
+}
 
 hipError_t launch_linear(const LinearArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
   Workspace ws(workspace);

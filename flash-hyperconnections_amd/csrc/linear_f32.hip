@@ -173,8 +173,9 @@ __device__ __forceinline__ void multiply(const Finder<ACols, kTile * Tall>& fa, 
   }
 }
 
-template <int Tall, bool ACols, bool BCols>
+template <int Tall, bool ACols, bool BCols, Finish F>
 __global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ProductArgs p) {
+  if (!fit<F, ACols>(p)) return;
   constexpr int kBuffer = 3 * (kPanel<kTile * Tall> + kPanel<kTile>);
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];  // [buffer][A's parts, B's parts]
   const int lane = threadIdx.x & 63;
@@ -232,14 +233,15 @@ __global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ProductArgs p)
         for (int e = 0; e < 4; ++e) v[e] = large[t][j][4 * q + e] + small[t][j][4 * q + e];
         park(area, 32 * t + (lane & 31), 8 * j + 2 * q + (lane >> 5), v);
       }
-  finish_parked<F32, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
+  finish_parked<F32, F, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // Sums of one step, at most 32 terms: one buffer, so that two workgroups share a compute
 // unit and one stores while the other loads.  Bound by the stores: dx of 16384 x 4096 into
 // 1 to 32 takes 56 to 63 us (268 MB), in the kernel above 79 to 85.
-template <bool ACols, bool BCols>
+template <bool ACols, bool BCols, Finish F>
 __global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ProductArgs p) {
+  if (!fit<F, ACols>(p)) return;
   constexpr int kParked = 8 * 8192;  // 32 x 64 sums of each wavefront
   static_assert(6 * kPanel<kTile> <= kParked, "the parts fit where the sums go");
   __shared__ __attribute__((aligned(1024))) char lds[kParked];
@@ -277,29 +279,22 @@ __global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ProductArgs p) {
       for (int e = 0; e < 4; ++e) v[e] = large[0][j][4 * q + e] + small[0][j][4 * q + e];
       park(area, lane & 31, 8 * j + 2 * q + (lane >> 5), v);
     }
-  finish_parked<F32, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
-}
-
-template <int Tall>
-void run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(kThreads);
-  if (!a_cols && !b_cols) f32_product_kernel<Tall, false, false><<<grid, block, 0, stream>>>(p);
-  if (!a_cols && b_cols) f32_product_kernel<Tall, false, true><<<grid, block, 0, stream>>>(p);
-  if (a_cols && b_cols) f32_product_kernel<Tall, true, true><<<grid, block, 0, stream>>>(p);
+  finish_parked<F32, F, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
 }
 
 }  // namespace
 
-hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
-  if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
-  if (p.side_m == kTile && p.k <= kDepth && p.slices == 1) {
-    const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n)), block(kThreads);
-    if (!a_cols && !b_cols) f32_outer_kernel<false, false><<<grid, block, 0, stream>>>(p);
-    if (!a_cols && b_cols) f32_outer_kernel<false, true><<<grid, block, 0, stream>>>(p);
-    if (a_cols && b_cols) f32_outer_kernel<true, true><<<grid, block, 0, stream>>>(p);
-  } else if (p.side_m == kTile) run<1>(p, a_cols, b_cols, stream);
-  else run<2>(p, a_cols, b_cols, stream);
-  return hipGetLastError();
+hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(kThreads);
+  return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
+    if (p.side_m == kTile && p.k <= kDepth && p.slices == 1)
+      f32_outer_kernel<a.value, b.value, f.value><<<dim3(grid.x), block, 0, stream>>>(p);
+    else if (p.side_m == kTile)
+      f32_product_kernel<1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+    else
+      f32_product_kernel<2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace fh

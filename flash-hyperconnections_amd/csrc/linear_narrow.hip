@@ -164,7 +164,7 @@ __device__ __forceinline__ void split_three(const float (&v)[3][8], U32x4 (&w)[3
 }
 
 // LongA: A is the long operand.
-template <typename T, bool LongA, bool LongCols, bool ShortCols>
+template <typename T, bool LongA, bool LongCols, bool ShortCols, Finish F>
 __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * kRing * kSlot];
   const int lane = threadIdx.x & 63;
@@ -173,6 +173,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
   // Each die takes neighbouring tiles: in columns one tile's 512 bytes of a row lie in two
   // of an L2's sixteen channels.
   const Tile tile = tile_of(p, blockIdx.x);
+  fit_live<F, LongA ? LongCols : ShortCols>(p);
   const int first = (tile.m + tile.n) * (LongCols ? 4 * kLong : kLong) + (LongCols ? wave * kLong : 0);
   constexpr bool f32 = T::code == F32::code;
   constexpr int E = f32 ? 4 : 2;
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
       const int m = i / groups, n = i % groups * 8;
       float v[8];
       get(area, m, n, v);
-      finish_some<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+      finish_some<T, F, groups>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
     }
   } else {
     __syncthreads();
@@ -296,23 +297,13 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    finish_some<T>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+    finish_some<T, F, groups>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
   }
-}
-
-template <typename T, bool LongA>
-hipError_t run(const ProductArgs& p, bool long_cols, bool short_cols, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(LongA ? p.tiles_m : p.tiles_n), static_cast<uint32_t>(p.slices)), block(256);
-  if (!long_cols && !short_cols) narrow_product_kernel<T, LongA, false, false><<<grid, block, 0, stream>>>(p);
-  if (long_cols && !short_cols) narrow_product_kernel<T, LongA, true, false><<<grid, block, 0, stream>>>(p);
-  if (!long_cols && short_cols) narrow_product_kernel<T, LongA, false, true><<<grid, block, 0, stream>>>(p);
-  if (long_cols && short_cols) narrow_product_kernel<T, LongA, true, true><<<grid, block, 0, stream>>>(p);
-  return hipGetLastError();
 }
 
 }  // namespace
 
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices) {
   if (p.m > kShort && p.n > kShort) return false;
   const bool f32 = dtype == F32::code;
   if (f32) {
@@ -333,15 +324,23 @@ bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   // Slices of at least four strips a wavefront until every compute unit has a workgroup; in
   // columns of 16 bits three for each (dW of 16384 x 16384 into 16: 149 us with 4 slices, 90
   // with 12); FP32 one (dx of 1 x 4096 x 16384: 69 us, with three 83).
-  p.slices = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>((compute_units() * (cols && !f32 ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
+  const int64_t slices =
+      std::min<int64_t>((compute_units() * (cols && !f32 ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16));
+  p.slices = most_slices == 1 ? 1 : static_cast<int>(std::max<int64_t>(1, slices));
   return true;
 }
 
-hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
+hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
+                                 hipStream_t stream) {
+  const bool long_a = p.m > p.n;
+  const dim3 grid(static_cast<uint32_t>(long_a ? p.tiles_m : p.tiles_n), static_cast<uint32_t>(p.slices)), block(256);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    return p.m > p.n ? run<T, true>(p, a_cols, b_cols, stream) : run<T, false>(p, b_cols, a_cols, stream);
+    return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
+      if (long_a) narrow_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      else narrow_product_kernel<T, false, b.value, a.value, f.value><<<grid, block, 0, stream>>>(p);
+      return hipGetLastError();
+    });
   });
 }
 

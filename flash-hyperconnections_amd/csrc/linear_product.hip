@@ -78,8 +78,9 @@ __device__ __forceinline__ void step(Feeder<ACols, kTile * Tall>& a, Feeder<BCol
   b.advance();
 }
 
-template <typename T, int Tall, bool ACols, bool BCols>
+template <typename T, int Tall, bool ACols, bool BCols, Finish F>
 __global__ __launch_bounds__(512, 2) void product_kernel(ProductArgs p) {
+  if (!fit<F, ACols>(p)) return;
   using S = Shape<Tall>;
   constexpr int kRing = S::kRing;
   __shared__ __attribute__((aligned(1024))) char lds[kRing * (S::kA + S::kB)];  // A's ring, B's ring
@@ -140,14 +141,15 @@ __global__ __launch_bounds__(512, 2) void product_kernel(ProductArgs p) {
         park(area, 32 * i + (lane & 31), 8 * j + 2 * q + (lane >> 5),
              Floats4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
       }
-  finish_parked<T, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
+  finish_parked<T, F, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // Sums of one step, at most 64 terms: two workgroups a compute unit, one storing while
 // the other loads.  Bound by the stores: 16384 x 16 x 16384 bf16 (537 MB) takes 124 to
 // 137 us; tiles of 256 x 256 took 157 to 166, the 128 x 128 tiles with a ring 179.
-template <typename T, bool ACols, bool BCols>
+template <typename T, bool ACols, bool BCols, Finish F>
 __global__ __launch_bounds__(512, 4) void outer_product_kernel(ProductArgs p) {
+  if (!fit<F, ACols>(p)) return;
   __shared__ __attribute__((aligned(1024))) char lds[8 * 8192];  // A's and B's step, then the results
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(512, 4) void outer_product_kernel(ProductArgs p) {
     for (int q = 0; q < 4; ++q)
       park(area, lane & 31, 8 * j + 2 * q + (lane >> 5),
            Floats4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]});
-  finish_parked<T, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
+  finish_parked<T, F, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
 }
 
 // sum += Count slices `size` apart, in order, all on their way at once.
@@ -204,8 +206,10 @@ __device__ __forceinline__ void add_slices(const float*& from, int64_t size, int
 // Adds the slices in order and finishes.  Bound by the loads' latency: 12 slices of 16 x
 // 16384 sums take 5.3 us, and took 7.9 with each waited for; 8 of 64 x 4096 take 4.1 and
 // took 5.1.  (Workgroups of one wavefront and of four take the same time.)
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
+template <typename T, Finish F>
+__global__ __launch_bounds__(256) void join_kernel(ProductArgs p, bool a_cols) {
+  if (a_cols) fit_live<F, true>(p);
+  else fit_live<F, false>(p);
   const int across = (p.n + 7) / 8, slices = p.slices;
   const int64_t total = static_cast<int64_t>(p.m) * across, size = static_cast<int64_t>(p.m) * p.n;
   p.slices = 1;
@@ -219,37 +223,30 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p) {
     if (slices & 4) add_slices<4>(from, size, left, sum);
     if (slices & 2) add_slices<2>(from, size, left, sum);
     if (slices & 1) add_slices<1>(from, size, left, sum);
-    finish_some<T>(p, 0, row, col, sum);
+    finish_some<T, F, 1>(p, 0, row, col, sum);
   }
 }
 
 template <typename T>
-hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
+hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
-  if (p.k <= kStep && p.slices == 1) {
-    if (!a_cols && !b_cols) outer_product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
-    if (!a_cols && b_cols) outer_product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
-    if (a_cols && b_cols) outer_product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
+  return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
+    if (p.k <= kStep && p.slices == 1)
+      outer_product_kernel<T, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+    else if (p.side_m == kTile)
+      product_kernel<T, 1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+    else
+      product_kernel<T, 2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
     return hipGetLastError();
-  }
-  if (p.side_m == kTile) {
-    if (!a_cols && !b_cols) product_kernel<T, 1, false, false><<<grid, block, 0, stream>>>(p);
-    if (!a_cols && b_cols) product_kernel<T, 1, false, true><<<grid, block, 0, stream>>>(p);
-    if (a_cols && b_cols) product_kernel<T, 1, true, true><<<grid, block, 0, stream>>>(p);
-  } else {
-    if (!a_cols && !b_cols) product_kernel<T, 2, false, false><<<grid, block, 0, stream>>>(p);
-    if (!a_cols && b_cols) product_kernel<T, 2, false, true><<<grid, block, 0, stream>>>(p);
-    if (a_cols && b_cols) product_kernel<T, 2, true, true><<<grid, block, 0, stream>>>(p);
-  }
-  if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
-  return hipGetLastError();
+  });
 }
 
 template <typename T>
-hipError_t join(const ProductArgs& p, hipStream_t stream) {
+hipError_t join(const ProductArgs& p, bool a_cols, Finish finish, hipStream_t stream) {
   const int64_t groups = static_cast<int64_t>(p.m) * ((p.n + 7) / 8);
-  join_kernel<T><<<dim3(static_cast<uint32_t>(std::min<int64_t>((groups + 255) / 256, 4096))), dim3(256), 0,
-                   stream>>>(p);
+  const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((groups + 255) / 256, 4096))), block(256);
+  if (finish == Finish::kSum) join_kernel<T, Finish::kSum><<<grid, block, 0, stream>>>(p, a_cols);
+  else join_kernel<T, Finish::kLinear><<<grid, block, 0, stream>>>(p, a_cols);
   return hipGetLastError();
 }
 
@@ -262,9 +259,10 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 
 }  // namespace
 
-void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
+void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
-  if (plan_narrow_product(p, dtype, a_cols, b_cols)) return;
+  const int most = finish == Finish::kStats || finish == Finish::kSlope ? 1 : 16;
+  if (plan_narrow_product(p, dtype, a_cols, b_cols, most)) return;
   if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);
     p.slices = 1;
@@ -294,7 +292,7 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   const auto consider = [&](const Cost& c) {
     set_tiles(p, c.rows, c.cols);
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-    for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
+    for (int64_t s = 1; s <= most && s <= std::max<int64_t>(1, steps / 4); ++s) {
       const double full = std::min(1.0, static_cast<double>(tiles * s) / static_cast<double>(units));
       const double us =
           rounds(tiles * s) * (c.fixed + (c.step + c.shared * full) * static_cast<double>((steps + s - 1) / s)) +
@@ -314,19 +312,20 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   p = chosen;
 }
 
-hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
+hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
+                          Finish finish) {
   hipError_t err;
   if (p.side_n < kTile) {
-    err = launch_narrow_product(p, dtype, a_cols, b_cols, stream);
+    err = launch_narrow_product(p, dtype, a_cols, b_cols, finish, stream);
   } else if (dtype == F32::code) {
-    err = launch_f32_product(p, a_cols, b_cols, stream);
+    err = launch_f32_product(p, a_cols, b_cols, finish, stream);
   } else if (p.side_n == 256) {
-    err = launch_wide_product(p, dtype, a_cols, b_cols, stream);
+    err = launch_wide_product(p, dtype, a_cols, b_cols, finish, stream);
   } else {
-    err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
+    err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, finish, stream); });
   }
   if (err != hipSuccess || p.slices == 1) return err;
-  return with_type(dtype, [&](auto t) { return join<decltype(t)>(p, stream); });
+  return with_type(dtype, [&](auto t) { return join<decltype(t)>(p, a_cols, finish, stream); });
 }
 
 }  // namespace fh

@@ -86,8 +86,9 @@ __device__ __forceinline__ void step(Feeder<ACols, kSide>& a, Feeder<BCols, kSid
   a.advance();
 }
 
-template <typename T, bool ACols, bool BCols>
+template <typename T, bool ACols, bool BCols, Finish F>
 __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
+  if (!fit<F, ACols>(p)) return;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kBuffer];  // A, A, B, B
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -149,24 +150,21 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
           park(area, 32 * i + (lane & 31), 8 * j + 2 * q + (lane >> 5),
                Floats4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
         }
-    finish_parked<T, 64>(p, slice, area, m0 + wm + 64 * half, n0 + wn, lane);
+    finish_parked<T, F, 64>(p, slice, area, m0 + wm + 64 * half, n0 + wn, lane);
   }
-}
-
-template <typename T>
-hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
-  if (!a_cols && !b_cols) wide_product_kernel<T, false, false><<<grid, block, 0, stream>>>(p);
-  if (!a_cols && b_cols) wide_product_kernel<T, false, true><<<grid, block, 0, stream>>>(p);
-  if (a_cols && b_cols) wide_product_kernel<T, true, true><<<grid, block, 0, stream>>>(p);
-  if (a_cols && !b_cols) return hipErrorInvalidValue;  // no such product
-  return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream) {
-  return with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, stream); });
+hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
+                               hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
+  return with_half_type(dtype, [&](auto t) {
+    return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
+      wide_product_kernel<decltype(t), a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      return hipGetLastError();
+    });
+  });
 }
 
 }  // namespace fh

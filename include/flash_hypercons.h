@@ -206,6 +206,52 @@ FH_API int fh_clip_gradients(int count, const void* const* grads, void* const* o
                       const int* dtypes, double norm_type, double max_norm, float* norm, void* workspace,
                       int64_t* workspace_bytes, hipStream_t stream);
 
+/* ---- the two ends of a network ---------------------------------------------------
+ *
+ * Rows of a table into the residual streams, and the softmax cross entropy of a linear
+ * layer over a large vocabulary; the reference has neither.  Rows, results and workspaces
+ * as above. */
+
+/* y[i, s] = scale weight[tokens[i]] for the `streams` (>= 1) streams s of [count, streams,
+ * cols], weight [vocab, cols]; 0 <= count < 2^28, 1 <= vocab < 2^28, 1 <= cols < 2^24.  A
+ * token that is not in 0 .. vocab - 1 gives NaN. */
+FH_API int fh_embedding(const int64_t* tokens, const void* weight, int64_t weight_stride, double scale, int streams,
+                 void* y, int dtype, int64_t count, int64_t vocab, int64_t cols, hipStream_t stream);
+
+/* Its gradient: dweight[v] = scale times the sum of grad[i, s] over the i with
+ * tokens[i] = v, in their order, and s, added in FP32; zeros for a v that does not occur
+ * or is `padding` (-1: none).  grad: [count * streams, cols].  Tokens out of range add to
+ * nothing. */
+FH_API int fh_embedding_backward(const int64_t* tokens, const void* grad, int64_t grad_stride, double scale, int streams,
+                          int64_t padding, void* dweight, void* workspace, int64_t* workspace_bytes, int dtype,
+                          int64_t count, int64_t vocab, int64_t cols, hipStream_t stream);
+
+/* What becomes of the losses of the rows: each by itself, their sum, or their mean over
+ * the rows that have a target (NaN where none has). */
+#define FH_REDUCE_NONE 0
+#define FH_REDUCE_SUM 1
+#define FH_REDUCE_MEAN 2
+
+/* loss[i] = log(sum over v of exp(z[i, v])) - z[i, targets[i]], z = x weight^T + bias for x
+ * [rows, cols] and weight [vocab, cols], in FP32 and without keeping z; 0 <= rows < 2^24,
+ * 1 <= cols, vocab < 2^22.  A row whose target is `ignore` has a loss of 0 and no part in
+ * anything else, whatever is in it; another target that is not in 0 .. vocab - 1 gives NaN.
+ * bias ([vocab] or NULL) is of bias_dtype: dtype or FH_DTYPE_F32.  loss: a float, [rows] of
+ * them for FH_REDUCE_NONE.  lse (float [rows]) is for the backward. */
+FH_API int fh_linear_cross_entropy(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                            const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore, int reduction,
+                            float* loss, float* lse, void* workspace, int64_t* workspace_bytes, int dtype,
+                            int64_t rows, int64_t cols, int64_t vocab, hipStream_t stream);
+
+/* Its gradients for the upstream gradient grad (a float, [rows] of them for FH_REDUCE_NONE):
+ * dx [rows, cols], dweight [vocab, cols] and dbias [vocab] (bias_dtype); each may be NULL.
+ * `lse` is the forward's; bias is the forward's too. */
+FH_API int fh_linear_cross_entropy_backward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                     const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore,
+                                     int reduction, const float* lse, const float* grad, void* dx, void* dweight,
+                                     void* dbias, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                                     int64_t cols, int64_t vocab, hipStream_t stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 FH_API const char* fh_last_error(void);
 
