@@ -55,7 +55,6 @@ __global__ __launch_bounds__(256) void embedding_kernel(EmbeddingArgs a) {
 // ---- sorting -------------------------------------------------------------------------
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kMostTile = 16 * kThreads;
 
 // A token's key: itself, or the first number past the vocabulary where it has no gradient.
 __device__ __forceinline__ uint32_t key_of(const EmbeddingArgs& a, int64_t i) {
@@ -128,6 +127,8 @@ __device__ __forceinline__ void rank(const uint32_t (&key)[P], int shift, uint32
   for (int i = 0; i < P; ++i) place[i] += counts[(key[i] >> shift & ((1u << Bits) - 1)) * kWaves + wave];
 }
 
+constexpr int kMostAlone = 4 * kThreads;
+
 // Up to 1024 P tokens, in one workgroup.  Three passes for 2^18 words; 16384 tokens in 18 us.
 template <int P>
 __global__ __launch_bounds__(kThreads) void sort_tile_kernel(EmbeddingArgs a, int bits, uint32_t* keys, int* order) {
@@ -172,29 +173,31 @@ __device__ __forceinline__ uint32_t key_at(const EmbeddingArgs& a, const uint32_
 }
 
 // How often each digit occurs in each tile: table[tile][digit].
-__global__ __launch_bounds__(kThreads) void count_kernel(EmbeddingArgs a, const uint32_t* keys, int shift,
+__global__ __launch_bounds__(kThreads) void count_kernel(EmbeddingArgs a, int tile, const uint32_t* keys, int shift,
                                                          uint32_t* table) {
   __shared__ uint32_t counts[1 << kDigit];
   for (int d = threadIdx.x; d < 1 << kDigit; d += kThreads) counts[d] = 0;
   __syncthreads();
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kMostTile;
-  for (int i = threadIdx.x; i < kMostTile && first + i < a.count; i += kThreads)
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * tile;
+  for (int i = threadIdx.x; i < tile && first + i < a.count; i += kThreads)
     atomicAdd(counts + (key_at(a, keys, first + i) >> shift & ((1u << kDigit) - 1)), 1u);
   __syncthreads();
   for (int d = threadIdx.x; d < 1 << kDigit; d += kThreads) table[(static_cast<int64_t>(blockIdx.x) << kDigit) + d] = counts[d];
 }
 
-// Moves a tile's keys to their places in the whole.
+// Moves a tile's 1024 P keys to their places in the whole.
+template <int P>
 __global__ __launch_bounds__(kThreads) void move_kernel(EmbeddingArgs a, const uint32_t* keys, const int* order,
                                                         int shift, const uint32_t* table, uint32_t* to_keys,
                                                         int* to_order) {
-  constexpr int P = kMostTile / kThreads, kDigits = 1 << kDigit;
+  constexpr int kDigits = 1 << kDigit;
   __shared__ uint32_t counts[kWaves << kDigit], area[kWaves], base[kDigits], other[kWaves];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kMostTile;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (P * kThreads);
   const int at = (threadIdx.x >> 6) * 64 * P + (threadIdx.x & 63);
   // A digit's place: after the smaller digits of all tiles and this one of the tiles before.
   uint32_t all[1] = {0}, before = 0;
   if (threadIdx.x < kDigits) {
+#pragma unroll 16
     for (uint32_t tile = 0; tile < gridDim.x; ++tile) {
       const uint32_t n = table[(static_cast<int64_t>(tile) << kDigit) + threadIdx.x];
       before += tile < blockIdx.x ? n : 0;
@@ -336,61 +339,65 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs p) {
   else put<T>(p, sum, key, c);
 }
 
+// The first place from `low` on whose key is above `key`, by a wavefront that asks 64 places at a time.
+__device__ __forceinline__ int64_t end_of_run(const uint32_t* keys, int64_t low, int64_t high, uint32_t key) {
+  while (low < high) {
+    const int64_t step = (high - low + 63) / 64, at = low + (threadIdx.x & 63) * step;
+    const int within = __popcll(__ballot(at < high && keys[at] <= key));  // of the places asked, in a row
+    if (within == 0) return low;
+    const int64_t last = low + (within - 1) * step;
+    high = last + step < high ? last + step : high;
+    low = last + 1;
+  }
+  return low;
+}
+
 // Runs over several chunks, by the chunk in which they begin: its part and those of the chunks after it, in
-// order, a quarter of them a wavefront.
+// order, an eighth of them a wavefront.
+constexpr int kJoining = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void join_runs_kernel(SumArgs p) {
-  constexpr int V = kVec<T>;
-  __shared__ float area[4][V][64];
+__global__ __launch_bounds__(64 * kJoining) void join_runs_kernel(SumArgs p) {
+  constexpr int V = kVec<T>, kAhead = 8;
+  __shared__ float area[kJoining][V][64];
   const int64_t chunk = blockIdx.x / p.strips, first = chunk * p.chunk, end = first + p.chunk;
   if (end >= p.a.count) return;
   const uint32_t key = p.keys[end - 1];
   if (key >= static_cast<uint32_t>(p.a.vocab) || p.keys[end] != key || (first > 0 && p.keys[first - 1] == key)) return;
-  // The first place past the run.
-  int64_t low = end, high = p.a.count;
-  while (low < high) {
-    const int64_t mid = (low + high) / 2;
-    if (p.keys[mid] <= key) low = mid + 1;
-    else high = mid;
-  }
+  const int64_t last = end_of_run(p.keys, end, p.a.count, key) - 1;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = (static_cast<int>(blockIdx.x) % p.strips * 64 + lane) * V, cols = static_cast<int>(p.a.cols);
-  const int64_t parts = (low - 1) / p.chunk - chunk + 1, from = parts * wave / 4, to = parts * (wave + 1) / 4;
+  const int64_t parts = last / p.chunk - chunk + 1, to = parts * (wave + 1) / kJoining;
   float sum[V] = {};
-  const auto load = [&](int64_t part, float (&f)[V]) {
-    const float* row = p.partial + ((chunk + part) * 2 + (part == 0 ? 1 : 0)) * p.a.cols;
+  for (int64_t i = parts * wave / kJoining; i < to; i += kAhead) {
+    float f[kAhead][V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = 0.f;
-    if (c + V <= cols) {
-      __builtin_memcpy(f, row + c, sizeof(f));
-    } else {
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u >= to) break;
+      const float* row = p.partial + ((chunk + i + u) * 2 + (i + u == 0 ? 1 : 0)) * p.a.cols;
+      if (c + V <= cols) {
+        __builtin_memcpy(f[u], row + c, sizeof(f[u]));
+      } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (c + k < cols) f[k] = row[c + k];
+        for (int k = 0; k < V; ++k) f[u][k] = c + k < cols ? row[c + k] : 0.f;
+      }
     }
-  };
-  int64_t i = from;
-  for (; i + 4 <= to; i += 4) {
-    float f[4][V];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load(i + u, f[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < kAhead; ++u) {
+      if (i + u >= to) break;
 #pragma unroll
       for (int k = 0; k < V; ++k) sum[k] += f[u][k];
-  }
-  for (; i < to; ++i) {
-    float f[V];
-    load(i, f);
-#pragma unroll
-    for (int k = 0; k < V; ++k) sum[k] += f[k];
+    }
   }
 #pragma unroll
   for (int k = 0; k < V; ++k) area[wave][k][lane] = sum[k];
   __syncthreads();
   if (wave != 0) return;
 #pragma unroll
-  for (int k = 0; k < V; ++k) sum[k] = ((area[0][k][lane] + area[1][k][lane]) + area[2][k][lane]) + area[3][k][lane];
+  for (int k = 0; k < V; ++k) {
+    sum[k] = area[0][k][lane];
+#pragma unroll
+    for (int w = 1; w < kJoining; ++w) sum[k] += area[w][k][lane];
+  }
   put<T>(p, sum, key, c);
 }
 
@@ -402,23 +409,26 @@ hipError_t sort_tokens(const EmbeddingArgs& a, Workspace& ws, uint32_t*& keys, i
   order = ws.take<int>(a.count);
   int bits = 1;
   while (a.vocab >> bits != 0) ++bits;  // of the vocabulary's size, the last key
-  if (a.count <= kMostTile) {
+  if (a.count <= kMostAlone) {
     if (ws.dry()) return hipSuccess;
     if (a.count <= kThreads) sort_tile_kernel<1><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
-    else if (a.count <= 4 * kThreads) sort_tile_kernel<4><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
-    else sort_tile_kernel<16><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
+    else sort_tile_kernel<4><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
     return hipGetLastError();
   }
   auto* other_keys = ws.take<uint32_t>(a.count);
   auto* other_order = ws.take<int>(a.count);
-  const dim3 tiles = blocks_of(a.count, kMostTile);
+  const int each = a.count <= 64 * kThreads ? 1 : a.count <= 512 * kThreads ? 4 : 16;
+  const int tile = each * kThreads;
+  const dim3 tiles = blocks_of(a.count, tile), block(kThreads);
   auto* table = ws.take<uint32_t>(static_cast<int64_t>(tiles.x) << kDigit);
   if (ws.dry()) return hipSuccess;
   for (int shift = 0; shift < bits; shift += kDigit) {
     const uint32_t* from = shift > 0 ? keys : nullptr;
-    count_kernel<<<tiles, dim3(kThreads), 0, stream>>>(a, from, shift, table);
-    move_kernel<<<tiles, dim3(kThreads), 0, stream>>>(a, from, shift > 0 ? order : nullptr, shift, table, other_keys,
-                                                      other_order);
+    const int* places = shift > 0 ? order : nullptr;
+    count_kernel<<<tiles, block, 0, stream>>>(a, tile, from, shift, table);
+    if (each == 1) move_kernel<1><<<tiles, block, 0, stream>>>(a, from, places, shift, table, other_keys, other_order);
+    else if (each == 4) move_kernel<4><<<tiles, block, 0, stream>>>(a, from, places, shift, table, other_keys, other_order);
+    else move_kernel<16><<<tiles, block, 0, stream>>>(a, from, places, shift, table, other_keys, other_order);
     std::swap(keys, other_keys);
     std::swap(order, other_order);
   }
@@ -468,7 +478,7 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* wo
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     sum_kernel<T><<<dim3(static_cast<uint32_t>(p.summing + (a.vocab + 63) / 64)), dim3(256), 0, stream>>>(p);
-    if (p.chunks > 1) join_runs_kernel<T><<<dim3(static_cast<uint32_t>(units)), dim3(256), 0, stream>>>(p);
+    if (p.chunks > 1) join_runs_kernel<T><<<dim3(static_cast<uint32_t>(units)), dim3(64 * kJoining), 0, stream>>>(p);
     return hipGetLastError();
   });
 }
