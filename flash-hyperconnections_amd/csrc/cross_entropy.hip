@@ -292,20 +292,28 @@ hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, Workspace& ws, R
 }
 
 // A product of the loss; a sum over few results may go in slices.
-hipError_t multiply(ProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols, Finish finish,
+hipError_t multiply(LossProductArgs& p, const Laid& a, const Laid& b, int dtype, bool a_cols, bool b_cols, Finish finish,
                     Workspace& ws, hipStream_t stream) {
   p.a = a.data;
   p.lda = a.ld;
   p.b = b.data;
   p.ldb = b.ld;
   plan_product(p, dtype, a_cols, b_cols, finish);
-  if (p.slices > 1) p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
-  return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream, finish);
+  const int64_t groups = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.slices, units = compute_units();
+  if (finish == Finish::kSum && !a_cols && p.side_n >= 128 && (p.slices > 1 || p.k > 64) && groups <= 4 * units) {
+    // Rows without a target may leave compute units without a tile, and the sum go in more slices.
+    p.loss.groups = static_cast<int>(groups);
+    p.loss.units = static_cast<int>(units);
+    p.partial = ws.take<float>(groups / p.tiles_n * p.side_m * p.n);
+  } else if (p.slices > 1) {
+    p.partial = ws.take<float>(static_cast<int64_t>(p.slices) * p.m * p.n);
+  }
+  return ws.dry() ? hipSuccess : launch_product(p, dtype, a_cols, b_cols, stream, finish, &p.loss);
 }
 
 // z = x W^T + b of `count` rows and `outs` of the vocabulary.
-ProductArgs logits(const LossArgs& a, const Rows& rows, int64_t row0, int64_t count, int64_t col0, int64_t outs) {
-  ProductArgs p{};
+LossProductArgs logits(const LossArgs& a, const Rows& rows, int64_t row0, int64_t count, int64_t col0, int64_t outs) {
+  LossProductArgs p{};
   p.m = static_cast<int>(count);
   p.n = static_cast<int>(outs);
   p.k = static_cast<int>(a.cols);
@@ -344,7 +352,7 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
   while (across > a.rows || (across > 4 && a.rows / across < compute_units())) across >>= 1;
   if (err == hipSuccess) {
     err = in_slices(a.rows, most, [&](int64_t row0, int64_t count) {
-      ProductArgs p = logits(a, rows, row0, count, 0, a.vocab);
+      LossProductArgs p = logits(a, rows, row0, count, 0, a.vocab);
       p.loss.stats = stats;
       p.loss.ld = most;
       p.loss.chosen = chosen;
@@ -414,20 +422,20 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
       const hipError_t all = in_slices(a.rows, most_rows, [&](int64_t row0, int64_t count) {
         const Laid xp = rows_from(rows.x, row0, a.dtype);
         hipError_t e = shared([&](Workspace& part) {
-          ProductArgs p = logits(a, rows, row0, count, col0, outs);
+          LossProductArgs p = logits(a, rows, row0, count, col0, outs);
           p.loss.row = r.row + row0;
           p.loss.ld = (outs + 7) / 8 * 8;
           p.out = const_cast<void*>(dz.data);
           return multiply(p, xp, wp, a.dtype, false, false, Finish::kSlope, part, stream);
         });
         const Laid d{dz.data, (outs + 7) / 8 * 8};
-        ProductArgs s{};
+        LossProductArgs s{};
         s.loss.live = rows.live;
         s.loss.row0 = static_cast<int>(row0);
         s.loss.scale = r.scale;
         if (e == hipSuccess && a.dx != nullptr) {
           e = shared([&](Workspace& part) {
-            ProductArgs p = s;
+            LossProductArgs p = s;
             p.m = static_cast<int>(count);
             p.n = static_cast<int>(a.cols);
             p.k = static_cast<int>(outs);
@@ -441,7 +449,7 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
         }
         if (e == hipSuccess && a.dweight != nullptr) {
           e = shared([&](Workspace& part) {
-            ProductArgs p = s;
+            LossProductArgs p = s;
             p.m = static_cast<int>(outs);
             p.n = static_cast<int>(a.cols);
             p.k = static_cast<int>(count);

@@ -33,6 +33,7 @@ struct LossParts {
   int first, last;       // kSum: whether sums is not read, or not written but scaled into out
   const float* scale;    // kSum
   const int* index;      // kSum: [rows] rows of out, or null
+  int groups, units;     // kSum, A in rows: workgroups launched and compute units, or 0 where slices stay as planned
 };
 
 // D[m][n] = sum over k of A[m][k] B[n][k] and what follows it.  An operand is in
@@ -54,29 +55,52 @@ struct ProductArgs {
   int act;
   void* saved;           // receives the sum with its bias, or null
   void* out;             // [m, n] contiguous
+};
+struct LossProductArgs : ProductArgs {
   LossParts loss;
 };
+// What a kernel with this finish is given.
+template <Finish F>
+using ArgsOf = std::conditional_t<F == Finish::kLinear, ProductArgs, LossProductArgs>;
+template <Finish F>
+ArgsOf<F> args_of(const ProductArgs& p, const LossParts* loss) {
+  ArgsOf<F> args{};
+  static_cast<ProductArgs&>(args) = p;
+  if constexpr (F != Finish::kLinear) args.loss = *loss;
+  return args;
+}
 
 // Fits a product's rows, or its sum where A is in columns, to what is live.
 template <Finish F, bool ACols>
-__device__ __forceinline__ void fit_live(ProductArgs& p) {
+__device__ __forceinline__ void fit_live(ArgsOf<F>& p) {
   if constexpr (F != Finish::kLinear) {
     const int more = *p.loss.live - p.loss.row0, live = more > 0 ? more : 0;
     int& rows = ACols ? p.k : p.m;
     rows = live < rows ? live : rows;
   }
 }
-// The same and its tiles; false for a workgroup past them.
+// The same and its tiles; false for a workgroup past them.  A sum of fewer rows than it was planned for goes in
+// more slices, as far as workgroups were launched, for no compute unit to be without (4096 x 2048 rows of which
+// 1640 have a target, 32768 words: dx 325 -> 212 us).
 template <Finish F, bool ACols>
-__device__ __forceinline__ bool fit(ProductArgs& p) {
-  if constexpr (F != Finish::kLinear) {
+__device__ __forceinline__ bool fit(ArgsOf<F>& p) {
+  if constexpr (F != Finish::kLinear && !ACols) {
+    const int planned = p.tiles_m;
     fit_live<F, ACols>(p);
-    if constexpr (!ACols) {
-      p.tiles_m = (p.m + p.side_m - 1) / p.side_m;
-      return blockIdx.x < static_cast<uint32_t>(p.tiles_m * p.tiles_n);
+    p.tiles_m = (p.m + p.side_m - 1) / p.side_m;
+    const int tiles = p.tiles_m * p.tiles_n;
+    if constexpr (F == Finish::kSum) {
+      if (p.loss.groups != 0 && p.tiles_m < planned && tiles > 0) {
+        const int most = p.loss.groups < p.loss.units ? p.loss.groups : p.loss.units;
+        const int slices = most / tiles < 16 ? most / tiles : 16;
+        p.slices = slices > p.slices ? slices : p.slices;
+      }
     }
+    return blockIdx.x + gridDim.x * blockIdx.y < static_cast<uint32_t>(tiles * p.slices);
+  } else {
+    fit_live<F, ACols>(p);
+    return true;
   }
-  return true;
 }
 
 // What the backward needs of the sum z = x W^T + b: FP32 for FP32 results, and
@@ -253,10 +277,6 @@ __device__ __forceinline__ void add_bias(const ProductArgs& p, int j, int left, 
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// exp(v): the hardware's exp2 where the argument is small in size or the result is rounded
-// to 16 bits; its argument's rounding is worth |v| 2^-24 of the result.
-__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
-
 // A value of the lane that the quad's permutation or the mirror of 8 or 16 lanes gives.
 template <int Control>
 __device__ __forceinline__ float from_lane(float v) {
@@ -272,29 +292,63 @@ __device__ __forceinline__ float over_lanes(float v, F f) {
   return v;
 }
 
+// What a finish needs of a row.  It is loaded for all of a wavefront's rows at once: a load
+// waited for in each of eight turns took a quarter of a short sum's time.
+template <Finish F>
+struct RowOf {
+  __device__ __forceinline__ void load(const ArgsOf<F>&, int) {}
+};
+template <>
+struct RowOf<Finish::kStats> {
+  int label;
+  __device__ __forceinline__ void load(const LossProductArgs& p, int i) { label = i < p.m ? p.loss.label[i] - p.loss.col0 : 0; }
+};
+template <>
+struct RowOf<Finish::kSlope> {
+  int label;
+  float2 row;
+  __device__ __forceinline__ void load(const LossProductArgs& p, int i) {
+    label = i < p.m ? p.loss.label[i] - p.loss.col0 : 0;
+    row = i < p.m ? p.loss.row[i] : make_float2(0.f, 0.f);
+  }
+};
+
+// exp(v - from).  For results of 16 bits by the hardware's exp2, whose argument's rounding is
+// worth 2^-23 of |v - from|.  (One multiply-add instead of the difference overflows where both
+// are the type's lowest value.)
+template <typename T>
+__device__ __forceinline__ float exp_from(float v, float from) {
+  if constexpr (T::code == F32::code) return expf(v - from);
+  return __builtin_amdgcn_exp2f((v - from) * kLog2e);
+}
+
 // Logits of Lanes V neighbouring columns of row i, V a lane: their maximum m and the sum
 // of exp(z - m), as far as columns are valid, and the target's logit.  -inf alone gives
 // m = -inf and a sum of zero; a NaN or +inf makes the sum NaN.
 template <typename T, int Lanes, int V>
-__device__ __forceinline__ void stats_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+__device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf<Finish::kStats>& of, int i, int j,
+                                           float (&v)[V]) {
   if (i >= p.m) return;  // the same in all of these lanes
   const int left = p.n - j;
   if (left > 0) add_bias<T>(p, j, left, v);
   const float none = -__builtin_inff();
-  float m = none;
+  if (left < V) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    if (k >= left) v[k] = none;
-    m = __builtin_fmaxf(m, v[k]);
+    for (int k = 0; k < V; ++k) v[k] = k < left ? v[k] : none;
   }
+  float m = v[0];
+#pragma unroll
+  for (int k = 1; k < V; ++k) m = __builtin_fmaxf(m, v[k]);
   m = over_lanes<Lanes>(m, [](float a, float b) { return __builtin_fmaxf(a, b); });
-  const int at = p.loss.label[i] - p.loss.col0 - j;
   const float from = m == none ? 0.f : m;
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    if (k == at && k < left) p.loss.chosen[i] = v[k];
-    s += exp_of(v[k] - from);
+  for (int k = 0; k < V; ++k) s += exp_from<T>(v[k], from);
+  const int at = of.label - j;
+  if (at >= 0 && at < V && at < left) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k == at) p.loss.chosen[i] = v[k];
   }
   s = over_lanes<Lanes>(s, [](float a, float b) { return a + b; });
   if (j % 64 == 0 && left > 0) p.loss.stats[static_cast<int64_t>(j / 64) * p.loss.ld + i] = make_float2(m, s);
@@ -302,23 +356,25 @@ __device__ __forceinline__ void stats_some(const ProductArgs& p, int i, int j, f
 
 // Logits on their way to the gradients of z: (exp(z - lse) - [target]) times the row's
 // factor, rounded to the storage type, which the products that follow take.  (Root mean
-// square 0.0017 of a term in bf16, beside as much for their results' own rounding.)  A
-// factor of zero gives zeros whatever z is.
+// square 0.0017 of a term in bf16, beside as much for their results' own rounding.)
 template <typename T, int V>
-__device__ __forceinline__ void slope_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+__device__ __forceinline__ void slope_some(const LossProductArgs& p, const RowOf<Finish::kSlope>& of, int i, int j,
+                                           float (&v)[V]) {
   using S = typename T::storage;
   if (i >= p.m || j >= p.loss.ld) return;
-  const int left = p.n - j;
-  const float2 row = p.loss.row[i];
-  const int at = p.loss.label[i] - p.loss.col0 - j;
+  const int left = p.n - j, at = of.label - j;
   if (left > 0) add_bias<T>(p, j, left, v);
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    float e;
-    if constexpr (T::code == F32::code) e = expf(v[k] - row.x);
-    else e = exp_of(v[k] - row.x);
-    if (k == at) e -= 1.f;
-    v[k] = k < left && row.y != 0.f ? e * row.y : 0.f;
+  for (int k = 0; k < V; ++k) v[k] = exp_from<T>(v[k], of.row.x);
+  if (at >= 0 && at < V) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] -= k == at ? 1.f : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] *= of.row.y;
+  if (left < V) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = k < left ? v[k] : 0.f;
   }
   S e[V];
   round_some<T>(v, e);
@@ -327,7 +383,7 @@ __device__ __forceinline__ void slope_some(const ProductArgs& p, int i, int j, f
 
 // V results of a sum on their way into the sum so far, or at its end scaled and out.
 template <typename T, int V>
-__device__ __forceinline__ void sum_some(const ProductArgs& p, int i, int j, float (&v)[V]) {
+__device__ __forceinline__ void sum_some(const LossProductArgs& p, int i, int j, float (&v)[V]) {
   using S = typename T::storage;
   const int64_t at = static_cast<int64_t>(i) * p.n + j;
   const int left = p.n - j;
@@ -354,14 +410,15 @@ __device__ __forceinline__ void sum_some(const ProductArgs& p, int i, int j, flo
 // activation, residual; or into the slice's partial sums.  Lanes neighbouring lanes have
 // the results beside these.
 template <typename T, Finish F, int Lanes, int V>
-__device__ __forceinline__ void finish_some(const ProductArgs& p, int slice, int i, int j, float (&v)[V]) {
+__device__ __forceinline__ void finish_some(const ArgsOf<F>& p, const RowOf<F>& of, int slice, int i, int j,
+                                            float (&v)[V]) {
   using S = typename T::storage;
   using Z = Saved<T>;
   if constexpr (F == Finish::kStats) {
-    stats_some<T, Lanes>(p, i, j, v);
+    stats_some<T, Lanes>(p, of, i, j, v);
     return;
   } else if constexpr (F == Finish::kSlope) {
-    slope_some<T>(p, i, j, v);
+    slope_some<T>(p, of, i, j, v);
     return;
   }
   if (i >= p.m || j >= p.n) return;
@@ -405,26 +462,35 @@ __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
   *reinterpret_cast<Floats4*>(area + r * 256 + ((c ^ (r & 15)) << 4)) = v;
 }
 template <typename T, Finish F, int Rows>
-__device__ __forceinline__ void finish_parked(const ProductArgs& p, int slice, const char* area, int row, int col,
+__device__ __forceinline__ void finish_parked(const ArgsOf<F>& p, int slice, const char* area, int row, int col,
                                               int lane) {
+  constexpr int down = T::code == F32::code ? 4 : 8, turns = Rows / down;  // rows at a time
+  const int first = T::code == F32::code ? lane >> 4 : lane >> 3;
+  RowOf<F> of[turns];
+#pragma unroll
+  for (int it = 0; it < turns; ++it) of[it].load(p, row + first + down * it);
   asm volatile("" ::: "memory");  // one wavefront's LDS accesses run in order
-  if constexpr (T::code == F32::code) {
-#pragma unroll 2
-    for (int it = 0; it < Rows / 4; ++it) {
-      const int r = 4 * it + (lane >> 4), c = lane & 15;
+  const auto turn = [&](int it) {
+    const int r = down * it + first;
+    if constexpr (T::code == F32::code) {
+      const int c = lane & 15;
       float v[4];
       __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
-      finish_some<T, F, 16>(p, slice, row + r, col + 4 * c, v);
-    }
-  } else {
-#pragma unroll 2
-    for (int it = 0; it < Rows / 8; ++it) {
-      const int r = 8 * it + (lane >> 3), c = 2 * (lane & 7);
+      finish_some<T, F, 16>(p, of[it], slice, row + r, col + 4 * c, v);
+    } else {
+      const int c = 2 * (lane & 7);
       float v[8];
       __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
       __builtin_memcpy(v + 4, area + r * 256 + (((c + 1) ^ (r & 15)) << 4), 16);
-      finish_some<T, F, 8>(p, slice, row + r, col + 8 * (lane & 7), v);
+      finish_some<T, F, 8>(p, of[it], slice, row + r, col + 8 * (lane & 7), v);
     }
+  };
+  if constexpr (F == Finish::kStats || F == Finish::kSlope) {
+#pragma unroll
+    for (int it = 0; it < turns; ++it) turn(it);
+  } else {
+#pragma unroll 2
+    for (int it = 0; it < turns; ++it) turn(it);
   }
   asm volatile("" ::: "memory");
 }
@@ -471,6 +537,24 @@ __device__ __forceinline__ Tile tile_of(const ProductArgs& p, int block) {
   return {first + in % high, in / high};
 }
 
+// The same with the sum's slices.  With B in columns each die takes one eighth of the slices' tiles, those of a
+// slice in a row, so that most dies read a part of the operands that no other does, and whole rows of it: the 256
+// bytes that a tile has of each lie in few of an L2's channels (dx of 200 x 1024 into 50001 words, 16 slices: 60
+// -> 42 us).  In rows the other way is 6% faster (64 x 16384 x 4096).
+struct Piece {
+  Tile tile;
+  int slice;
+};
+template <bool BCols>
+__device__ __forceinline__ Piece piece_of(const ProductArgs& p) {
+  if (!BCols || p.slices == 1) return {tile_of(p, blockIdx.x), static_cast<int>(blockIdx.y)};
+  const int tiles = p.tiles_m * p.tiles_n, all = tiles * p.slices;
+  const int block = blockIdx.x + gridDim.x * blockIdx.y, die = block & 7, each = all >> 3, more = all & 7;
+  const int at = die * each + (die < more ? die : more) + (block >> 3);
+  const int slice = at / tiles, in = at % tiles;
+  return {{in % p.tiles_m, in / p.tiles_m}, slice};
+}
+
 // The steps of Depth in k that a slice of a sum takes.
 template <int Depth>
 struct Steps {
@@ -498,14 +582,16 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
 // vectors; false for others.
 bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices);
+// `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
-                          Finish finish = Finish::kLinear);
-hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream);
+                          Finish finish = Finish::kLinear, const LossParts* loss = nullptr);
+hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, const LossParts* loss,
+                              hipStream_t stream);
 hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
-                                 hipStream_t stream);
+                                 const LossParts* loss, hipStream_t stream);
 // 16-bit types.
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
-                               hipStream_t stream);
+                               const LossParts* loss, hipStream_t stream);
 
 // Calls f with the operands' layouts and the finish as types, where there is such a product:
 // of rows by rows (logits and their gradients too), rows by columns, columns by columns.

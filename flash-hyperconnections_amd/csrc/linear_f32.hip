@@ -174,14 +174,14 @@ __device__ __forceinline__ void multiply(const Finder<ACols, kTile * Tall>& fa, 
 }
 
 template <int Tall, bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
   constexpr int kBuffer = 3 * (kPanel<kTile * Tall> + kPanel<kTile>);
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];  // [buffer][A's parts, B's parts]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = tile_of(p, blockIdx.x);
-  const int m0 = tile.m * kTile * Tall, n0 = tile.n * kTile, slice = blockIdx.y;
+  const auto [tile, slice] = piece_of<BCols>(p);
+  const int m0 = tile.m * kTile * Tall, n0 = tile.n * kTile;
   const Steps<kDepth> steps(p, slice);
   const int count = steps.end - steps.begin;
   const uint32_t lds_a = lds_address(lds), lds_b = lds_a + 3 * kPanel<kTile * Tall>;
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kThreads, 2) void f32_product_kernel(ProductArgs p)
 // unit and one stores while the other loads.  Bound by the stores: dx of 16384 x 4096 into
 // 1 to 32 takes 56 to 63 us (268 MB), in the kernel above 79 to 85.
 template <bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ProductArgs p) {
+__global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
   constexpr int kParked = 8 * 8192;  // 32 x 64 sums of each wavefront
   static_assert(6 * kPanel<kTile> <= kParked, "the parts fit where the sums go");
@@ -284,15 +284,15 @@ __global__ __launch_bounds__(kThreads, 4) void f32_outer_kernel(ProductArgs p) {
 
 }  // namespace
 
-hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream) {
+hipError_t launch_f32_product(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, const LossParts* loss, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(kThreads);
   return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
     if (p.side_m == kTile && p.k <= kDepth && p.slices == 1)
-      f32_outer_kernel<a.value, b.value, f.value><<<dim3(grid.x), block, 0, stream>>>(p);
+      f32_outer_kernel<a.value, b.value, f.value><<<dim3(grid.x), block, 0, stream>>>(args_of<f.value>(p, loss));
     else if (p.side_m == kTile)
-      f32_product_kernel<1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      f32_product_kernel<1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     else
-      f32_product_kernel<2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      f32_product_kernel<2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     return hipGetLastError();
   });
 }

@@ -165,7 +165,7 @@ __device__ __forceinline__ void split_three(const float (&v)[3][8], U32x4 (&w)[3
 
 // LongA: A is the long operand.
 template <typename T, bool LongA, bool LongCols, bool ShortCols, Finish F>
-__global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(256) void narrow_product_kernel(ArgsOf<F> p) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * kRing * kSlot];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -283,11 +283,15 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
       const int m = i / groups, n = i % groups * 8;
       float v[8];
       get(area, m, n, v);
-      finish_some<T, F, groups>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+      RowOf<F> of;
+      of.load(p, (LongA ? first : 0) + m);
+      finish_some<T, F, groups>(p, of, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
     }
   } else {
-    __syncthreads();
     const int m = threadIdx.x / groups, n = threadIdx.x % groups * 8;
+    RowOf<F> of;
+    of.load(p, (LongA ? first : 0) + m);
+    __syncthreads();
     static_assert(groups * down == 256, "one group of results a thread");
     float v[8], w[8];
     get(reinterpret_cast<const float*>(lds), m, n, v);
@@ -297,7 +301,7 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ProductArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    finish_some<T, F, groups>(p, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+    finish_some<T, F, groups>(p, of, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
   }
 }
 
@@ -331,14 +335,14 @@ bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, in
 }
 
 hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
-                                 hipStream_t stream) {
+                                 const LossParts* loss, hipStream_t stream) {
   const bool long_a = p.m > p.n;
   const dim3 grid(static_cast<uint32_t>(long_a ? p.tiles_m : p.tiles_n), static_cast<uint32_t>(p.slices)), block(256);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
-      if (long_a) narrow_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
-      else narrow_product_kernel<T, false, b.value, a.value, f.value><<<grid, block, 0, stream>>>(p);
+      if (long_a) narrow_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
+      else narrow_product_kernel<T, false, b.value, a.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
       return hipGetLastError();
     });
   });

@@ -79,15 +79,15 @@ __device__ __forceinline__ void step(Feeder<ACols, kTile * Tall>& a, Feeder<BCol
 }
 
 template <typename T, int Tall, bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(512, 2) void product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(512, 2) void product_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
   using S = Shape<Tall>;
   constexpr int kRing = S::kRing;
   __shared__ __attribute__((aligned(1024))) char lds[kRing * (S::kA + S::kB)];  // A's ring, B's ring
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = tile_of(p, blockIdx.x);
-  const int m0 = tile.m * S::kRows, n0 = tile.n * kTile, slice = blockIdx.y;
+  const auto [tile, slice] = piece_of<BCols>(p);
+  const int m0 = tile.m * S::kRows, n0 = tile.n * kTile;
   const Steps<kStep> steps(p, slice);
   const int count = steps.end - steps.begin;
   Feeder<ACols, kTile * Tall> a;
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(512, 2) void product_kernel(ProductArgs p) {
 // the other loads.  Bound by the stores: 16384 x 16 x 16384 bf16 (537 MB) takes 124 to
 // 137 us; tiles of 256 x 256 took 157 to 166, the 128 x 128 tiles with a ring 179.
 template <typename T, bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(512, 4) void outer_product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(512, 4) void outer_product_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
   __shared__ __attribute__((aligned(1024))) char lds[8 * 8192];  // A's and B's step, then the results
   const int lane = threadIdx.x & 63;
@@ -207,9 +207,13 @@ __device__ __forceinline__ void add_slices(const float*& from, int64_t size, int
 // 16384 sums take 5.3 us, and took 7.9 with each waited for; 8 of 64 x 4096 take 4.1 and
 // took 5.1.  (Workgroups of one wavefront and of four take the same time.)
 template <typename T, Finish F>
-__global__ __launch_bounds__(256) void join_kernel(ProductArgs p, bool a_cols) {
-  if (a_cols) fit_live<F, true>(p);
-  else fit_live<F, false>(p);
+__global__ __launch_bounds__(256) void join_kernel(ArgsOf<F> p, bool a_cols) {
+  if (a_cols) {
+    fit_live<F, true>(p);
+  } else {
+    (void)fit<F, false>(p);
+    if (p.slices == 1) return;  // the products' workgroups finished
+  }
   const int across = (p.n + 7) / 8, slices = p.slices;
   const int64_t total = static_cast<int64_t>(p.m) * across, size = static_cast<int64_t>(p.m) * p.n;
   p.slices = 1;
@@ -223,29 +227,29 @@ __global__ __launch_bounds__(256) void join_kernel(ProductArgs p, bool a_cols) {
     if (slices & 4) add_slices<4>(from, size, left, sum);
     if (slices & 2) add_slices<2>(from, size, left, sum);
     if (slices & 1) add_slices<1>(from, size, left, sum);
-    finish_some<T, F, 1>(p, 0, row, col, sum);
+    finish_some<T, F, 1>(p, RowOf<F>{}, 0, row, col, sum);
   }
 }
 
 template <typename T>
-hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, hipStream_t stream) {
+hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, const LossParts* loss, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
   return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
     if (p.k <= kStep && p.slices == 1)
-      outer_product_kernel<T, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      outer_product_kernel<T, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     else if (p.side_m == kTile)
-      product_kernel<T, 1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      product_kernel<T, 1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     else
-      product_kernel<T, 2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      product_kernel<T, 2, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     return hipGetLastError();
   });
 }
 
 template <typename T>
-hipError_t join(const ProductArgs& p, bool a_cols, Finish finish, hipStream_t stream) {
+hipError_t join(const ProductArgs& p, bool a_cols, Finish finish, const LossParts* loss, hipStream_t stream) {
   const int64_t groups = static_cast<int64_t>(p.m) * ((p.n + 7) / 8);
   const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((groups + 255) / 256, 4096))), block(256);
-  if (finish == Finish::kSum) join_kernel<T, Finish::kSum><<<grid, block, 0, stream>>>(p, a_cols);
+  if (finish == Finish::kSum) join_kernel<T, Finish::kSum><<<grid, block, 0, stream>>>(args_of<Finish::kSum>(p, loss), a_cols);
   else join_kernel<T, Finish::kLinear><<<grid, block, 0, stream>>>(p, a_cols);
   return hipGetLastError();
 }
@@ -313,19 +317,19 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
 }
 
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
-                          Finish finish) {
+                          Finish finish, const LossParts* loss) {
   hipError_t err;
   if (p.side_n < kTile) {
-    err = launch_narrow_product(p, dtype, a_cols, b_cols, finish, stream);
+    err = launch_narrow_product(p, dtype, a_cols, b_cols, finish, loss, stream);
   } else if (dtype == F32::code) {
-    err = launch_f32_product(p, a_cols, b_cols, finish, stream);
+    err = launch_f32_product(p, a_cols, b_cols, finish, loss, stream);
   } else if (p.side_n == 256) {
-    err = launch_wide_product(p, dtype, a_cols, b_cols, finish, stream);
+    err = launch_wide_product(p, dtype, a_cols, b_cols, finish, loss, stream);
   } else {
-    err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, finish, stream); });
+    err = with_half_type(dtype, [&](auto t) { return run<decltype(t)>(p, a_cols, b_cols, finish, loss, stream); });
   }
-  if (err != hipSuccess || p.slices == 1) return err;
-  return with_type(dtype, [&](auto t) { return join<decltype(t)>(p, a_cols, finish, stream); });
+  if (err != hipSuccess || (p.slices == 1 && (loss == nullptr || loss->groups == 0))) return err;
+  return with_type(dtype, [&](auto t) { return join<decltype(t)>(p, a_cols, finish, loss, stream); });
 }
 
 }  // namespace fh

@@ -87,13 +87,13 @@ __device__ __forceinline__ void step(Feeder<ACols, kSide>& a, Feeder<BCols, kSid
 }
 
 template <typename T, bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(512, 2) void wide_product_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kBuffer];  // A, A, B, B
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = tile_of(p, blockIdx.x);
-  const int m0 = tile.m * kSide, n0 = tile.n * kSide, slice = blockIdx.y;
+  const auto [tile, slice] = piece_of<BCols>(p);
+  const int m0 = tile.m * kSide, n0 = tile.n * kSide;
   const Steps<kStep> steps(p, slice);
   const int count = steps.end - steps.begin;
   Feeder<ACols, kSide> a;
@@ -157,11 +157,11 @@ __global__ __launch_bounds__(512, 2) void wide_product_kernel(ProductArgs p) {
 }  // namespace
 
 hipError_t launch_wide_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish,
-                               hipStream_t stream) {
+                               const LossParts* loss, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
   return with_half_type(dtype, [&](auto t) {
     return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
-      wide_product_kernel<decltype(t), a.value, b.value, f.value><<<grid, block, 0, stream>>>(p);
+      wide_product_kernel<decltype(t), a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
       return hipGetLastError();
     });
   });
