@@ -401,6 +401,124 @@ __global__ __launch_bounds__(64 * kJoining) void join_runs_kernel(SumArgs p) {
   put<T>(p, sum, key, c);
 }
 
+// ---- few tokens ------------------------------------------------------------------------
+
+constexpr int kFew = 2048, kRows = 64, kLong = 32;
+
+// A wavefront's tokens in a block of rows: place and row of each, in their order.
+struct Found {
+  const uint32_t* list;
+  int count;
+};
+
+// Adds the gradients of the tokens that are row `r`.
+template <typename T>
+__device__ __forceinline__ void add_found(const EmbeddingArgs& a, const Found& found, uint32_t r, int c,
+                                          float (&sum)[kVec<T>]) {
+  using S = typename T::storage;
+  constexpr int V = kVec<T>, kAhead = 8;
+  const int lane = threadIdx.x & 63, cols = static_cast<int>(a.cols);
+  for (int base = 0; base < found.count; base += 64) {
+    const uint32_t entry = base + lane < found.count ? found.list[base + lane] : ~0u;
+    uint64_t left = __ballot(entry >> 16 == r);
+    int stream = 0;
+    while (left != 0) {
+      U32x4 raw[kAhead];
+      int loaded = 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (left == 0) break;
+        const int at = __builtin_amdgcn_readlane(entry, __ffsll(static_cast<unsigned long long>(left)) - 1) & 0xFFFF;
+        raw[u] = load_row<T>(static_cast<const S*>(a.grad) + (static_cast<int64_t>(at) * a.streams + stream) * a.g_stride,
+                             c, cols);
+        ++loaded;
+        if (++stream == a.streams) {
+          stream = 0;
+          left &= left - 1;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (u >= loaded) break;
+        float f[V];
+        to_floats<T>(raw[u], f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum[k] += f[k];
+      }
+    }
+  }
+}
+
+// The gradient of up to 64 rows, 2^shift apart, and a strip of columns, for up to 2048 tokens: every
+// workgroup looks through them for its rows' itself, in one launch where sorting takes two more.  (The
+// frequent words of a vocabulary in the order of their frequency are neighbours: 64 rows in a row left
+// most of the work to one workgroup, 90 us.)  A wavefront to a row, all four to one that occurs often.
+template <typename T>
+__global__ __launch_bounds__(256) void few_kernel(EmbeddingArgs a, int strips, int shift) {
+  constexpr int V = kVec<T>;
+  __shared__ uint32_t list[4][kFew / 4], often[kRows], counts[4];
+  __shared__ float area[4][V][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t first = blockIdx.x / strips, apart = 1u << shift;
+  const int c = (static_cast<int>(blockIdx.x % strips) * 64 + lane) * V, cols = static_cast<int>(a.cols);
+  if (threadIdx.x < kRows) often[threadIdx.x] = 0;
+  __syncthreads();
+  const int begin = static_cast<int>(a.count * wave / 4), end = static_cast<int>(a.count * (wave + 1) / 4);
+  constexpr int kTurns = kFew / 4 / 64;
+  uint32_t keys[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int at = begin + 64 * i + lane;
+    keys[i] = at < end ? key_of(a, at) : static_cast<uint32_t>(a.vocab);
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const uint32_t row = keys[i] >> shift;
+    const bool mine = keys[i] < a.vocab && (keys[i] & (apart - 1)) == first;
+    const uint64_t those = __ballot(mine);
+    if (mine) {
+      list[wave][count + lanes_below(those)] = row << 16 | static_cast<uint32_t>(begin + 64 * i + lane);
+      atomicAdd(often + row, 1u);
+    }
+    count += __popcll(those);
+  }
+  if (lane == 0) counts[wave] = count;
+  __syncthreads();
+  using S = typename T::storage;
+  const int rows = static_cast<int>((a.vocab - first + apart - 1) >> shift);
+  const auto write = [&](int r, float (&sum)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] *= a.scale;
+    store_row<T>(from_floats<T>(sum), static_cast<S*>(a.out) + (first + (static_cast<int64_t>(r) << shift)) * a.cols,
+                 c, cols);
+  };
+  const uint32_t times = often[lane];
+  const uint64_t here = __ballot(times != 0), many = __ballot(times >= kLong);
+  for (int r = wave; r < rows; r += 4) {
+    if (many >> r & 1) continue;
+    float sum[V] = {};
+    if (here >> r & 1) {
+      for (int w = 0; w < 4; ++w) add_found<T>(a, {list[w], static_cast<int>(counts[w])}, r, c, sum);
+    }
+    write(r, sum);
+  }
+  for (uint64_t left = many; left != 0; left &= left - 1) {
+    const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
+    float sum[V] = {};
+    add_found<T>(a, {list[wave], count}, r, c, sum);
+#pragma unroll
+    for (int k = 0; k < V; ++k) area[wave][k][lane] = sum[k];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] = ((area[0][k][lane] + area[1][k][lane]) + area[2][k][lane]) + area[3][k][lane];
+      write(r, sum);
+    }
+    __syncthreads();
+  }
+}
+
 dim3 blocks_of(int64_t items, int64_t each) { return dim3(static_cast<uint32_t>((items + each - 1) / each)); }
 
 // The keys in `keys` and `order` afterwards, through another pair.
@@ -411,8 +529,7 @@ hipError_t sort_tokens(const EmbeddingArgs& a, Workspace& ws, uint32_t*& keys, i
   while (a.vocab >> bits != 0) ++bits;  // of the vocabulary's size, the last key
   if (a.count <= kMostAlone) {
     if (ws.dry()) return hipSuccess;
-    if (a.count <= kThreads) sort_tile_kernel<1><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
-    else sort_tile_kernel<4><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
+    sort_tile_kernel<4><<<dim3(1), dim3(kThreads), 0, stream>>>(a, bits, keys, order);
     return hipGetLastError();
   }
   auto* other_keys = ws.take<uint32_t>(a.count);
@@ -455,6 +572,19 @@ hipError_t launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t strea
 
 hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* workspace, int64_t* bytes,
                                      hipStream_t stream) {
+  const int64_t strip = 64 * (dtype == F32::code ? 4 : 8), strips = (a.cols + strip - 1) / strip;
+  int shift = 0;
+  while ((int64_t{kRows} << shift) < a.vocab) ++shift;
+  const int64_t few = std::min<int64_t>(int64_t{1} << shift, a.vocab) * strips;
+  if (a.count <= kFew && few <= most_groups(256)) {
+    if (bytes != nullptr) *bytes = 0;
+    if (workspace == nullptr) return hipSuccess;
+    return with_type(dtype, [&](auto t) {
+      few_kernel<decltype(t)>
+          <<<dim3(static_cast<uint32_t>(few)), dim3(256), 0, stream>>>(a, static_cast<int>(strips), shift);
+      return hipGetLastError();
+    });
+  }
   Workspace ws(workspace);
   SumArgs p{};
   p.a = a;
@@ -464,8 +594,7 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* wo
   if (err != hipSuccess) return err;
   p.keys = keys;
   p.order = order;
-  const int64_t strip = 64 * (dtype == F32::code ? 4 : 8);
-  p.strips = static_cast<int>((a.cols + strip - 1) / strip);
+  p.strips = static_cast<int>(strips);
   // Chunks for about eight wavefronts a compute unit, of 16 to 64 places.
   p.chunk = 64;
   while (p.chunk > 16 && a.count / p.chunk * p.strips < 8 * compute_units()) p.chunk /= 2;
