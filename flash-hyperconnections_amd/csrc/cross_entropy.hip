@@ -15,6 +15,12 @@
 // whose rows the piece completes.  The logits' second product is what not keeping them
 // costs: 8 operations a weight and row where 6 would do.
 //
+// Ahead: where all f_i will be the same number the gradients are formed with the loss, but
+// for that number, in 6.  The rows go in chunks.  A chunk's logits leave their product as
+// exponentials beside the maximum of their 64; once all of the chunk's rows have their lse,
+// slope_kernel turns these into dz, which is multiplied into dx and a running FP32 sum of dW.
+// FP32 sums are what stays for the backward, which scales and rounds them.
+//
 // In FP16 dz is held times a power of two that puts the largest |f_i| between 2^14 and 2^15:
 // probabilities down to 2^-39 of the largest factor stay above zero then.  The results' last
 // step divides by it, exactly.  The other types have the range without.
@@ -158,6 +164,99 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(const int64_t* targets, 
   for (int c = (threadIdx.x & 63) * kVec<T>; c < cols; c += 64 * kVec<T>) store_row<T>(U32x4{0, 0, 0, 0}, to, c, cols);
 }
 
+struct SlopeArgs {
+  void* dz;             // [rows, ld]: exponentials, and then the gradients
+  int64_t ld;
+  const float2* stats;  // [groups, stats_ld]
+  int64_t stats_ld;
+  const float *lse, *chosen;
+  const int *live, *label;
+  int row0, rows;
+};
+
+// exp(z - lse) - [target] from exp(z - maximum of its 64): 64 vectors of 64 rows a workgroup, a
+// wavefront to every fourth row.  The target's is formed from its logit, in FP32: 1 - p would
+// show the exponential's rounding where p is close to one.  Bound by memory.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
+  using S = typename T::storage;
+  using Z = Saved<T>;
+  constexpr int V = kVec<T>, kAhead = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (static_cast<int>(blockIdx.x) * 64 + lane) * V;
+  const int more = *a.live - a.row0, rows = more < a.rows ? more : a.rows;
+  if (c >= a.ld) return;
+  const float2* stats = a.stats + static_cast<int64_t>(c / 64) * a.stats_ld;
+  const int last = static_cast<int>(blockIdx.y) * 64 + 64 < rows ? static_cast<int>(blockIdx.y) * 64 + 64 : rows;
+  for (int first = blockIdx.y * 64 + wave; first < last; first += 4 * kAhead) {
+    U32x4 raw[kAhead];
+    float top[kAhead], lse[kAhead], chosen[kAhead];
+    int label[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int r = first + 4 * u < last ? first + 4 * u : first;
+      __builtin_memcpy(&raw[u], static_cast<const S*>(a.dz) + r * a.ld + c, 16);
+      top[u] = stats[r].x;
+      lse[u] = a.lse[r];
+      label[u] = a.label[r];
+      chosen[u] = a.chosen[r];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (first + 4 * u >= last) break;
+      float f[V];
+      to_floats<Z>(raw[u], f);
+      // A target out of range makes its row NaN.
+      const float times = (label[u] < 0 ? __builtin_nanf("") : expf(top[u] - lse[u])) *
+                          (T::code == BF16::code ? 1.f / kKept : 1.f);  // FP16 and FP32 keep their scales
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] *= times;
+      const int at = label[u] - c;
+      if (at >= 0 && at < V) {
+        const float hit = (expf(chosen[u] - lse[u]) - 1.f) * (T::code == F16::code ? kKept : 1.f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = k == at ? hit : f[k];
+      }
+      const U32x4 w = from_floats<T>(f);
+      __builtin_memcpy(static_cast<S*>(a.dz) + (first + 4 * u) * a.ld + c, &w, 16);
+    }
+  }
+}
+
+// out = sums times grad, over how many rows have a target for a mean (nothing where none has): a
+// wavefront to a row, or to every gridDim.y-th 512 columns of it.  With an index the first `live`
+// rows, row k into row index[k].
+struct ScaleArgs {
+  const float* sums;
+  const int *live, *index;
+  const float* grad;
+  int mean;
+  float factor;
+  int64_t rows;
+  int cols;
+  void* out;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void scale_kernel(ScaleArgs a) {
+  constexpr int V = 8;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= (a.index != nullptr ? *a.live : a.rows)) return;
+  const int live = *a.live;
+  const float times = live == 0 ? 0.f : *a.grad / (a.mean ? static_cast<float>(live) : 1.f);
+  const float* from = a.sums + row * a.cols;
+  auto* to = static_cast<typename T::storage*>(a.out) + (a.index != nullptr ? a.index[row] : row) * a.cols;
+  for (int c = (blockIdx.y * 64 + (threadIdx.x & 63)) * V; c < a.cols; c += gridDim.y * 64 * V) {
+    float f[V];
+    load_some(from + c, a.cols - c, f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = f[k] * a.factor * times;
+    typename T::storage e[V];
+    if constexpr (T::code == F32::code) __builtin_memcpy(e, f, sizeof(e));
+    else round_some<T>(f, e);
+    store_some(e, to + c, a.cols - c);
+  }
+}
+
 struct LseArgs {
   const float2* stats;  // [groups, ld]
   int64_t ld;
@@ -245,15 +344,27 @@ __global__ __launch_bounds__(256) void bias_kernel(const void* dz, int64_t ld, i
           ((area[0][i][lane] + area[1][i][lane]) + area[2][i][lane]) + area[3][i][lane];
 }
 
-// db from `count` partial sums.
+// db from `count` partial sums; `scale` may be null.
 template <typename T>
 __global__ __launch_bounds__(256) void join_bias_kernel(const float* partial, int count, int cols, const float* scale,
                                                         void* out) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   float sum = 0.f;
+#pragma unroll 8
   for (int i = 0; i < count; ++i) sum += partial[static_cast<int64_t>(i) * cols + c];
-  static_cast<typename T::storage*>(out)[c] = from_f32<T>(sum * *scale);
+  static_cast<typename T::storage*>(out)[c] = from_f32<T>(scale != nullptr ? sum * *scale : sum);
+}
+
+hipError_t launch_bias(const Laid& dz, int64_t cols, int64_t rows, const int* live, int64_t row0, int down,
+                       float* partial, int dtype, hipStream_t stream) {
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid(static_cast<uint32_t>((cols + 64 * kVec<T> - 1) / (64 * kVec<T>)), static_cast<uint32_t>(down));
+    bias_kernel<T><<<grid, dim3(256), 0, stream>>>(dz.data, dz.ld, static_cast<int>(cols), static_cast<int>(rows), live,
+                                                   static_cast<int>(row0), partial);
+    return hipGetLastError();
+  });
 }
 
 int element(int dtype) { return dtype == F32::code ? 4 : 2; }
@@ -276,8 +387,8 @@ hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, Workspace& ws, R
   r.ignore = a.ignore;
   r.rows = static_cast<int>(a.rows);
   r.vocab = static_cast<int>(a.vocab);
-  r.live = got.live = ws.take<int>(1);
-  r.index = got.index = ws.take<int>(a.rows);
+  r.live = got.live = a.places != nullptr ? a.places : ws.take<int>(1);
+  r.index = got.index = a.places != nullptr ? a.places + 1 : ws.take<int>(a.rows);
   r.label = got.label = ws.take<int>(a.rows);
   GatherArgs g{a.x, a.x_stride, got.live, got.index, ws.take<char>(a.rows * ld * element(a.dtype)), ld,
                static_cast<int>(a.cols)};
@@ -328,6 +439,13 @@ LossProductArgs logits(const LossArgs& a, const Rows& rows, int64_t row0, int64_
 
 Laid rows_from(const Laid& a, int64_t row, int dtype) { return {bytes_on(a.data, row * a.ld * element(dtype)), a.ld}; }
 
+// Rows of a workgroup that joins their statistics, a power of two.
+int lse_rows(int64_t rows) {
+  int across = 64;
+  while (across > rows || (across > 4 && rows / across < compute_units())) across >>= 1;
+  return across;
+}
+
 constexpr int64_t kStats = int64_t{1} << 25;  // maxima and sums at a time: 256 MB
 constexpr int64_t kPiece = int64_t{1} << 30;  // bytes of dz at a time
 
@@ -348,13 +466,12 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
   auto* stats = ws.take<float2>(groups * most);
   auto* chosen = ws.take<float>(most);
   float* losses = by_row ? a.loss : ws.take<float>(a.rows);
-  int across = 64;  // rows of a workgroup that joins them
-  while (across > a.rows || (across > 4 && a.rows / across < compute_units())) across >>= 1;
+  const int across = lse_rows(a.rows);
   if (err == hipSuccess) {
     err = in_slices(a.rows, most, [&](int64_t row0, int64_t count) {
       LossProductArgs p = logits(a, rows, row0, count, 0, a.vocab);
       p.loss.stats = stats;
-      p.loss.ld = most;
+      p.loss.stats_ld = most;
       p.loss.chosen = chosen;
       const hipError_t e = multiply(p, rows_from(rows.x, row0, a.dtype), w, a.dtype, false, false, Finish::kStats, ws, stream);
       if (e != hipSuccess || ws.dry()) return e;
@@ -369,6 +486,124 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
     err = hipGetLastError();
   }
   if (bytes != nullptr) *bytes = ws.used();
+  return err;
+}
+
+hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
+  Workspace ws(workspace);
+  Rows rows;
+  hipError_t err = gather(a, RowsArgs{}, false, ws, rows, stream);
+  Laid w;
+  if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
+  if (err != hipSuccess) return err;
+  const int64_t groups = (a.vocab + 63) / 64, ld = (a.vocab + 7) / 8 * 8;
+  const int64_t most = std::min<int64_t>(
+      std::min<int64_t>(a.rows, most_product_rows(std::max(a.vocab, a.cols))),
+      std::max<int64_t>(256, std::min<int64_t>(kStats / groups, kPiece / (ld * element(a.dtype))) / 256 * 256));
+  auto* stats = ws.take<float2>(groups * most);
+  auto* chosen = ws.take<float>(most);
+  auto* lse = ws.take<float>(a.rows);
+  auto* losses = ws.take<float>(a.rows);
+  const Laid dz{ws.take<char>(most * ld * element(a.dtype)), ld};
+  const int64_t chunks = (a.rows + most - 1) / most;
+  const int down = static_cast<int>(std::min<int64_t>((most + 15) / 16, 64));
+  auto* partial = a.db_sums != nullptr ? ws.take<float>(chunks * down * a.vocab) : nullptr;
+  const int64_t before = ws.used();
+  int64_t most_used = before;
+  // Products follow one another on the stream, and share the space for what their slices add up to.
+  const auto multiply_next = [&](LossProductArgs& p, const Laid& x, const Laid& y, bool a_cols, bool b_cols, Finish finish) {
+    Workspace part(bytes_on(workspace, before));
+    const hipError_t e = multiply(p, x, y, a.dtype, a_cols, b_cols, finish, part, stream);
+    most_used = std::max(most_used, before + part.used());
+    return e;
+  };
+  err = in_slices(a.rows, most, [&](int64_t row0, int64_t count) {
+    const Laid x = rows_from(rows.x, row0, a.dtype);
+    LossProductArgs p = logits(a, rows, row0, count, 0, a.vocab);
+    p.loss.stats = stats;
+    p.loss.stats_ld = most;
+    p.loss.chosen = chosen;
+    p.loss.ld = ld;
+    p.out = const_cast<void*>(dz.data);
+    hipError_t e = multiply_next(p, x, w, false, false, Finish::kExp);
+    if (e == hipSuccess && !ws.dry()) {
+      const int across = lse_rows(count);
+      const LseArgs l{stats, most, static_cast<int>(groups), static_cast<int>(count), rows.live, static_cast<int>(row0),
+                      rows.label + row0, rows.index + row0, chosen, lse + row0, losses + row0, 0};
+      lse_kernel<<<blocks_of(count, across), dim3(1024), 0, stream>>>(l, across);
+      const SlopeArgs s{const_cast<void*>(dz.data), ld, stats, most, lse + row0, chosen, rows.live, rows.label + row0,
+                        static_cast<int>(row0), static_cast<int>(count)};
+      e = with_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        const dim3 grid(blocks_of(ld, 64 * kVec<T>).x, blocks_of(count, 64).x);
+        slope_kernel<T><<<grid, dim3(256), 0, stream>>>(s);
+        return hipGetLastError();
+      });
+      if (e == hipSuccess && a.db_sums != nullptr)
+        e = launch_bias(dz, a.vocab, count, rows.live, row0, down, partial + row0 / most * down * a.vocab, a.dtype, stream);
+    }
+    LossProductArgs s{};
+    s.loss.live = rows.live;
+    s.loss.row0 = static_cast<int>(row0);
+    s.n = static_cast<int>(a.cols);
+    if (e == hipSuccess && a.dx_sums != nullptr) {
+      LossProductArgs q = s;
+      q.m = static_cast<int>(count);
+      q.k = static_cast<int>(a.vocab);
+      q.loss.sums = a.dx_sums + row0 * a.cols;
+      q.loss.first = 1;
+      e = multiply_next(q, dz, w, false, true, Finish::kSum);
+    }
+    if (e == hipSuccess && a.dw_sums != nullptr) {
+      LossProductArgs q = s;
+      q.m = static_cast<int>(a.vocab);
+      q.k = static_cast<int>(count);
+      q.loss.sums = a.dw_sums;
+      q.loss.first = row0 == 0;
+      e = multiply_next(q, dz, x, true, true, Finish::kSum);
+    }
+    return e;
+  });
+  if (err == hipSuccess && !ws.dry()) {
+    loss_kernel<<<dim3(1), dim3(1024), 0, stream>>>(losses, rows.live, a.reduction == FH_REDUCE_MEAN, a.loss);
+    if (a.db_sums != nullptr)
+      join_bias_kernel<F32><<<blocks_of(a.vocab, 256), dim3(256), 0, stream>>>(
+          partial, static_cast<int>(chunks) * down, static_cast<int>(a.vocab), nullptr, a.db_sums);
+    err = hipGetLastError();
+  }
+  if (bytes != nullptr) *bytes = most_used;
+  return err;
+}
+
+hipError_t launch_cross_entropy_scale(const LossArgs& a, hipStream_t stream) {
+  ScaleArgs s{};
+  s.live = a.places;
+  s.grad = a.grad;
+  s.mean = a.reduction == FH_REDUCE_MEAN;
+  s.factor = a.dtype == F16::code ? 1.f / kKept : 1.f;
+  const auto scale = [&](int64_t rows, int64_t cols, const float* sums, const int* index, void* out, int dtype) {
+    s.rows = rows;
+    s.cols = static_cast<int>(cols);
+    s.sums = sums;
+    s.index = index;
+    s.out = out;
+    return with_type(dtype, [&](auto t) {
+      const int64_t across = rows >= 4 * compute_units() ? 1 : std::min<int64_t>((cols + 511) / 512, 1024);
+      scale_kernel<decltype(t)><<<dim3(blocks_of(rows, 4).x, static_cast<uint32_t>(across)), dim3(256), 0, stream>>>(s);
+      return hipGetLastError();
+    });
+  };
+  hipError_t err = hipSuccess;
+  if (a.dx != nullptr) {
+    err = with_type(a.dtype, [&](auto t) {
+      zero_rows_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(
+          a.targets, a.ignore, a.rows, static_cast<int>(a.cols), a.dx);
+      return hipGetLastError();
+    });
+    if (err == hipSuccess) err = scale(a.rows, a.cols, a.dx_sums, a.places + 1, a.dx, a.dtype);
+  }
+  if (err == hipSuccess && a.dweight != nullptr) err = scale(a.vocab, a.cols, a.dw_sums, nullptr, a.dweight, a.dtype);
+  if (err == hipSuccess && a.dbias != nullptr) err = scale(1, a.vocab, a.db_sums, nullptr, a.dbias, a.bias_dtype);
   return err;
 }
 
@@ -460,16 +695,8 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
             return multiply(p, d, xp, a.dtype, true, true, Finish::kSum, part, stream);
           });
         }
-        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) {
-          e = with_type(a.dtype, [&](auto t) {
-            using T = decltype(t);
-            const dim3 grid(static_cast<uint32_t>((outs + 64 * kVec<T> - 1) / (64 * kVec<T>)), static_cast<uint32_t>(down));
-            bias_kernel<T><<<grid, dim3(256), 0, stream>>>(d.data, d.ld, static_cast<int>(outs), static_cast<int>(count),
-                                                           rows.live, static_cast<int>(row0),
-                                                           db_sums + row0 / most_rows * down * outs);
-            return hipGetLastError();
-          });
-        }
+        if (e == hipSuccess && a.dbias != nullptr && !ws.dry())
+          e = launch_bias(d, outs, count, rows.live, row0, down, db_sums + row0 / most_rows * down * outs, a.dtype, stream);
         return e;
       });
       if (all != hipSuccess || a.dbias == nullptr || ws.dry()) return all;

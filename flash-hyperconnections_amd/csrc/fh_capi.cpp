@@ -268,7 +268,8 @@ int validate_loss(const fh::LossArgs& a) {
   if (a.reduction < FH_REDUCE_NONE || a.reduction > FH_REDUCE_MEAN)
     return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: unknown reduction");
   if (a.rows > 0 && (!rows_ok(a.x, a.x_stride, a.dtype) || !rows_ok(a.weight, a.w_stride, a.dtype) ||
-                     a.targets == nullptr || !aligned(a.targets, 8) || a.lse == nullptr || !aligned(a.lse, 4) ||
+                     a.targets == nullptr || !aligned(a.targets, 8) || !aligned(a.lse, 4) ||
+                     (a.lse == nullptr && a.places == nullptr) ||
                      (a.bias != nullptr && !aligned(a.bias, element_size(a.bias_dtype)))))
     return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
   return FH_OK;
@@ -694,6 +695,62 @@ int fh_linear_cross_entropy_backward(const void* x, int64_t x_stride, const void
   rc = check_workspace("linear_cross_entropy", workspace, workspace_bytes, need, &query);
   if (rc != FH_OK || query) return rc;
   return launched(fh::launch_cross_entropy_backward(a, workspace, nullptr, stream));
+}
+
+int fh_linear_cross_entropy_ahead(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                  const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore,
+                                  int reduction, float* loss, int* places, float* dx_sums, float* dw_sums,
+                                  float* db_sums, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                                  int64_t cols, int64_t vocab, hipStream_t stream) {
+  fh::LossArgs a = loss_args(x, x_stride, weight, weight_stride, bias, bias_dtype, targets, ignore, reduction, nullptr,
+                             dtype, rows, cols, vocab);
+  a.loss = loss;
+  a.places = places;
+  a.dx_sums = dx_sums;
+  a.dw_sums = dw_sums;
+  a.db_sums = db_sums;
+  int rc = validate_loss(a);
+  if (rc != FH_OK) return rc;
+  if (rows == 0) return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: no rows, whose loss is the caller's");
+  if (reduction == FH_REDUCE_NONE)
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: each row's loss has an upstream gradient of its own");
+  if (loss == nullptr || !aligned(loss, 4) || !aligned(places, 4) || !aligned(dx_sums, 4) || !aligned(dw_sums, 4) ||
+      !aligned(db_sums, 4))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
+  int64_t need = 0;
+  bool query = false;
+  (void)fh::launch_cross_entropy_ahead(a, nullptr, &need, stream);
+  rc = check_workspace("linear_cross_entropy", workspace, workspace_bytes, need, &query);
+  if (rc != FH_OK || query) return rc;
+  return launched(fh::launch_cross_entropy_ahead(a, workspace, nullptr, stream));
+}
+
+int fh_linear_cross_entropy_scale(const float* grad, const int64_t* targets, int64_t ignore, int reduction,
+                                  const int* places, const float* dx_sums, const float* dw_sums, const float* db_sums,
+                                  void* dx, void* dweight, void* dbias, int bias_dtype, int dtype, int64_t rows,
+                                  int64_t cols, int64_t vocab, hipStream_t stream) {
+  // x and the weight have been read: their place is taken by what is there.
+  fh::LossArgs a = loss_args(grad, 0, grad, 0, nullptr, bias_dtype, targets, ignore, reduction, grad, dtype, rows, cols,
+                             vocab);
+  a.grad = grad;
+  a.places = const_cast<int*>(places);
+  a.dx_sums = const_cast<float*>(dx_sums);
+  a.dw_sums = const_cast<float*>(dw_sums);
+  a.db_sums = const_cast<float*>(db_sums);
+  a.dx = dx;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  const int rc = validate_loss(a);
+  if (rc != FH_OK) return rc;
+  if (rows == 0 || reduction == FH_REDUCE_NONE)
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: no rows, or an upstream gradient for each");
+  const auto sums_ok = [](const float* sums, const void* out, int type) {
+    return out == nullptr || (sums != nullptr && aligned(sums, 4) && aligned(out, element_size(type)));
+  };
+  if (places == nullptr || !aligned(places, 4) || !sums_ok(dx_sums, dx, dtype) || !sums_ok(dw_sums, dweight, dtype) ||
+      !sums_ok(db_sums, dbias, bias_dtype))
+    return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
+  return launched(fh::launch_cross_entropy_scale(a, stream));
 }
 
 const char* fh_last_error(void) { return g_error.c_str(); }

@@ -133,10 +133,17 @@ struct LossArgs {
   float* lse;             // [rows], for the backward
   const float* grad;      // backward: one, or [rows]
   void *dx, *dweight, *dbias;  // contiguous; each may be null
+  // Ahead: [1 + rows] how many rows have a target and which; the gradients for an upstream gradient of one,
+  // [of these rows, cols], [vocab, cols] and [vocab], each of which may be null.
+  int* places;
+  float *dx_sums, *dw_sums, *db_sums;
   int64_t rows, cols, vocab;
 };
 // As launch_linear and launch_linear_backward.
 hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
 hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
+// The loss, a sum or a mean, and the sums; and the gradients from these.
+hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream);
+hipError_t launch_cross_entropy_scale(const LossArgs& a, hipStream_t stream);
 
 }  // namespace fh

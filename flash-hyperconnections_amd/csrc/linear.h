@@ -14,21 +14,23 @@ namespace fh {
 typedef float Floats4 __attribute__((ext_vector_type(4)));
 
 // What becomes of a product's results: the linear layer's epilogue; the softmax
-// statistics of logits, which are not kept; the logits' gradients; or a sum that goes on
-// from another product's and is scaled at its end.
-enum class Finish { kLinear, kStats, kSlope, kSum };
+// statistics of logits, which are not kept; these and the logits' exponentials; the logits'
+// gradients; or a sum that goes on from another product's and is scaled at its end.
+enum class Finish { kLinear, kStats, kExp, kSlope, kSum };
+constexpr bool whole_sums(Finish f) { return f == Finish::kStats || f == Finish::kExp || f == Finish::kSlope; }
 
-// What the last three need beside the product.  Their rows are the first *live ones from
+// What the others need beside the product.  Their rows are the first *live ones from
 // row0 on (of the sum where A is in columns), as many as there are targets.
 struct LossParts {
   const int* live;
   int row0;
   const int* label;      // [rows] targets, negative where out of range
   int col0;              // the vocabulary's entry of column 0
-  float2* stats;         // kStats: [columns / 64, rows] maximum and sum of exponentials, groups ld apart
-  float* chosen;         // kStats: [rows] logits of the targets
+  float2* stats;         // kStats, kExp: [columns / 64, rows] maximum and sum of exponentials, groups stats_ld apart
+  int64_t stats_ld;
+  float* chosen;         // kStats, kExp: [rows] logits of the targets
   const float2* row;     // kSlope: [rows] the logarithm of the row's sum, and the factor of its gradient
-  int64_t ld;            // kStats: groups; kSlope: rows of out, whole vectors, zero past n
+  int64_t ld;            // kExp, kSlope: rows of out, whole vectors, zero past n
   float* sums;           // kSum: [m, n] of the sum so far
   int first, last;       // kSum: whether sums is not read, or not written but scaled into out
   const float* scale;    // kSum
@@ -99,6 +101,7 @@ __device__ __forceinline__ bool fit(ArgsOf<F>& p) {
     return blockIdx.x + gridDim.x * blockIdx.y < static_cast<uint32_t>(tiles * p.slices);
   } else {
     fit_live<F, ACols>(p);
+    if constexpr (F == Finish::kSum) return p.k > 0 || p.loss.first || p.loss.last;  // or nothing is added
     return true;
   }
 }
@@ -304,6 +307,8 @@ struct RowOf<Finish::kStats> {
   __device__ __forceinline__ void load(const LossProductArgs& p, int i) { label = i < p.m ? p.loss.label[i] - p.loss.col0 : 0; }
 };
 template <>
+struct RowOf<Finish::kExp> : RowOf<Finish::kStats> {};
+template <>
 struct RowOf<Finish::kSlope> {
   int label;
   float2 row;
@@ -322,11 +327,16 @@ __device__ __forceinline__ float exp_from(float v, float from) {
   return __builtin_amdgcn_exp2f((v - from) * kLog2e);
 }
 
+// Exponentials are kept in FP16 beside 16-bit operands, times 2^15: they lie in 0 .. 1, keep 11
+// bits down to 2^-29 and are zero below 2^-40, where bf16 would keep 8.
+constexpr float kKept = 32768.f;
+
 // Logits of Lanes V neighbouring columns of row i, V a lane: their maximum m and the sum
-// of exp(z - m), as far as columns are valid, and the target's logit.  -inf alone gives
-// m = -inf and a sum of zero; a NaN or +inf makes the sum NaN.
-template <typename T, int Lanes, int V>
-__device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf<Finish::kStats>& of, int i, int j,
+// of exp(z - m), as far as columns are valid, and the target's logit; for kExp the
+// exponentials too.  -inf alone gives m = -inf and a sum of zero; a NaN or +inf makes the sum
+// NaN.
+template <typename T, Finish F, int Lanes, int V>
+__device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf<F>& of, int i, int j,
                                            float (&v)[V]) {
   if (i >= p.m) return;  // the same in all of these lanes
   const int left = p.n - j;
@@ -341,17 +351,28 @@ __device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf
   for (int k = 1; k < V; ++k) m = __builtin_fmaxf(m, v[k]);
   m = over_lanes<Lanes>(m, [](float a, float b) { return __builtin_fmaxf(a, b); });
   const float from = m == none ? 0.f : m;
-  float s = 0.f;
-#pragma unroll
-  for (int k = 0; k < V; ++k) s += exp_from<T>(v[k], from);
   const int at = of.label - j;
   if (at >= 0 && at < V && at < left) {
 #pragma unroll
     for (int k = 0; k < V; ++k)
       if (k == at) p.loss.chosen[i] = v[k];
   }
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    v[k] = exp_from<T>(v[k], from);
+    s += v[k];
+  }
+  if (F == Finish::kExp && j < p.loss.ld) {
+    using Z = Saved<T>;
+    typename Z::storage e[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= T::code == F32::code ? 1.f : kKept;
+    round_some<Z>(v, e);
+    store_some(e, static_cast<typename Z::storage*>(p.out) + static_cast<int64_t>(i) * p.loss.ld + j, V);
+  }
   s = over_lanes<Lanes>(s, [](float a, float b) { return a + b; });
-  if (j % 64 == 0 && left > 0) p.loss.stats[static_cast<int64_t>(j / 64) * p.loss.ld + i] = make_float2(m, s);
+  if (j % 64 == 0 && left > 0) p.loss.stats[static_cast<int64_t>(j / 64) * p.loss.stats_ld + i] = make_float2(m, s);
 }
 
 // Logits on their way to the gradients of z: (exp(z - lse) - [target]) times the row's
@@ -414,8 +435,8 @@ __device__ __forceinline__ void finish_some(const ArgsOf<F>& p, const RowOf<F>& 
                                             float (&v)[V]) {
   using S = typename T::storage;
   using Z = Saved<T>;
-  if constexpr (F == Finish::kStats) {
-    stats_some<T, Lanes>(p, of, i, j, v);
+  if constexpr (F == Finish::kStats || F == Finish::kExp) {
+    stats_some<T, F, Lanes>(p, of, i, j, v);
     return;
   } else if constexpr (F == Finish::kSlope) {
     slope_some<T>(p, of, i, j, v);
@@ -485,7 +506,7 @@ __device__ __forceinline__ void finish_parked(const ArgsOf<F>& p, int slice, con
       finish_some<T, F, 8>(p, of[it], slice, row + r, col + 8 * (lane & 7), v);
     }
   };
-  if constexpr (F == Finish::kStats || F == Finish::kSlope) {
+  if constexpr (whole_sums(F)) {
 #pragma unroll
     for (int it = 0; it < turns; ++it) turn(it);
   } else {
@@ -576,7 +597,7 @@ __device__ __forceinline__ void wait_loads() {
 constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16-bit tile within 2^31 bytes
 
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
-// floats.  `dtype` is the operands' and the output's; Finish::kStats and kSlope need whole
+// floats.  `dtype` is the operands' and the output's; some finishes need whole
 // sums, in one slice.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
@@ -604,6 +625,7 @@ hipError_t with_layout(bool a_cols, bool b_cols, Finish finish, Call call) {
   if (!a_cols && !b_cols) {
     if (finish == Finish::kLinear) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kLinear>{});
     if (finish == Finish::kStats) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kStats>{});
+    if (finish == Finish::kExp) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kExp>{});
     if (finish == Finish::kSlope) return call(Flag<false>{}, Flag<false>{}, FinishType<Finish::kSlope>{});
   } else if (b_cols) {
     if (finish == Finish::kLinear && !a_cols) return call(Flag<false>{}, Flag<true>{}, FinishType<Finish::kLinear>{});

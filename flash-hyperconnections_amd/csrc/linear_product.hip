@@ -209,7 +209,7 @@ __device__ __forceinline__ void add_slices(const float*& from, int64_t size, int
 template <typename T, Finish F>
 __global__ __launch_bounds__(256) void join_kernel(ArgsOf<F> p, bool a_cols) {
   if (a_cols) {
-    fit_live<F, true>(p);
+    if (!fit<F, true>(p)) return;
   } else {
     (void)fit<F, false>(p);
     if (p.slices == 1) return;  // the products' workgroups finished
@@ -265,7 +265,7 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
-  const int most = finish == Finish::kStats || finish == Finish::kSlope ? 1 : 16;
+  const int most = whole_sums(finish) ? 1 : 16;
   if (plan_narrow_product(p, dtype, a_cols, b_cols, most)) return;
   if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);

@@ -156,6 +156,73 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> loss_backward_hip(const at::Tenso
   return {dx, dw, db};
 }
 
+// Whether a step forms the gradients with the loss, for the upstream gradient to scale: one product of
+// four fewer, for FP32 sums of the weight's size.  On a step of 4096 x 32768 the two ways cross between 512
+// and 1024 rows (16 bits), and between 128 and 256 (FP32).
+bool ahead_of(const at::Tensor& x, int64_t reduction) {
+  return reduction != FH_REDUCE_NONE && x.sym_numel() >= x.sym_size(-1) * (x.scalar_type() == at::kFloat ? 256 : 1024);
+}
+
+// (loss, places, sums of dx, dweight and dbias), the last three empty where not wanted.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> loss_ahead_hip(
+    const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, const OptTensor& bias, int64_t ignore,
+    int64_t reduction, bool want_x, bool want_weight, bool want_bias) {
+  check_loss(x, weight, targets, bias, reduction);
+  const int64_t cols = x.size(-1), vocab = weight.size(0), rows = x.numel() / cols;
+  TORCH_CHECK(reduction != FH_REDUCE_NONE && rows > 0, "linear_cross_entropy: expected a sum or mean over some rows");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  const auto floats = x.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({}, floats), places = at::empty({rows + 1}, x.options().dtype(at::kInt));
+  at::Tensor dx = want_x ? at::empty({rows, cols}, floats) : at::empty({0}, floats);
+  at::Tensor dw = want_weight ? at::empty({vocab, cols}, floats) : at::empty({0}, floats);
+  at::Tensor db = want_bias ? at::empty({vocab}, floats) : at::empty({0}, floats);
+  const at::Tensor xr = rows_of(x, cols), w = rows_of(weight, cols), b = vector_of(bias), t = indices_of(targets);
+  with_workspace(x, [&](void* workspace, int64_t* bytes) {
+    return fh_linear_cross_entropy_ahead(
+        xr.const_data_ptr(), stride_of(xr), w.const_data_ptr(), stride_of(w), data_of(b),
+        dtype_code(b.defined() ? b.scalar_type() : x.scalar_type()), t.const_data_ptr<int64_t>(), ignore,
+        static_cast<int>(reduction), loss.mutable_data_ptr<float>(), places.mutable_data_ptr<int>(),
+        want_x ? dx.mutable_data_ptr<float>() : nullptr, want_weight ? dw.mutable_data_ptr<float>() : nullptr,
+        want_bias ? db.mutable_data_ptr<float>() : nullptr, workspace, bytes, dtype_code(x.scalar_type()), rows, cols,
+        vocab, current_stream());
+  });
+  return {loss, places, dx, dw, db};
+}
+
+// (dx, dweight, dbias) from these, empty where their sums are.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> loss_scale_hip(const at::Tensor& grad, const at::Tensor& x,
+                                                              const at::Tensor& weight, const at::Tensor& targets,
+                                                              const OptTensor& bias, const at::Tensor& places,
+                                                              const at::Tensor& dx_sums, const at::Tensor& dw_sums,
+                                                              const at::Tensor& db_sums, int64_t ignore,
+                                                              int64_t reduction) {
+  check_loss(x, weight, targets, bias, reduction);
+  const int64_t cols = x.size(-1), vocab = weight.size(0), rows = x.numel() / cols;
+  TORCH_CHECK(strided_on(grad, x) && grad.scalar_type() == at::kFloat && grad.dim() == 0,
+              "linear_cross_entropy: grad must match the result");
+  const auto matches = [&](const at::Tensor& t, int64_t count, at::ScalarType type) {
+    return strided_on(t, x) && t.scalar_type() == type && t.is_contiguous() && (t.numel() == 0 || t.numel() == count);
+  };
+  TORCH_CHECK(matches(places, rows + 1, at::kInt) && places.numel() > 0 && matches(dx_sums, rows * cols, at::kFloat) &&
+                  matches(dw_sums, vocab * cols, at::kFloat) && matches(db_sums, vocab, at::kFloat),
+              "linear_cross_entropy: expected the forward's sums");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  const at::ScalarType bias_type = bias.has_value() ? bias->scalar_type() : x.scalar_type();
+  const auto make = [&](const at::Tensor& sums, at::IntArrayRef sizes, at::ScalarType type) {
+    return at::empty(sums.numel() > 0 ? sizes : at::IntArrayRef{0}, x.options().dtype(type));
+  };
+  at::Tensor dx = make(dx_sums, x.sizes(), x.scalar_type()), dw = make(dw_sums, weight.sizes(), x.scalar_type()),
+             db = make(db_sums, {vocab}, bias_type);
+  const auto floats = [](const at::Tensor& t) { return t.numel() > 0 ? t.const_data_ptr<float>() : nullptr; };
+  const auto out = [](at::Tensor& t) { return t.numel() > 0 ? t.mutable_data_ptr() : nullptr; };
+  const at::Tensor t = indices_of(targets), g = grad.resolve_neg();
+  check_status(fh_linear_cross_entropy_scale(
+      g.const_data_ptr<float>(), t.const_data_ptr<int64_t>(), ignore, static_cast<int>(reduction),
+      places.const_data_ptr<int>(), floats(dx_sums), floats(dw_sums), floats(db_sums), out(dx), out(dw), out(db),
+      dtype_code(bias_type), dtype_code(x.scalar_type()), rows, cols, vocab, current_stream()));
+  return {dx, dw, db};
+}
+
 // ---- autograd -----------------------------------------------------------------------
 
 class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
@@ -166,7 +233,7 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
         "flash_hypercons::_embedding");
     at::AutoDispatchBelowADInplaceOrView below;
     ctx->save_for_backward({tokens});
-    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["vocab"] = weight.sym_size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["streams"] = streams;
     ctx->saved_data["padding"] = padding;
@@ -176,22 +243,22 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
     const at::Tensor tokens = ctx->get_saved_variables()[0], &grad = grads[0];
-    const int64_t vocab = ctx->saved_data["vocab"].toInt(), streams = ctx->saved_data["streams"].toInt(),
-                  padding = ctx->saved_data["padding"].toInt();
+    const c10::SymInt vocab = ctx->saved_data["vocab"].toSymInt();
+    const int64_t streams = ctx->saved_data["streams"].toInt(), padding = ctx->saved_data["padding"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     if (at::GradMode::is_enabled()) {
       // From differentiable pieces, for a backward that builds a graph.
-      const int64_t cols = grad.size(-1);
+      const int64_t rows = vocab.expect_int(), cols = grad.size(-1);
       at::Tensor g = grad.to(at::kFloat);
       if (streams > 0) g = g.sum(-2);
       const at::Tensor t = tokens.reshape({-1}).to(at::kLong);
-      const at::Tensor valid = (t >= 0).logical_and(t < vocab).logical_and(t != padding);
+      const at::Tensor valid = (t >= 0).logical_and(t < rows).logical_and(t != padding);
       g = at::where(valid.unsqueeze(1), g.reshape({-1, cols}) * scale, at::zeros({}, g.options()));
-      const at::Tensor dw = at::zeros({vocab, cols}, g.options()).index_add(0, at::where(valid, t, at::zeros_like(t)), g);
+      const at::Tensor dw = at::zeros({rows, cols}, g.options()).index_add(0, at::where(valid, t, at::zeros_like(t)), g);
       return {{}, dw.to(grad.scalar_type()), {}, {}, {}};
     }
     static const auto op =
-        find_op<at::Tensor(const at::Tensor&, const at::Tensor&, int64_t, double, int64_t, int64_t)>(
+        find_op<at::Tensor(const at::Tensor&, const at::Tensor&, c10::SymInt, double, int64_t, int64_t)>(
             "flash_hypercons::_embedding_backward");
     return {{}, op.call(grad, tokens, vocab, scale, streams, padding), {}, {}, {}};
   }
@@ -231,35 +298,54 @@ class LossFunction : public torch::autograd::Function<LossFunction> {
  public:
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
                             const at::Tensor& targets, const OptTensor& bias, int64_t ignore, int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    const int64_t want = wanted(x, weight, targets, bias);
+    ctx->saved_data["wanted"] = want;
+    if (ahead_of(x, reduction)) {
+      static const auto op = find_op<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>(
+          const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&, int64_t, int64_t, bool, bool, bool)>(
+          "flash_hypercons::_linear_cross_entropy_ahead");
+      auto [loss, places, dx, dw, db] =
+          op.call(x, weight, targets, bias, ignore, reduction, want & 1, want & 2, want & 8);
+      ctx->save_for_backward({x, weight, targets, bias.value_or(at::Tensor()), places, dx, dw, db});
+      return loss;
+    }
     static const auto op =
         find_op<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&,
                                                    const OptTensor&, int64_t, int64_t)>(
             "flash_hypercons::_linear_cross_entropy_forward");
-    at::AutoDispatchBelowADInplaceOrView below;
     auto [loss, lse] = op.call(x, weight, targets, bias, ignore, reduction);
     ctx->save_for_backward({x, weight, targets, bias.value_or(at::Tensor()), lse});
-    ctx->saved_data["ignore"] = ignore;
-    ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["wanted"] = wanted(x, weight, bias);
     return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}};
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &weight = saved[1], &targets = saved[2], &bias = saved[3], &lse = saved[4];
+    const at::Tensor &x = saved[0], &weight = saved[1], &targets = saved[2], &bias = saved[3];
     const int64_t ignore = ctx->saved_data["ignore"].toInt(), reduction = ctx->saved_data["reduction"].toInt();
     const int64_t want = ctx->saved_data["wanted"].toInt();
-    const bool want_x = want & 1, want_weight = want & 2, want_bias = want & 4;
+    const bool want_x = want & 1, want_weight = want & 2, want_bias = want & 8;
+    at::Tensor dx, dw, db;
     if (at::GradMode::is_enabled()) {
       const variable_list g = loss_gradients(grads[0], x, weight, targets, bias, ignore, reduction);
-      return {want_x ? g[0] : at::Tensor(), want_weight ? g[1] : at::Tensor(), {}, want_bias ? g[2] : at::Tensor(), {}, {}};
+      std::tie(dx, dw, db) = std::make_tuple(g[0], g[1], g[2]);
+    } else if (saved.size() > 5) {
+      static const auto op = find_op<std::tuple<at::Tensor, at::Tensor, at::Tensor>(
+          const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+          const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t)>(
+          "flash_hypercons::_linear_cross_entropy_scale");
+      std::tie(dx, dw, db) = op.call(grads[0], x, weight, targets, optional_of(bias), saved[4], saved[5], saved[6],
+                                     saved[7], ignore, reduction);
+    } else {
+      static const auto op = find_op<std::tuple<at::Tensor, at::Tensor, at::Tensor>(
+          const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+          const at::Tensor&, int64_t, int64_t, bool, bool, bool)>("flash_hypercons::_linear_cross_entropy_backward");
+      std::tie(dx, dw, db) = op.call(grads[0], x, weight, targets, optional_of(bias), saved[4], ignore, reduction,
+                                     want_x, want_weight, want_bias);
     }
-    static const auto op = find_op<std::tuple<at::Tensor, at::Tensor, at::Tensor>(
-        const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&, const at::Tensor&,
-        int64_t, int64_t, bool, bool, bool)>("flash_hypercons::_linear_cross_entropy_backward");
-    auto [dx, dw, db] = op.call(grads[0], x, weight, targets, optional_of(bias), lse, ignore, reduction, want_x,
-                                want_weight, want_bias);
     return {want_x ? dx : at::Tensor(), want_weight ? dw : at::Tensor(), {}, want_bias ? db : at::Tensor(), {}, {}};
   }
 };
@@ -279,16 +365,22 @@ at::Tensor loss_autograd(const at::Tensor& x, const at::Tensor& weight, const at
 
 TORCH_LIBRARY_FRAGMENT(flash_hypercons, m) {
   m.def("_embedding(Tensor tokens, Tensor weight, float scale, int streams, int padding) -> Tensor");
-  m.def("_embedding_backward(Tensor grad, Tensor tokens, int vocab, float scale, int streams, int padding) -> Tensor");
+  m.def("_embedding_backward(Tensor grad, Tensor tokens, SymInt vocab, float scale, int streams, int padding) -> Tensor");
   m.def("_linear_cross_entropy(Tensor x, Tensor weight, Tensor targets, Tensor? bias, int ignore, int reduction) -> "
         "Tensor");
   m.def("_linear_cross_entropy_forward(Tensor x, Tensor weight, Tensor targets, Tensor? bias, int ignore, "
         "int reduction) -> (Tensor, Tensor)");
   m.def("_linear_cross_entropy_backward(Tensor grad, Tensor x, Tensor weight, Tensor targets, Tensor? bias, Tensor lse, "
         "int ignore, int reduction, bool want_x, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)");
+  m.def("_linear_cross_entropy_ahead(Tensor x, Tensor weight, Tensor targets, Tensor? bias, int ignore, int reduction, "
+        "bool want_x, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("_linear_cross_entropy_scale(Tensor grad, Tensor x, Tensor weight, Tensor targets, Tensor? bias, Tensor places, "
+        "Tensor dx_sums, Tensor dw_sums, Tensor db_sums, int ignore, int reduction) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(flash_hypercons, CUDA, m) {
+  m.impl("_linear_cross_entropy_ahead", &flash_hypercons::loss_ahead_hip);
+  m.impl("_linear_cross_entropy_scale", &flash_hypercons::loss_scale_hip);
   m.impl("_embedding", &flash_hypercons::embedding_hip);
   m.impl("_embedding_backward", &flash_hypercons::embedding_backward_hip);
   m.impl("_linear_cross_entropy", &flash_hypercons::loss_hip);

@@ -75,6 +75,24 @@ def _linear_cross_entropy_backward_fake(grad, x, weight, targets, bias, lse, ign
             x.new_empty((weight.shape[0] if want_bias else 0,), dtype=x.dtype if bias is None else bias.dtype))
 
 
+@torch.library.register_fake("flash_hypercons::_linear_cross_entropy_ahead")
+def _linear_cross_entropy_ahead_fake(x, weight, targets, bias, ignore, reduction, want_x, want_weight, want_bias):
+    rows, cols = x.numel() // x.shape[-1], x.shape[-1]
+
+    def sums(want, *shape):
+        return x.new_empty(shape if want else (0,), dtype=torch.float32)
+
+    return (sums(True), x.new_empty((rows + 1,), dtype=torch.int32), sums(want_x, rows, cols),
+            sums(want_weight, weight.shape[0], cols), sums(want_bias, weight.shape[0]))
+
+
+@torch.library.register_fake("flash_hypercons::_linear_cross_entropy_scale")
+def _linear_cross_entropy_scale_fake(grad, x, weight, targets, bias, places, dx_sums, dw_sums, db_sums, ignore,
+                                     reduction):
+    return (x.new_empty(x.shape if dx_sums.numel() else (0,)), x.new_empty(weight.shape if dw_sums.numel() else (0,)),
+            x.new_empty((weight.shape[0] if db_sums.numel() else 0,), dtype=x.dtype if bias is None else bias.dtype))
+
+
 def embedding(
     tokens: torch.Tensor,
     weight: torch.Tensor,
@@ -123,8 +141,10 @@ def linear_cross_entropy(
 ) -> torch.Tensor:
     """The softmax cross entropy of x @ weight.T + bias for x [..., K], weight [V, K] and targets [...].
 
-    bias: [V] of x's type or float32.  The logits are formed in pieces, in float32, and never kept; the
-    backward forms them again.  Losses are float32 (float64 for float64 operands): of each position for
+    bias: [V] of x's type or float32.  The logits are formed in pieces, in float32, and never kept.  Where
+    a gradient is wanted of a sum or mean over 1024 positions or more (256 in float32), the gradients are
+    formed with the loss, as float32 sums that the backward scales by the upstream gradient; otherwise the
+    backward forms the logits again.  Losses are float32 (float64 for float64 operands): of each position for
     reduction "none", else their "sum", or their "mean" over the positions with a target (NaN where there
     is none).  A position whose target is `ignore_index` has a loss and gradients of zero, whatever x holds
     there, and costs next to nothing.  Differentiable in x, weight and bias; the logits' gradients are

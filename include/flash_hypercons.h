@@ -252,6 +252,24 @@ FH_API int fh_linear_cross_entropy_backward(const void* x, int64_t x_stride, con
                                      void* dbias, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
                                      int64_t cols, int64_t vocab, hipStream_t stream);
 
+/* The same loss, a sum or a mean (not FH_REDUCE_NONE), and with it the gradients but for the
+ * upstream gradient, which is one number: with a product fewer than the two calls above make of
+ * the logits, for FP32 sums in their place.  places (int [1 + rows]) receives how many rows
+ * have a target and which; dx_sums (float [rows, cols]), dw_sums (float [vocab, cols]) and
+ * db_sums (float [vocab]) may each be NULL. */
+FH_API int fh_linear_cross_entropy_ahead(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                  const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore,
+                                  int reduction, float* loss, int* places, float* dx_sums, float* dw_sums,
+                                  float* db_sums, void* workspace, int64_t* workspace_bytes, int dtype, int64_t rows,
+                                  int64_t cols, int64_t vocab, hipStream_t stream);
+
+/* The gradients from these for the upstream gradient grad (a float): dx, dweight and dbias
+ * (bias_dtype), each NULL or with its sums. */
+FH_API int fh_linear_cross_entropy_scale(const float* grad, const int64_t* targets, int64_t ignore, int reduction,
+                                  const int* places, const float* dx_sums, const float* dw_sums, const float* db_sums,
+                                  void* dx, void* dweight, void* dbias, int bias_dtype, int dtype, int64_t rows,
+                                  int64_t cols, int64_t vocab, hipStream_t stream);
+
 /* Message of the last failing call on this thread ("" if none). */
 FH_API const char* fh_last_error(void);
 

@@ -205,12 +205,14 @@ def test_second_derivatives_go_native():
 
 @gpu
 def test_compiled_step_matches():
-    t, w, g = _inputs((4, 33), 40, 100, torch.bfloat16, 3)
-    leaf = w.clone().requires_grad_()
-    y = torch.compile(lambda a, b: fh.embedding(a, b, scale=0.5, streams=3), fullgraph=True, backend="aot_eager")(t, leaf)
-    (dw,) = torch.autograd.grad(y, leaf, g)
-    want = _step(t, w, g, scale=0.5, streams=3)
-    assert torch.equal(y, want[0]) and torch.equal(dw, want[1])
+    f = torch.compile(lambda a, b: fh.embedding(a, b, scale=0.5, streams=3), fullgraph=True, backend="aot_eager")
+    for rows, vocab in ((4, 100), (7, 101), (90, 1000)):  # sizes become symbols
+        t, w, g = _inputs((rows, 33), 40, vocab, torch.bfloat16, 3)
+        leaf = w.clone().requires_grad_()
+        y = f(t, leaf)
+        (dw,) = torch.autograd.grad(y, leaf, g)
+        want = _step(t, w, g, scale=0.5, streams=3)
+        assert torch.equal(y, want[0]) and torch.equal(dw, want[1])
 
 
 @gpu

@@ -18,6 +18,10 @@ may count as zero: the hardware's exponential gives none below it, and the matri
 FP32 operand's last bf16 part lies up to 2^-16 below the operand) nor give one out: 2^-125 for each p, dz and
 product.  The results' own storage type adds half an ulp, and half a subnormal step; beyond its range they
 are infinite.
+
+Where the gradients are formed with the loss, 16-bit operands' exponentials beside the maximum of their 64 are
+kept in FP16 times 2^15: off by 2^-11 of themselves and 2^-40, except the target's.  FP16's dz is then kept
+in steps of 2^-40.  Every test below that compares with the formula takes both ways.
 """
 
 import pytest
@@ -37,7 +41,7 @@ def _sum_error(k, dtype):
     return ((2 * k + 16) if dtype == torch.float32 else (k + 8)) * U
 
 
-def _formula(x, w, targets, b, reduction, g, ignore=-100):
+def _formula(x, w, targets, b, reduction, g, ignore=-100, ahead=False):
     """loss, dx, dw, db in 64 bits and their bounds, for targets in range or ignored."""
     dtype, dev = x.dtype, x.device
     k, vocab = x.shape[-1], w.shape[0]
@@ -75,6 +79,8 @@ def _formula(x, w, targets, b, reduction, g, ignore=-100):
         el[s] = torch.where(here[s], (elz + ez.gather(1, at) + 2 * U * (lse - zt).abs()).squeeze(1), 0.0)
         ep = 1.1 * p * (ez + elz + (2 * far + 2 * (top - lse).abs() + 4) * U)
         hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+        if ahead and dtype != torch.float32:
+            ep = ep + (1 - hot) * (2.0**-11 * p * (1 + 1.1 * U) + 2.0**-40 + 2.0**-11 * ep)
         dz = (p - hot) * f[s, None]
         edz = (ep + 2 * U * hot + TINY) * f[s, None].abs() + 2 * U * dz.abs() + TINY * (f[s, None] != 0)
         edz = edz + half_ulp(dtype) * (dz.abs() + edz) + (2.0**-39 * most if dtype == torch.float16 else floor(dtype)) * (f[s, None] != 0)
@@ -104,25 +110,50 @@ def _check(got, want, bound, what):
     assert bool(good.all()), f"{what}: {(off / limit).nan_to_num(9e9).max().item():.2f} times the bound"
 
 
-def _step(x, w, targets, b, reduction, g, **args):
-    leaves = [t.detach().requires_grad_() if t is not None else None for t in (x, w, b)]
-    loss = fh.linear_cross_entropy(leaves[0], leaves[1], targets, leaves[2], reduction=reduction, **args)
-    grads = list(torch.autograd.grad(loss, [t for t in leaves if t is not None], g))
-    return [loss.detach(), *grads]
+OPS = torch.ops.flash_hypercons
+
+
+def _step(x, w, targets, b, reduction, g, way=None, **args):
+    """Loss and gradients: by autograd, or by the operators of one way of forming them."""
+    if way is None:
+        leaves = [t.detach().requires_grad_() if t is not None else None for t in (x, w, b)]
+        loss = fh.linear_cross_entropy(leaves[0], leaves[1], targets, leaves[2], reduction=reduction, **args)
+        grads = list(torch.autograd.grad(loss, [t for t in leaves if t is not None], g))
+        return [loss.detach(), *grads]
+    how = args.get("ignore_index", -100), {"none": 0, "sum": 1, "mean": 2}[reduction]
+    wanted = True, True, b is not None
+    if way == "ahead":
+        loss, *sums = OPS._linear_cross_entropy_ahead(x, w, targets, b, *how, *wanted)
+        grads = OPS._linear_cross_entropy_scale(g, x, w, targets, b, *sums, *how)
+    else:
+        loss, lse = OPS._linear_cross_entropy_forward(x, w, targets, b, *how)
+        grads = OPS._linear_cross_entropy_backward(g, x, w, targets, b, lse, *how, *wanted)
+    return [loss, *grads[: 2 + (b is not None)]]
+
+
+def _ways(reduction):
+    return ["again"] if reduction == "none" else ["again", "ahead"]
 
 
 def _compare(x, w, targets, b=None, reduction="mean", g=None, **args):
     if g is None:
         g = torch.rand(targets.shape, device=x.device) if reduction == "none" else torch.tensor(3.0, device=x.device)
-    got = _step(x, w, targets, b, reduction, g, **args)
-    want, bound = _formula(x, w, targets, b, reduction, g, args.get("ignore_index", -100))
-    assert got[0].dtype == torch.float32
-    for name, a, e, limit in zip(("loss", "dx", "dw", "db"), got, want, bound):
-        _check(a, e, limit, name)
+    default = _step(x, w, targets, b, reduction, g, **args)
+    found = []
+    for way in _ways(reduction):
+        got = _step(x, w, targets, b, reduction, g, way, **args)
+        want, bound = _formula(x, w, targets, b, reduction, g, args.get("ignore_index", -100), way == "ahead")
+        assert got[0].dtype == torch.float32
+        for name, a, e, limit in zip(("loss", "dx", "dw", "db"), got, want, bound):
+            _check(a, e, limit, f"{way} {name}")
+        found.append(all(torch.equal(a.nan_to_num(7e7), e.nan_to_num(7e7)) for a, e in zip(default, got)))
+    rows = targets.numel()
+    ahead = reduction != "none" and rows >= (256 if x.dtype == torch.float32 else 1024)
+    assert found[ahead]  # what autograd takes
     with torch.no_grad():
         again = fh.linear_cross_entropy(x, w, targets, b, reduction=reduction, **args)
-    torch.testing.assert_close(again, got[0], rtol=0, atol=0, equal_nan=True)
-    return got
+    torch.testing.assert_close(again, default[0], rtol=1e-6, atol=0, equal_nan=True)
+    return default
 
 
 def _inputs(m, k, v, dtype, seed=0, device="cuda", ignored=0.0, bias=None, sure=6.0):
@@ -163,19 +194,20 @@ def test_reductions(m, reduction, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("way", ["again", "ahead"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("m", [1, 90, 600])
-def test_positions_without_a_target_take_no_part(m, dtype):
+def test_positions_without_a_target_take_no_part(m, dtype, way):
     x, w, t, b = _inputs(m + 40, 72, 500, dtype, seed=m)
     t[5:45] = -1
     x[5:45] = float("nan")
     x[20] = float("inf")
     keep = torch.ones(m + 40, dtype=torch.bool, device="cuda")
     keep[5:45] = t[m + 1:m + 1] = False
-    for reduction in REDUCTIONS:
+    for reduction in (r for r in REDUCTIONS if way in _ways(r)):
         g = torch.rand(m + 40, device="cuda") if reduction == "none" else torch.tensor(1.0, device="cuda")
-        got = _step(x, w, t, b, reduction, g, ignore_index=-1)
-        alone = _step(x[keep], w, t[keep], b, reduction, g[keep] if reduction == "none" else g)
+        got = _step(x, w, t, b, reduction, g, way, ignore_index=-1)
+        alone = _step(x[keep], w, t[keep], b, reduction, g[keep] if reduction == "none" else g, way)
         assert not got[1][5:45].any()
         if reduction == "none":
             assert not got[0][5:45].any()
@@ -185,14 +217,15 @@ def test_positions_without_a_target_take_no_part(m, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("way", ["again", "ahead"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("m", [1, 300])
-def test_no_target_at_all(m, dtype):
+def test_no_target_at_all(m, dtype, way):
     x, w, t, b = _inputs(m, 40, 100, dtype)
     t[:] = -100
-    for reduction in REDUCTIONS:
+    for reduction in (r for r in REDUCTIONS if way in _ways(r)):
         g = torch.ones(m if reduction == "none" else (), device="cuda")
-        loss, *grads = _step(x, w, t, b, reduction, g)
+        loss, *grads = _step(x, w, t, b, reduction, g, way)
         assert loss.isnan().all() if reduction == "mean" else not loss.any()
         assert not any(d.any() for d in grads)
 
@@ -218,19 +251,22 @@ def test_targets_out_of_range(m, dtype):
     assert loss[[1, 2]].isnan().all() and loss[good].isfinite().all()
     assert dx[[1, 2]].isnan().all() and dx[good].isfinite().all() and dw.isnan().all()
     assert fh.linear_cross_entropy(x, w, t).isnan()
+    loss, dx, dw = _step(x, w, t, None, "sum", g[0], "ahead")
+    assert loss.isnan() and dx[[1, 2]].isnan().all() and dx[good].isfinite().all() and dw.isnan().all()
 
 
 @gpu
+@pytest.mark.parametrize("way", ["again", "ahead"])
 @pytest.mark.parametrize("m", [2, 150])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_words_that_a_bias_rules_out(m, dtype):
+def test_words_that_a_bias_rules_out(m, dtype, way):
     """A bias of -inf or of the type's lowest value, as a padded vocabulary has."""
     x, w, t, b = _inputs(m, 64, 300, dtype)
     t = t % 200
     for low in (float("-inf"), torch.finfo(dtype).min):
         b[200:] = low
-        got = _step(x, w, t, b, "mean", torch.tensor(1.0, device="cuda"))
-        want, bound = _formula(x, w[:200], t, b[:200], "mean", torch.tensor(1.0, device="cuda"))
+        got = _step(x, w, t, b, "mean", torch.tensor(1.0, device="cuda"), way)
+        want, bound = _formula(x, w[:200], t, b[:200], "mean", torch.tensor(1.0, device="cuda"), ahead=way == "ahead")
         _check(got[0], want[0], bound[0], "loss")
         _check(got[1], want[1], bound[1], "dx")
         _check(got[2][:200], want[2], bound[2], "dw")
@@ -251,6 +287,8 @@ def test_infinity_and_nan_stay_in_their_row(m, dtype):
     loss, dx, _ = _step(x, w, t, None, "none", torch.ones(m, device="cuda"))
     good = [i for i in range(m) if i not in (1, 2)]
     assert loss[[1, 2]].isnan().all() and loss[good].isfinite().all() and dx[good].isfinite().all()
+    loss, dx, _ = _step(x, w, t, None, "sum", torch.tensor(1.0, device="cuda"), "ahead")
+    assert loss.isnan() and dx[[1, 2]].isnan().all() and dx[good].isfinite().all()
 
 
 @gpu
@@ -258,8 +296,9 @@ def test_infinity_and_nan_stay_in_their_row(m, dtype):
 def test_large_logits(dtype):
     """Logits far beyond exp's range, certain and hopeless targets."""
     x, w, t, _ = _inputs(100, 64, 200, dtype, sure=0.0)
-    _compare(x * 60, w * 4, t, None, "none")
-    _compare(x * 60, w * 4, (x.float() @ w.float().t()).argmax(1), None, "none")
+    for reduction in ("none", "sum"):
+        _compare(x * 60, w * 4, t, None, reduction)
+        _compare(x * 60, w * 4, (x.float() @ w.float().t()).argmax(1), None, reduction)
 
 
 @gpu
@@ -278,8 +317,11 @@ def test_upstream_gradients_of_any_size(dtype, scale):
 @gpu
 def test_zero_and_infinite_upstream_gradients():
     x, w, t, b = _inputs(40, 64, 300, torch.float16)
-    assert not any(d.any() for d in _step(x, w, t, b, "mean", torch.tensor(0.0, device="cuda"))[1:])
-    assert all(not d.isfinite().all() for d in _step(x, w, t, b, "mean", torch.tensor(float("inf"), device="cuda"))[1:])
+    for way in _ways("mean"):
+        assert not any(d.any() for d in _step(x, w, t, b, "mean", torch.tensor(0.0, device="cuda"), way)[1:])
+        for bad in (float("inf"), float("nan")):
+            grads = _step(x, w, t, b, "mean", torch.tensor(bad, device="cuda"), way)[1:]
+            assert all(not d.isfinite().all() for d in grads)
 
 
 @gpu
@@ -309,8 +351,9 @@ def test_views(dtype, m):
 
 
 @gpu
-def test_partial_gradients():
-    x, w, t, b = _inputs(50, 80, 1000, torch.bfloat16, ignored=0.3)
+@pytest.mark.parametrize("m", [50, 1100])
+def test_partial_gradients(m):
+    x, w, t, b = _inputs(m, 80, 1000, torch.bfloat16, ignored=0.3)
     g = torch.tensor(2.0, device="cuda")
     full = _step(x, w, t, b, "mean", g)[1:]
     for only in range(3):
@@ -322,7 +365,7 @@ def test_partial_gradients():
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("m,k,v", [(2, 4096, 1000), (400, 512, 3000), (700, 72, 20)])
+@pytest.mark.parametrize("m,k,v", [(2, 4096, 1000), (400, 512, 3000), (700, 72, 20), (1500, 256, 4000)])
 def test_results_are_the_same_bits_again(m, k, v, dtype):
     x, w, t, b = _inputs(m, k, v, dtype, ignored=0.2)
     g = torch.tensor(1.0, device="cuda")
@@ -372,14 +415,26 @@ def test_second_derivatives_go_native(reduction):
 
 
 @gpu
-def test_compiled_step_matches():
-    x, w, t, b = _inputs(33, 72, 400, torch.bfloat16)
+def test_a_graph_that_is_walked_twice():
+    x, w, t, b = _inputs(1100, 80, 500, torch.bfloat16)
     leaves = [a.clone().requires_grad_() for a in (x, w, b)]
-    f = torch.compile(lambda a, ww, bb: fh.linear_cross_entropy(a, ww, t, bb), fullgraph=True, backend="aot_eager")
+    loss = fh.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    for g in (1.0, 0.125):
+        g = torch.tensor(g, device="cuda")
+        got = torch.autograd.grad(loss, leaves, g, retain_graph=True)
+        assert all(map(torch.equal, got, _step(x, w, t, b, "mean", g)[1:]))
+
+
+@gpu
+def test_compiled_step_matches():
+    f = torch.compile(lambda a, ww, tt, bb: fh.linear_cross_entropy(a, ww, tt, bb), fullgraph=True, backend="aot_eager")
     g = torch.tensor(1.0, device="cuda")
-    loss = f(*leaves)
-    got = [loss, *torch.autograd.grad(loss, leaves, g)]
-    assert all(map(torch.equal, got, _step(x, w, t, b, "mean", g)))
+    for m, v in ((33, 400), (40, 401), (1200, 500), (1100, 700)):  # sizes become symbols; both ways
+        x, w, t, b = _inputs(m, 72, v, torch.bfloat16)
+        leaves = [a.clone().requires_grad_() for a in (x, w, b)]
+        loss = f(leaves[0], leaves[1], t, leaves[2])
+        got = [loss.detach(), *torch.autograd.grad(loss, leaves, g)]
+        assert all(map(torch.equal, got, _step(x, w, t, b, "mean", g)))
 
 
 @pytest.mark.parametrize("reduction", REDUCTIONS)
@@ -423,3 +478,13 @@ def test_refusals():
         ops._linear_cross_entropy_backward(loss, x, w, t, b, lse.half(), -100, 2, True, True, True)
     with pytest.raises(RuntimeError, match="grad"):
         ops._linear_cross_entropy_backward(lse, x, w, t, b, lse, -100, 2, True, True, True)
+    with pytest.raises(RuntimeError, match="sum or mean"):
+        ops._linear_cross_entropy_ahead(x, w, t, b, -100, 0, True, True, True)
+    loss, *sums = ops._linear_cross_entropy_ahead(x, w, t, b, -100, 2, True, True, False)
+    assert [a.numel() for a in sums] == [5, 40, 60, 0]
+    with pytest.raises(RuntimeError, match="sums"):
+        ops._linear_cross_entropy_scale(loss, x, w, t, b, sums[0], sums[1][:2], *sums[2:], -100, 2)
+    with pytest.raises(RuntimeError, match="sums"):
+        ops._linear_cross_entropy_scale(loss, x, w, t, b, sums[0][:0], *sums[1:], -100, 2)
+    with pytest.raises(RuntimeError, match="grad"):
+        ops._linear_cross_entropy_scale(lse, x, w, t, b, *sums, -100, 2)
