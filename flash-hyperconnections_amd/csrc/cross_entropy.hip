@@ -138,13 +138,26 @@ struct GatherArgs {
   void* out;          // [rows, ld], zero past cols
   int64_t ld;
   int cols;
+  // Rows of dx without a target are zeroed, unless it is null.
+  const int64_t* targets;
+  int64_t ignore, rows;
+  void* dx;
 };
 
-// A wavefront to each row that has a target.
+template <typename T>
+__device__ __forceinline__ void zero_row(const int64_t* targets, int64_t ignore, int64_t row, int cols, void* dx) {
+  if (dx == nullptr || targets[row] != ignore) return;
+  auto* to = static_cast<typename T::storage*>(dx) + row * cols;
+  for (int c = (threadIdx.x & 63) * kVec<T>; c < cols; c += 64 * kVec<T>) store_row<T>(U32x4{0, 0, 0, 0}, to, c, cols);
+}
+
+// A wavefront to each row, and to each that has a target.
 template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
   using S = typename T::storage;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  zero_row<T>(a.targets, a.ignore, row, a.cols, a.dx);
   if (row >= *a.live) return;
   const S* from = static_cast<const S*>(a.src) + a.index[row] * a.src_stride;
   S* to = static_cast<S*>(a.out) + row * a.ld;
@@ -152,16 +165,6 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
     const U32x4 w = load_row<T>(from, c, a.cols);
     __builtin_memcpy(to + c, &w, 16);
   }
-}
-
-// Zeros for the rows without a target, a wavefront to each.
-template <typename T>
-__global__ __launch_bounds__(256) void zero_rows_kernel(const int64_t* targets, int64_t ignore, int64_t rows, int cols,
-                                                        void* out) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows || targets[row] != ignore) return;
-  auto* to = static_cast<typename T::storage*>(out) + row * cols;
-  for (int c = (threadIdx.x & 63) * kVec<T>; c < cols; c += 64 * kVec<T>) store_row<T>(U32x4{0, 0, 0, 0}, to, c, cols);
 }
 
 struct SlopeArgs {
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
 
 // out = sums times grad, over how many rows have a target for a mean (nothing where none has): a
 // wavefront to a row, or to every gridDim.y-th 512 columns of it.  With an index the first `live`
-// rows, row k into row index[k].
+// rows, row k into row index[k], beside zeros for those without a target.
 struct ScaleArgs {
   const float* sums;
   const int *live, *index;
@@ -235,13 +238,19 @@ struct ScaleArgs {
   int64_t rows;
   int cols;
   void* out;
+  const int64_t* targets;
+  int64_t ignore;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(ScaleArgs a) {
   constexpr int V = 8;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= (a.index != nullptr ? *a.live : a.rows)) return;
+  if (row >= a.rows) return;
   const int live = *a.live;
+  if (a.index != nullptr) {
+    if (blockIdx.y == 0) zero_row<T>(a.targets, a.ignore, row, a.cols, a.out);
+    if (row >= live) return;
+  }
   const float times = live == 0 ? 0.f : *a.grad / (a.mean ? static_cast<float>(live) : 1.f);
   const float* from = a.sums + row * a.cols;
   auto* to = static_cast<typename T::storage*>(a.out) + (a.index != nullptr ? a.index[row] : row) * a.cols;
@@ -316,55 +325,63 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* losses, const i
   if (threadIdx.x == 0) *out = static_cast<float>(mean ? sum / count : sum);
 }
 
-// Column sums of dz [rows, ld]: 64 V columns and every gridDim.y-th four rows a workgroup.
+struct BiasArgs {
+  const void* dz;      // [rows, ld]
+  int64_t ld;
+  int cols, rows;
+  const int* live;
+  int row0;
+  float* partial;      // [gridDim.y, cols], or null where the sums are db already
+  const float* scale;  // what db is times, or null
+  void* out;
+  int out_f32;         // its type: FP32, or dz's
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void bias_kernel(const void* dz, int64_t ld, int cols, int most, const int* live,
-                                                   int row0, float* partial) {
+__device__ __forceinline__ void put_bias(const BiasArgs& a, int c, float sum) {
+  if (a.scale != nullptr) sum *= *a.scale;
+  if (a.out_f32) static_cast<float*>(a.out)[c] = sum;
+  else static_cast<typename T::storage*>(a.out)[c] = from_f32<T>(sum);
+}
+
+// Column sums of dz: 64 V columns and every gridDim.y-th sixteen rows a workgroup, a row a wavefront.
+template <typename T>
+__global__ __launch_bounds__(1024) void bias_kernel(BiasArgs a) {
   using S = typename T::storage;
   constexpr int V = kVec<T>;
-  __shared__ float area[4][V][64];
+  __shared__ float area[16][V][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = (static_cast<int>(blockIdx.x) * 64 + lane) * V;
-  const int more = *live - row0, rows = more < most ? more : most;
+  const int first = static_cast<int>(blockIdx.x) * 64 * V, c = first + lane * V;
+  const int more = *a.live - a.row0, rows = more < a.rows ? more : a.rows;
   float sums[V] = {};
-  for (int row = blockIdx.y * 4 + wave; row < rows; row += gridDim.y * 4) {
+#pragma unroll 4
+  for (int row = blockIdx.y * 16 + wave; row < rows; row += gridDim.y * 16) {
     float f[V];
-    to_floats<T>(load_row<T>(static_cast<const S*>(dz) + row * ld, c, cols), f);
+    to_floats<T>(load_row<T>(static_cast<const S*>(a.dz) + row * a.ld, c, a.cols), f);
 #pragma unroll
     for (int i = 0; i < V; ++i) sums[i] += f[i];
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) area[wave][i][lane] = sums[i];
   __syncthreads();
-  if (wave != 0) return;
+  const int mine = static_cast<int>(threadIdx.x), to = first + mine;
+  if (mine >= 64 * V || to >= a.cols) return;
+  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (c + i < cols)
-      partial[static_cast<int64_t>(blockIdx.y) * cols + c + i] =
-          ((area[0][i][lane] + area[1][i][lane]) + area[2][i][lane]) + area[3][i][lane];
+  for (int w = 0; w < 16; ++w) sum += area[w][mine % V][mine / V];
+  if (a.partial != nullptr) a.partial[static_cast<int64_t>(blockIdx.y) * a.cols + to] = sum;
+  else put_bias<T>(a, to, sum);
 }
 
-// db from `count` partial sums; `scale` may be null.
+// db from `count` partial sums.
 template <typename T>
-__global__ __launch_bounds__(256) void join_bias_kernel(const float* partial, int count, int cols, const float* scale,
-                                                        void* out) {
+__global__ __launch_bounds__(256) void join_bias_kernel(BiasArgs a, int count) {
   const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+  if (c >= a.cols) return;
   float sum = 0.f;
 #pragma unroll 8
-  for (int i = 0; i < count; ++i) sum += partial[static_cast<int64_t>(i) * cols + c];
-  static_cast<typename T::storage*>(out)[c] = from_f32<T>(scale != nullptr ? sum * *scale : sum);
-}
-
-hipError_t launch_bias(const Laid& dz, int64_t cols, int64_t rows, const int* live, int64_t row0, int down,
-                       float* partial, int dtype, hipStream_t stream) {
-  return with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    const dim3 grid(static_cast<uint32_t>((cols + 64 * kVec<T> - 1) / (64 * kVec<T>)), static_cast<uint32_t>(down));
-    bias_kernel<T><<<grid, dim3(256), 0, stream>>>(dz.data, dz.ld, static_cast<int>(cols), static_cast<int>(rows), live,
-                                                   static_cast<int>(row0), partial);
-    return hipGetLastError();
-  });
+  for (int i = 0; i < count; ++i) sum += a.partial[static_cast<int64_t>(i) * a.cols + c];
+  put_bias<T>(a, c, sum);
 }
 
 int element(int dtype) { return dtype == F32::code ? 4 : 2; }
@@ -374,6 +391,47 @@ char* bytes_on(const void* p, int64_t bytes) {
 }
 
 dim3 blocks_of(int64_t items, int each) { return dim3(static_cast<uint32_t>((items + each - 1) / each)); }
+
+// db of `cols` words from the dz of `chunks` chunks of up to `most` rows each, one after the other.
+class BiasSums {
+ public:
+  BiasSums(bool wanted, int64_t chunks, int64_t most, int64_t cols, int dtype, Workspace& ws)
+      : dtype_(dtype), chunks_(static_cast<int>(chunks)), most_(most),
+        down_(most <= 512 ? 1 : static_cast<int>(std::min<int64_t>(most / 256, 64))) {
+    if (wanted && chunks_ * down_ > 1) partial_ = ws.take<float>(chunks * down_ * cols);
+  }
+  // Adds rows row0 .. row0 + rows - 1; `args` has the output.
+  hipError_t add(BiasArgs args, const Laid& dz, int64_t row0, int64_t rows, hipStream_t stream) const {
+    args.dz = dz.data;
+    args.ld = dz.ld;
+    args.row0 = static_cast<int>(row0);
+    args.rows = static_cast<int>(rows);
+    const int64_t chunk = row0 / most_;
+    args.partial = partial_ != nullptr ? partial_ + chunk * down_ * args.cols : nullptr;
+    return with_type(dtype_, [&](auto t) {
+      using T = decltype(t);
+      const int64_t each = 64 * kVec<T>;
+      const dim3 grid(static_cast<uint32_t>((args.cols + each - 1) / each), static_cast<uint32_t>(down_));
+      bias_kernel<T><<<grid, dim3(1024), 0, stream>>>(args);
+      return hipGetLastError();
+    });
+  }
+  hipError_t join(BiasArgs args, hipStream_t stream) const {
+    if (partial_ == nullptr) return hipSuccess;
+    args.partial = partial_;
+    return with_type(dtype_, [&](auto t) {
+      const dim3 grid(static_cast<uint32_t>((args.cols + 255) / 256));
+      join_bias_kernel<decltype(t)><<<grid, dim3(256), 0, stream>>>(args, chunks_ * down_);
+      return hipGetLastError();
+    });
+  }
+
+ private:
+  int dtype_, chunks_;
+  int64_t most_;
+  int down_;
+  float* partial_ = nullptr;
+};
 
 // The rows with a target and x's rows of them.
 struct Rows {
@@ -391,7 +449,7 @@ hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, Workspace& ws, R
   r.index = got.index = a.places != nullptr ? a.places + 1 : ws.take<int>(a.rows);
   r.label = got.label = ws.take<int>(a.rows);
   GatherArgs g{a.x, a.x_stride, got.live, got.index, ws.take<char>(a.rows * ld * element(a.dtype)), ld,
-               static_cast<int>(a.cols)};
+               static_cast<int>(a.cols), a.targets, a.ignore, a.rows, backward ? a.dx : nullptr};
   got.x = {g.out, ld};
   if (ws.dry()) return hipSuccess;
   if (backward) rows_kernel<true><<<dim3(1), dim3(kRowThreads), 0, stream>>>(r);
@@ -447,7 +505,9 @@ int lse_rows(int64_t rows) {
 }
 
 constexpr int64_t kStats = int64_t{1} << 25;  // maxima and sums at a time: 256 MB
-constexpr int64_t kPiece = int64_t{1} << 30;  // bytes of dz at a time
+// Bytes of exponentials or dz at a time.  Half as many take 1 ms more of 44.7 for 16384 x 4096 into 131072 words: dW's
+// sum is read and written for each chunk.
+constexpr int64_t kPiece = int64_t{1} << 31;
 
 }  // namespace
 
@@ -505,9 +565,12 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   auto* lse = ws.take<float>(a.rows);
   auto* losses = ws.take<float>(a.rows);
   const Laid dz{ws.take<char>(most * ld * element(a.dtype)), ld};
-  const int64_t chunks = (a.rows + most - 1) / most;
-  const int down = static_cast<int>(std::min<int64_t>((most + 15) / 16, 64));
-  auto* partial = a.db_sums != nullptr ? ws.take<float>(chunks * down * a.vocab) : nullptr;
+  const BiasSums db(a.db_sums != nullptr, (a.rows + most - 1) / most, most, a.vocab, a.dtype, ws);
+  BiasArgs db_args{};
+  db_args.cols = static_cast<int>(a.vocab);
+  db_args.live = rows.live;
+  db_args.out = a.db_sums;
+  db_args.out_f32 = 1;
   const int64_t before = ws.used();
   int64_t most_used = before;
   // Products follow one another on the stream, and share the space for what their slices add up to.
@@ -539,8 +602,7 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
         slope_kernel<T><<<grid, dim3(256), 0, stream>>>(s);
         return hipGetLastError();
       });
-      if (e == hipSuccess && a.db_sums != nullptr)
-        e = launch_bias(dz, a.vocab, count, rows.live, row0, down, partial + row0 / most * down * a.vocab, a.dtype, stream);
+      if (e == hipSuccess && a.db_sums != nullptr) e = db.add(db_args, dz, row0, count, stream);
     }
     LossProductArgs s{};
     s.loss.live = rows.live;
@@ -566,10 +628,8 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   });
   if (err == hipSuccess && !ws.dry()) {
     loss_kernel<<<dim3(1), dim3(1024), 0, stream>>>(losses, rows.live, a.reduction == FH_REDUCE_MEAN, a.loss);
-    if (a.db_sums != nullptr)
-      join_bias_kernel<F32><<<blocks_of(a.vocab, 256), dim3(256), 0, stream>>>(
-          partial, static_cast<int>(chunks) * down, static_cast<int>(a.vocab), nullptr, a.db_sums);
     err = hipGetLastError();
+    if (err == hipSuccess && a.db_sums != nullptr) err = db.join(db_args, stream);
   }
   if (bytes != nullptr) *bytes = most_used;
   return err;
@@ -593,15 +653,10 @@ hipError_t launch_cross_entropy_scale(const LossArgs& a, hipStream_t stream) {
       return hipGetLastError();
     });
   };
+  s.targets = a.targets;
+  s.ignore = a.ignore;
   hipError_t err = hipSuccess;
-  if (a.dx != nullptr) {
-    err = with_type(a.dtype, [&](auto t) {
-      zero_rows_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(
-          a.targets, a.ignore, a.rows, static_cast<int>(a.cols), a.dx);
-      return hipGetLastError();
-    });
-    if (err == hipSuccess) err = scale(a.rows, a.cols, a.dx_sums, a.places + 1, a.dx, a.dtype);
-  }
+  if (a.dx != nullptr) err = scale(a.rows, a.cols, a.dx_sums, a.places + 1, a.dx, a.dtype);
   if (err == hipSuccess && a.dweight != nullptr) err = scale(a.vocab, a.cols, a.dw_sums, nullptr, a.dweight, a.dtype);
   if (err == hipSuccess && a.dbias != nullptr) err = scale(1, a.vocab, a.db_sums, nullptr, a.dbias, a.bias_dtype);
   return err;
@@ -633,15 +688,7 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
   const Laid dz{ws.take<char>(most_rows * ld * es), ld};
   auto* dx_sums = a.dx != nullptr && piece < a.vocab ? ws.take<float>(a.rows * a.cols) : nullptr;
   auto* dw_sums = a.dweight != nullptr && chunks > 1 ? ws.take<float>(piece * a.cols) : nullptr;
-  const int down = static_cast<int>(std::min<int64_t>((most_rows + 15) / 16, 64));  // partial sums of db for each chunk
-  auto* db_sums = a.dbias != nullptr ? ws.take<float>(chunks * down * piece) : nullptr;
-  if (a.dx != nullptr && !ws.dry()) {
-    err = with_type(a.dtype, [&](auto t) {
-      zero_rows_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(
-          a.targets, a.ignore, a.rows, static_cast<int>(a.cols), a.dx);
-      return hipGetLastError();
-    });
-  }
+  const BiasSums db(a.dbias != nullptr, chunks, most_rows, piece, a.dtype, ws);
   // Products follow one another on the stream, and share the space for what their slices add up to.
   const int64_t before = ws.used();
   int64_t most_used = before;
@@ -654,6 +701,12 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
   if (err == hipSuccess) {
     err = in_slices(a.vocab, piece, [&](int64_t col0, int64_t outs) {
       const Laid wp = rows_from(w, col0, a.dtype);
+      BiasArgs db_args{};
+      db_args.cols = static_cast<int>(outs);
+      db_args.live = rows.live;
+      db_args.scale = r.scale;
+      db_args.out = bytes_on(a.dbias, col0 * element(a.bias_dtype));
+      db_args.out_f32 = a.bias_dtype == F32::code;
       const hipError_t all = in_slices(a.rows, most_rows, [&](int64_t row0, int64_t count) {
         const Laid xp = rows_from(rows.x, row0, a.dtype);
         hipError_t e = shared([&](Workspace& part) {
@@ -695,17 +748,10 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
             return multiply(p, d, xp, a.dtype, true, true, Finish::kSum, part, stream);
           });
         }
-        if (e == hipSuccess && a.dbias != nullptr && !ws.dry())
-          e = launch_bias(d, outs, count, rows.live, row0, down, db_sums + row0 / most_rows * down * outs, a.dtype, stream);
+        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) e = db.add(db_args, d, row0, count, stream);
         return e;
       });
-      if (all != hipSuccess || a.dbias == nullptr || ws.dry()) return all;
-      return with_type(a.bias_dtype, [&](auto t) {
-        join_bias_kernel<decltype(t)><<<blocks_of(outs, 256), dim3(256), 0, stream>>>(
-            db_sums, static_cast<int>(chunks) * down, static_cast<int>(outs), r.scale,
-            bytes_on(a.dbias, col0 * element(a.bias_dtype)));
-        return hipGetLastError();
-      });
+      return all != hipSuccess || a.dbias == nullptr || ws.dry() ? all : db.join(db_args, stream);
     });
   }
   if (bytes != nullptr) *bytes = most_used;

@@ -49,6 +49,7 @@ struct ProductArgs {
   int tiles_m, tiles_n;
   int side_m, side_n;    // of a tile
   int slices;            // of the sum over k
+  int paired;            // 16 bits, 128 x 128: two workgroups a compute unit
   float* partial;        // [slices, m, n] where there are several
   const void* bias;      // [n] or null, FP32 or the output's type
   int bias_f32;
@@ -485,6 +486,35 @@ __device__ __forceinline__ void park(char* area, int r, int c, Floats4 v) {
 template <typename T, Finish F, int Rows>
 __device__ __forceinline__ void finish_parked(const ArgsOf<F>& p, int slice, const char* area, int row, int col,
                                               int lane) {
+  if constexpr (F == Finish::kSum && T::code != F32::code) {
+    // FP32 sums in whole lines, sixteen lanes to a row, four rows' loads on their way at a time.
+    if (p.slices == 1 && !p.loss.last) {
+      asm volatile("" ::: "memory");
+      const int c = lane & 15, j = col + 4 * c, left = p.n - j;
+#pragma unroll 1
+      for (int it = 0; it < Rows / 4; it += 4) {
+        float before[4][4] = {};
+        int64_t at[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = row + 4 * (it + u) + (lane >> 4);
+          at[u] = i < p.m && left > 0 ? static_cast<int64_t>(i) * p.n + j : -1;
+          if (!p.loss.first && at[u] >= 0) load_some(p.loss.sums + at[u], left, before[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = 4 * (it + u) + (lane >> 4);
+          float v[4];
+          __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] += before[u][k];
+          if (at[u] >= 0) store_some(v, p.loss.sums + at[u], left);
+        }
+      }
+      asm volatile("" ::: "memory");
+      return;
+    }
+  }
   constexpr int down = T::code == F32::code ? 4 : 8, turns = Rows / down;  // rows at a time
   const int first = T::code == F32::code ? lane >> 4 : lane >> 3;
   RowOf<F> of[turns];
@@ -601,7 +631,7 @@ constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16
 // sums, in one slice.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
-// vectors; false for others.
+// vectors; false for others.  Not for Finish::kExp.
 bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices);
 // `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,

@@ -144,26 +144,39 @@ __global__ __launch_bounds__(512, 2) void product_kernel(ArgsOf<F> p) {
   finish_parked<T, F, 32 * Tall>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
-// Sums of one step, at most 64 terms: two workgroups a compute unit, one storing while
-// the other loads.  Bound by the stores: 16384 x 16 x 16384 bf16 (537 MB) takes 124 to
-// 137 us; tiles of 256 x 256 took 157 to 166, the 128 x 128 tiles with a ring 179.
-template <typename T, bool ACols, bool BCols, Finish F>
-__global__ __launch_bounds__(512, 4) void outer_product_kernel(ArgsOf<F> p) {
+// Two workgroups a compute unit, one of them storing or waiting for its loads while the other computes, with two
+// steps' buffers each: for sums of one step, and where there are more than one of these tiles a unit.  16384 x 16 x
+// 16384 bf16 (537 MB, bound by the stores) takes 124 to 137 us, in tiles of 256 x 256 157 to 166, in 128 x 128 tiles
+// with a ring 179; dW of 200 x 1024 into 50001 words, four steps, 47 us, 64 and 75; 64 rows' logits there 22, 29 and 28.
+// One: sums of at most 64 terms in one slice, whose second buffers stay empty (318 us for the three products of 16384
+// x 16384 into 16, 341 in the general form).
+template <typename T, bool One, bool ACols, bool BCols, Finish F>
+__global__ __launch_bounds__(512, 4) void paired_product_kernel(ArgsOf<F> p) {
   if (!fit<F, ACols>(p)) return;
-  __shared__ __attribute__((aligned(1024))) char lds[8 * 8192];  // A's and B's step, then the results
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kBuffer];  // A's and B's step, twice; then the results
+  static_assert(4 * kBuffer == 8 * 8192, "32 x 64 results a wavefront");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile tile = tile_of(p, blockIdx.x);
+  const auto [tile, slice] = One ? Piece{tile_of(p, blockIdx.x), 0} : piece_of<BCols>(p);
   const int m0 = tile.m * kTile, n0 = tile.n * kTile;
+  const Steps<kStep> steps(p, slice);
+  const int begin = One ? 0 : steps.begin, count = steps.end - begin;
   Feeder<ACols, kTile> a;
   Feeder<BCols, kTile> b;
-  a.init(p.a, p.lda, m0, p.m, p.k, 0, lds_address(lds), lane, wave);
-  b.init(p.b, p.ldb, n0, p.n, p.k, 0, lds_address(lds) + kBuffer, lane, wave);
+  a.init(p.a, p.lda, m0, p.m, p.k, begin, lds_address(lds), lane, wave);
+  b.init(p.b, p.ldb, n0, p.n, p.k, begin, lds_address(lds) + kBuffer, lane, wave);
+  const auto stage = [&](int offset) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    a.stage(u, 0);
-    b.stage(u, 0);
-  }
+    for (int u = 0; u < 2; ++u) {
+      a.stage(u, offset);
+      b.stage(u, offset);
+    }
+    if constexpr (!One) {
+      a.advance();
+      b.advance();
+    }
+  };
+  if constexpr (One) stage(0);
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 64;
   const Finder<ACols, kTile> fa(lds_address(lds), wm, lane);
   const Finder<BCols, kTile> fb(lds_address(lds) + kBuffer, wn, lane);
@@ -172,15 +185,37 @@ __global__ __launch_bounds__(512, 4) void outer_product_kernel(ArgsOf<F> p) {
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
-  wait_loads<0>();
-  meet();
+  const auto step = [&](auto at, bool more) {
+    constexpr int offset = decltype(at)::value * 2 * kBuffer;
+    if (more) {
+      stage(2 * kBuffer - offset);
+      wait_loads<4>();  // this step's are there once only the next one's are on their way
+    } else {
+      wait_loads<0>();
+    }
+    meet();
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    if (16 * kk >= p.k) break;
-    multiply<T>(acc, fa.read(0, 0, kk), fb.read(0, 0, kk), fb.read(0, 1, kk));
+    for (int kk = 0; kk < 4; ++kk) multiply<T>(acc, fa.read(offset, 0, kk), fb.read(offset, 0, kk), fb.read(offset, 1, kk));
+    wait_lds();
+    meet();  // the buffer has been read
+  };
+  if constexpr (One) {
+    wait_loads<0>();
+    meet();
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      if (16 * kk >= p.k) break;
+      multiply<T>(acc, fa.read(0, 0, kk), fb.read(0, 0, kk), fb.read(0, 1, kk));
+    }
+    wait_lds();
+    meet();
+  } else if (count > 0) {
+    stage(0);
+    for (int s = 0; s < count; s += 2) {
+      step(std::integral_constant<int, 0>{}, s + 1 < count);
+      if (s + 1 < count) step(std::integral_constant<int, 1>{}, s + 2 < count);
+    }
   }
-  wait_lds();
-  meet();
   char* area = lds + wave * 8192;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -188,7 +223,7 @@ __global__ __launch_bounds__(512, 4) void outer_product_kernel(ArgsOf<F> p) {
     for (int q = 0; q < 4; ++q)
       park(area, lane & 31, 8 * j + 2 * q + (lane >> 5),
            Floats4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]});
-  finish_parked<T, F, 32>(p, 0, area, m0 + wm, n0 + wn, lane);
+  finish_parked<T, F, 32>(p, slice, area, m0 + wm, n0 + wn, lane);
 }
 
 // sum += Count slices `size` apart, in order, all on their way at once.
@@ -235,8 +270,10 @@ template <typename T>
 hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, const LossParts* loss, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.tiles_m * p.tiles_n), static_cast<uint32_t>(p.slices)), block(512);
   return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
-    if (p.k <= kStep && p.slices == 1)
-      outer_product_kernel<T, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
+    if (p.paired && p.k <= kStep)
+      paired_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
+    else if (p.paired)
+      paired_product_kernel<T, false, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     else if (p.side_m == kTile)
       product_kernel<T, 1, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
     else
@@ -266,10 +303,11 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
   const int most = whole_sums(finish) ? 1 : 16;
-  if (plan_narrow_product(p, dtype, a_cols, b_cols, most)) return;
+  if (finish != Finish::kExp && plan_narrow_product(p, dtype, a_cols, b_cols, most)) return;
   if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);
     p.slices = 1;
+    p.paired = !f32;
     return;
   }
   const int64_t units = compute_units();
@@ -285,21 +323,28 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
   struct Cost {
     int rows, cols;
     double fixed, step, shared;
+    int paired;
   };
-  constexpr Cost kF32[] = {{kTile, kTile, 4.2, 1.27, 0.3}, {2 * kTile, kTile, 7.0, 2.1, 0.55}};
+  constexpr Cost kF32[] = {{kTile, kTile, 4.2, 1.27, 0.3, 0}, {2 * kTile, kTile, 7.0, 2.1, 0.55, 0}};
   constexpr Cost kHalf[] = {
-      {kTile, kTile, 4.2, 0.33, 0.2}, {2 * kTile, kTile, 7.0, 0.56, 0.34}, {256, 256, 10.0, 1.0, 0.55}};
+      {kTile, kTile, 4.2, 0.33, 0.2, 0}, {2 * kTile, kTile, 7.0, 0.56, 0.34, 0}, {256, 256, 10.0, 1.0, 0.55, 0}};
+  // Two workgroups on each unit: both together.  Fitted to the loss's products of 64 to 512 rows into 32768 to
+  // 65536 words, whose times it gives to 15%.
+  constexpr Cost kPaired{kTile, kTile, 2.5, 1.15, 0.0, 1};
   const int64_t steps = f32 ? (p.k + 31) / 32 : (p.k + 63) / 64;
   const double results = static_cast<double>(p.m) * p.n;
   double best = -1.0;
   ProductArgs chosen = p;
   const auto consider = [&](const Cost& c) {
     set_tiles(p, c.rows, c.cols);
+    p.paired = c.paired;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+    const int64_t at_once = c.paired ? 2 : 1;  // on a unit
     for (int64_t s = 1; s <= most && s <= std::max<int64_t>(1, steps / 4); ++s) {
+      if (c.paired && tiles * s <= units) continue;
       const double full = std::min(1.0, static_cast<double>(tiles * s) / static_cast<double>(units));
       const double us =
-          rounds(tiles * s) * (c.fixed + (c.step + c.shared * full) * static_cast<double>((steps + s - 1) / s)) +
+          rounds((tiles * s + at_once - 1) / at_once) * (c.fixed + (c.step + c.shared * full) * static_cast<double>((steps + s - 1) / s)) +
           (s > 1 ? 3.5 + 1.3e-6 * results * static_cast<double>(s) : 0.0);
       if (best < 0.0 || us < best) {
         best = us;
@@ -312,6 +357,7 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
     for (const Cost& c : kF32) consider(c);
   } else {
     for (const Cost& c : kHalf) consider(c);
+    if (finish != Finish::kLinear) consider(kPaired);
   }
   p = chosen;
 }

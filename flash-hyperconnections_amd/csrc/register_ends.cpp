@@ -157,10 +157,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> loss_backward_hip(const at::Tenso
 }
 
 // Whether a step forms the gradients with the loss, for the upstream gradient to scale: one product of
-// four fewer, for FP32 sums of the weight's size.  On a step of 4096 x 32768 the two ways cross between 512
-// and 1024 rows (16 bits), and between 128 and 256 (FP32).
+// four fewer, for FP32 sums of the weight's size, which are written and read once more.  Against forming the
+// logits again, at 4096 x 32768, 1024 x 131072 (FP32: 10007) and 2048 x 10007: 0.99 to 1.04 times as long at 768
+// rows of 16 bits, 0.95 to 0.98 at 1024, 0.88 to 0.90 at 2048; FP32 0.86 to 1.01 at 128, 0.86 to 0.89 at 256.
 bool ahead_of(const at::Tensor& x, int64_t reduction) {
-  return reduction != FH_REDUCE_NONE && x.sym_numel() >= x.sym_size(-1) * (x.scalar_type() == at::kFloat ? 256 : 1024);
+  return reduction != FH_REDUCE_NONE && x.sym_numel() >= x.sym_size(-1) * (x.scalar_type() == at::kFloat ? 128 : 1024);
 }
 
 // (loss, places, sums of dx, dweight and dbias), the last three empty where not wanted.

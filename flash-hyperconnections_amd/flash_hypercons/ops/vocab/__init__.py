@@ -142,7 +142,7 @@ def linear_cross_entropy(
     """The softmax cross entropy of x @ weight.T + bias for x [..., K], weight [V, K] and targets [...].
 
     bias: [V] of x's type or float32.  The logits are formed in pieces, in float32, and never kept.  Where
-    a gradient is wanted of a sum or mean over 1024 positions or more (256 in float32), the gradients are
+    a gradient is wanted of a sum or mean over 1024 positions or more (128 in float32), the gradients are
     formed with the loss, as float32 sums that the backward scales by the upstream gradient; otherwise the
     backward forms the logits again.  Losses are float32 (float64 for float64 operands): of each position for
     reduction "none", else their "sum", or their "mean" over the positions with a target (NaN where there

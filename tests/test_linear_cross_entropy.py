@@ -148,7 +148,7 @@ def _compare(x, w, targets, b=None, reduction="mean", g=None, **args):
             _check(a, e, limit, f"{way} {name}")
         found.append(all(torch.equal(a.nan_to_num(7e7), e.nan_to_num(7e7)) for a, e in zip(default, got)))
     rows = targets.numel()
-    ahead = reduction != "none" and rows >= (256 if x.dtype == torch.float32 else 1024)
+    ahead = reduction != "none" and rows >= (128 if x.dtype == torch.float32 else 1024)
     assert found[ahead]  # what autograd takes
     with torch.no_grad():
         again = fh.linear_cross_entropy(x, w, targets, b, reduction=reduction, **args)
@@ -351,7 +351,7 @@ def test_views(dtype, m):
 
 
 @gpu
-@pytest.mark.parametrize("m", [50, 1100])
+@pytest.mark.parametrize("m", [50, 1300])
 def test_partial_gradients(m):
     x, w, t, b = _inputs(m, 80, 1000, torch.bfloat16, ignored=0.3)
     g = torch.tensor(2.0, device="cuda")
@@ -416,7 +416,7 @@ def test_second_derivatives_go_native(reduction):
 
 @gpu
 def test_a_graph_that_is_walked_twice():
-    x, w, t, b = _inputs(1100, 80, 500, torch.bfloat16)
+    x, w, t, b = _inputs(1300, 80, 500, torch.bfloat16)
     leaves = [a.clone().requires_grad_() for a in (x, w, b)]
     loss = fh.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
     for g in (1.0, 0.125):
@@ -429,7 +429,7 @@ def test_a_graph_that_is_walked_twice():
 def test_compiled_step_matches():
     f = torch.compile(lambda a, ww, tt, bb: fh.linear_cross_entropy(a, ww, tt, bb), fullgraph=True, backend="aot_eager")
     g = torch.tensor(1.0, device="cuda")
-    for m, v in ((33, 400), (40, 401), (1200, 500), (1100, 700)):  # sizes become symbols; both ways
+    for m, v in ((33, 400), (40, 401), (1300, 500), (1400, 700)):  # sizes become symbols; both ways
         x, w, t, b = _inputs(m, 72, v, torch.bfloat16)
         leaves = [a.clone().requires_grad_() for a in (x, w, b)]
         loss = f(leaves[0], leaves[1], t, leaves[2])
