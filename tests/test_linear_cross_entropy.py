@@ -382,6 +382,28 @@ def test_a_long_batch_over_many_words(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("m", [5, 300, 1100])
+def test_a_weight_beyond_two_billion_elements(m):
+    """Offsets past 2^31 elements: the loss, dx and some rows of dW against FP32 products, to FP32 and bf16 rounding."""
+    k, v = 17000, 131072
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    w = torch.randn(v, k, generator=gen, device="cuda", dtype=torch.bfloat16).mul_(k**-0.5)
+    t = torch.randint(0, v, (m,), generator=gen, device="cuda")
+    t[0], t[1] = v - 1, 0
+    x = torch.randn(m, k, generator=gen, device="cuda").add_(5 * w[t].float()).bfloat16()
+    loss, dx, dw = _step(x, w, t, None, "mean", torch.tensor(float(m), device="cuda"))
+    z = torch.cat([x.float() @ w[i:i + 16384].float().t() for i in range(0, v, 16384)], 1)
+    torch.testing.assert_close(loss, torch.nn.functional.cross_entropy(z, t), rtol=1e-5, atol=1e-5)
+    dz = z.softmax(1)
+    dz[torch.arange(m), t] -= 1
+    want = sum(dz[:, i:i + 16384] @ w[i:i + 16384].float() for i in range(0, v, 16384))
+    assert (dx.float() - want).norm() <= 6e-3 * want.norm()
+    rows = torch.tensor([0, 1, 63, 126322, 126323, 126400, v - 2, v - 1], device="cuda")  # 2^31 / k = 126322.6
+    want = dz[:, rows].t() @ x.float()
+    assert ((dw[rows].float() - want).norm(dim=1) <= 6e-3 * want.norm(dim=1)).all()
+
+
+@gpu
 def test_gradients_against_differences():
     """Central differences in FP32 at h = 2^-6: the third derivatives' h^2 / 6 and u / h a logit stay below 1%."""
     x, w, t, b = _inputs(6, 24, 40, torch.float32, seed=11, ignored=0.2)
