@@ -344,31 +344,31 @@ __device__ __forceinline__ void put_bias(const BiasArgs& a, int c, float sum) {
   else static_cast<typename T::storage*>(a.out)[c] = from_f32<T>(sum);
 }
 
-// Column sums of dz: 64 V columns and every gridDim.y-th sixteen rows a workgroup, a row a wavefront.
+// Column sums of dz: 32 V columns and every gridDim.y-th 32 rows a workgroup, half a wavefront to a row.
 template <typename T>
 __global__ __launch_bounds__(1024) void bias_kernel(BiasArgs a) {
   using S = typename T::storage;
   constexpr int V = kVec<T>;
-  __shared__ float area[16][V][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int first = static_cast<int>(blockIdx.x) * 64 * V, c = first + lane * V;
+  __shared__ float area[32][V][32];
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5;
+  const int first = static_cast<int>(blockIdx.x) * 32 * V, c = first + lane * V;
   const int more = *a.live - a.row0, rows = more < a.rows ? more : a.rows;
   float sums[V] = {};
 #pragma unroll 4
-  for (int row = blockIdx.y * 16 + wave; row < rows; row += gridDim.y * 16) {
+  for (int row = blockIdx.y * 32 + half; row < rows; row += gridDim.y * 32) {
     float f[V];
     to_floats<T>(load_row<T>(static_cast<const S*>(a.dz) + row * a.ld, c, a.cols), f);
 #pragma unroll
     for (int i = 0; i < V; ++i) sums[i] += f[i];
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) area[wave][i][lane] = sums[i];
+  for (int i = 0; i < V; ++i) area[half][i][lane] = sums[i];
   __syncthreads();
   const int mine = static_cast<int>(threadIdx.x), to = first + mine;
-  if (mine >= 64 * V || to >= a.cols) return;
+  if (mine >= 32 * V || to >= a.cols) return;
   float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) sum += area[w][mine % V][mine / V];
+  for (int w = 0; w < 32; ++w) sum += area[w][mine % V][mine / V];
   if (a.partial != nullptr) a.partial[static_cast<int64_t>(blockIdx.y) * a.cols + to] = sum;
   else put_bias<T>(a, to, sum);
 }
@@ -410,7 +410,7 @@ class BiasSums {
     args.partial = partial_ != nullptr ? partial_ + chunk * down_ * args.cols : nullptr;
     return with_type(dtype_, [&](auto t) {
       using T = decltype(t);
-      const int64_t each = 64 * kVec<T>;
+      const int64_t each = 32 * kVec<T>;
       const dim3 grid(static_cast<uint32_t>((args.cols + each - 1) / each), static_cast<uint32_t>(down_));
       bias_kernel<T><<<grid, dim3(1024), 0, stream>>>(args);
       return hipGetLastError();
