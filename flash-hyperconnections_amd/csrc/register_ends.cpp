@@ -11,7 +11,9 @@
 namespace flash_hypercons {
 namespace {
 
-at::Tensor indices_of(const at::Tensor& t) { return t.to(at::kLong).contiguous(); }
+at::Tensor indices_of(const at::Tensor& t) {
+  return (t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous();
+}
 
 bool index_type(const at::Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
 
@@ -261,6 +263,7 @@ class EmbeddingFunction : public torch::autograd::Function<EmbeddingFunction> {
     static const auto op =
         find_op<at::Tensor(const at::Tensor&, const at::Tensor&, c10::SymInt, double, int64_t, int64_t)>(
             "flash_hypercons::_embedding_backward");
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing is recorded: straight to the kernels
     return {{}, op.call(grad, tokens, vocab, scale, streams, padding), {}, {}, {}};
   }
 };
@@ -333,7 +336,10 @@ class LossFunction : public torch::autograd::Function<LossFunction> {
     if (at::GradMode::is_enabled()) {
       const variable_list g = loss_gradients(grads[0], x, weight, targets, bias, ignore, reduction);
       std::tie(dx, dw, db) = std::make_tuple(g[0], g[1], g[2]);
-    } else if (saved.size() > 5) {
+      return {want_x ? dx : at::Tensor(), want_weight ? dw : at::Tensor(), {}, want_bias ? db : at::Tensor(), {}, {}};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing is recorded: straight to the kernels
+    if (saved.size() > 5) {
       static const auto op = find_op<std::tuple<at::Tensor, at::Tensor, at::Tensor>(
           const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
           const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t)>(

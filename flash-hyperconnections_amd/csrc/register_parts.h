@@ -56,7 +56,12 @@ template <typename Call>
 void with_workspace(const at::Tensor& like, Call call) {
   int64_t bytes = 0;
   check_status(call(nullptr, &bytes));
-  const at::Tensor workspace = at::empty({std::max<int64_t>(bytes, 16)}, like.options().dtype(at::kByte));
+  if (bytes == 0) {
+    alignas(16) char none[16];  // any address will do
+    check_status(call(none, &bytes));
+    return;
+  }
+  const at::Tensor workspace = at::empty({bytes}, like.options().dtype(at::kByte));
   check_status(call(workspace.mutable_data_ptr(), &bytes));
 }
 
