@@ -95,6 +95,20 @@ def test_runs_of_any_length(tokens, hot):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [40, 3000, 5000, 20000, 600000])
+def test_vocabularies_of_many_digits(tokens):
+    """Three and four passes of a sort, by one workgroup and by several of one, four and sixteen thousand keys."""
+    for vocab in (3_000_000, 1 << 27 | 1):
+        t = torch.randint(0, vocab, (tokens,), device="cuda")
+        t[: tokens // 3] = t[0]
+        w = torch.arange(vocab, device="cuda").unsqueeze(1).float()
+        g = torch.randint(-8, 9, (tokens, 1), device="cuda").float()  # whole numbers: sums are exact in any order
+        y, dw = _step(t, w, g)
+        assert torch.equal(y, w[t])
+        assert torch.equal(dw, torch.zeros(vocab, 1, device="cuda").index_add_(0, t, g))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_runs_that_end_at_the_borders_of_chunks(dtype):
     for length in (15, 16, 17, 31, 32, 33, 64, 128):

@@ -420,11 +420,12 @@ def test_gradients_against_differences():
 
 
 @gpu
+@pytest.mark.parametrize("m", [7, 140])  # of the gradients formed again, and with the loss
 @pytest.mark.parametrize("reduction", REDUCTIONS)
-def test_second_derivatives_go_native(reduction):
-    x, w, t, b = _inputs(7, 12, 9, torch.float32, ignored=0.3)
+def test_second_derivatives_go_native(reduction, m):
+    x, w, t, b = _inputs(m, 12, 9, torch.float32, ignored=0.3)
     x, w, b = (a.requires_grad_() for a in (x, w, b))
-    g = torch.rand(7 if reduction == "none" else (), device="cuda")
+    g = torch.rand(m if reduction == "none" else (), device="cuda")
 
     def grads(loss):
         d = torch.autograd.grad(loss, (x, w, b), g, create_graph=True)
@@ -434,6 +435,18 @@ def test_second_derivatives_go_native(reduction):
     native = torch.nn.functional.cross_entropy(torch.nn.functional.linear(x, w, b), t, reduction=reduction)
     for a, e in zip(got, grads(native)):
         torch.testing.assert_close(a, e, rtol=1e-4, atol=1e-5)
+
+
+@gpu
+def test_function_transforms_and_tangents_go_native():
+    x, w, t, _ = _inputs(6, 12, 9, torch.float32)
+    loss = lambda a, b: fh.linear_cross_entropy(a, b, t)  # noqa: E731
+    native = lambda a, b: torch.nn.functional.cross_entropy(a @ b.t(), t)  # noqa: E731
+    torch.testing.assert_close(torch.func.grad(loss, (0, 1))(x, w), torch.func.grad(native, (0, 1))(x, w))
+    for a, e in zip(torch.func.jvp(loss, (x, w), (w[:6], w + 1)), torch.func.jvp(native, (x, w), (w[:6], w + 1))):
+        torch.testing.assert_close(a, e)
+    many = torch.func.vmap(lambda a: fh.linear_cross_entropy(a, w, t, reduction="sum"))(torch.stack((x, x + 1)))
+    torch.testing.assert_close(many[1], fh.linear_cross_entropy(x + 1, w, t, reduction="sum"))
 
 
 @gpu
