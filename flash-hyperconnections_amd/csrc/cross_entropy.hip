@@ -38,15 +38,15 @@ struct RowsArgs {
   const int64_t* targets;
   int64_t ignore;
   int rows, vocab;
-  int* live;          // how many rows have a target
+  int* live;          // how many rows have a target; backward: and twice as many
   int* index;         // [rows] which ones, in their order
   int* label;         // [rows] their targets; -1 for one that is out of range
   float* losses;      // forward: [rows] zeroed where there is no target, or null
   // backward
   const float* grad;  // of the loss, or of each row's
   int per_row, mean, scaled;
-  const float* lse;   // [rows] in the order of `index`
-  float2* row;        // [rows] lse and the factor
+  const float2* lse;  // [rows] in the order of `index`: lse and 1 - p of the target
+  float4* row;        // [rows] lse, the factor and p - 1
   float* scale;       // what undoes the factors' power of two
 };
 
@@ -121,13 +121,16 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(RowsArgs a) {
       a.label[at] = valid ? static_cast<int>(t) : -1;
       if constexpr (Backward) {
         const float f = valid ? a.grad[a.per_row ? r : 0] / mean * power : __builtin_nanf("");
-        a.row[at] = make_float2(a.lse[at], f);
+        a.row[at] = make_float4(a.lse[at].x, f, -a.lse[at].y, 0.f);
       }
     } else if (!Backward && r < a.rows && a.losses != nullptr) {
       a.losses[r] = 0.f;
     }
   }
-  if (threadIdx.x == 0) *a.live = done;
+  if (threadIdx.x == 0) {
+    a.live[0] = done;
+    if (Backward) a.live[1] = 2 * done;
+  }
 }
 
 struct GatherArgs {
@@ -136,6 +139,7 @@ struct GatherArgs {
   const int* live;
   const int* index;
   void* out;          // [rows, ld], zero past cols
+  void* twice;        // [2 rows, ld] each row twice, or null
   int64_t ld;
   int cols;
   // Rows of dx without a target are zeroed, unless it is null.
@@ -164,6 +168,10 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
   for (int c = (threadIdx.x & 63) * kVec<T>; c < a.ld; c += 64 * kVec<T>) {
     const U32x4 w = load_row<T>(from, c, a.cols);
     __builtin_memcpy(to + c, &w, 16);
+    if (a.twice != nullptr) {
+      __builtin_memcpy(static_cast<S*>(a.twice) + 2 * row * a.ld + c, &w, 16);
+      __builtin_memcpy(static_cast<S*>(a.twice) + (2 * row + 1) * a.ld + c, &w, 16);
+    }
   }
 }
 
@@ -172,28 +180,33 @@ struct SlopeArgs {
   int64_t ld;
   const float2* stats;  // [groups, stats_ld]
   int64_t stats_ld;
-  const float *lse, *chosen;
+  const float2* lse;    // lse and 1 - p of the target
   const int *live, *label;
   int row0, rows;
+  float* sums;          // [all rows / 64, ld] column sums of each 64 rows, or null
 };
 
 // exp(z - lse) - [target] from exp(z - maximum of its 64): 64 vectors of 64 rows a workgroup, a
-// wavefront to every fourth row.  The target's is formed from its logit, in FP32: 1 - p would
-// show the exponential's rounding where p is close to one.  Bound by memory.
+// wavefront to every fourth row.  The target's is what its logit gave, in FP32: 1 - p would show the
+// exponential's rounding where p is close to one.  Column sums are of what is not rounded yet.  Bound by
+// memory: 8192 rows of 131072 words, 4.3 GB, take 0.79 ms (5.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   using S = typename T::storage;
   using Z = Saved<T>;
   constexpr int V = kVec<T>, kAhead = 4;
+  __shared__ float area[4][V][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = (static_cast<int>(blockIdx.x) * 64 + lane) * V;
   const int more = *a.live - a.row0, rows = more < a.rows ? more : a.rows;
-  if (c >= a.ld) return;
   const float2* stats = a.stats + static_cast<int64_t>(c / 64) * a.stats_ld;
-  const int last = static_cast<int>(blockIdx.y) * 64 + 64 < rows ? static_cast<int>(blockIdx.y) * 64 + 64 : rows;
-  for (int first = blockIdx.y * 64 + wave; first < last; first += 4 * kAhead) {
+  const int start = static_cast<int>(blockIdx.y) * 64, last = start + 64 < rows ? start + 64 : rows;
+  if (start >= rows) return;  // the whole workgroup
+  float sums[V] = {};
+  for (int first = start + wave; c < a.ld && first < last; first += 4 * kAhead) {
     U32x4 raw[kAhead];
-    float top[kAhead], lse[kAhead], chosen[kAhead];
+    float top[kAhead];
+    float2 lse[kAhead];
     int label[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -202,7 +215,6 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
       top[u] = stats[r].x;
       lse[u] = a.lse[r];
       label[u] = a.label[r];
-      chosen[u] = a.chosen[r];
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -210,19 +222,49 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
       float f[V];
       to_floats<Z>(raw[u], f);
       // A target out of range makes its row NaN.
-      const float times = (label[u] < 0 ? __builtin_nanf("") : expf(top[u] - lse[u])) *
+      const float times = (label[u] < 0 ? __builtin_nanf("") : expf(top[u] - lse[u].x)) *
                           (T::code == BF16::code ? 1.f / kKept : 1.f);  // FP16 and FP32 keep their scales
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] *= times;
       const int at = label[u] - c;
       if (at >= 0 && at < V) {
-        const float hit = (expf(chosen[u] - lse[u]) - 1.f) * (T::code == F16::code ? kKept : 1.f);
+        const float hit = -lse[u].y * (T::code == F16::code ? kKept : 1.f);
 #pragma unroll
         for (int k = 0; k < V; ++k) f[k] = k == at ? hit : f[k];
       }
       const U32x4 w = from_floats<T>(f);
       __builtin_memcpy(static_cast<S*>(a.dz) + (first + 4 * u) * a.ld + c, &w, 16);
+#pragma unroll
+      for (int k = 0; k < V; ++k) sums[k] += f[k];
     }
+  }
+  if (a.sums == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < V; ++k) area[wave][k][lane] = sums[k];
+  __syncthreads();
+  float* to = a.sums + (a.row0 / 64 + static_cast<int64_t>(blockIdx.y)) * a.ld + static_cast<int64_t>(blockIdx.x) * 64 * V;
+  for (int i = threadIdx.x; i < 64 * V && static_cast<int>(blockIdx.x) * 64 * V + i < a.ld; i += 256)
+    to[i] = ((area[0][i % V][i / V] + area[1][i % V][i / V]) + area[2][i % V][i / V]) + area[3][i % V][i / V];
+}
+
+// out[index[i]] = (sums[2 i] + sums[2 i + 1]) scale: rows in two parts.
+template <typename T>
+__global__ __launch_bounds__(256) void parts_kernel(const float* sums, const int* live, const int* index,
+                                                    const float* scale, int cols, void* out) {
+  constexpr int V = 8;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= *live) return;
+  const float* from = sums + 2 * row * cols;
+  auto* to = static_cast<typename T::storage*>(out) + static_cast<int64_t>(index[row]) * cols;
+  for (int c = (threadIdx.x & 63) * V; c < cols; c += 64 * V) {
+    float f[V], g[V];
+    load_some(from + c, cols - c, f);
+    load_some(from + cols + c, cols - c, g);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = (f[k] + g[k]) * *scale;
+    typename T::storage e[V];
+    round_some<T>(f, e);
+    store_some(e, to + c, cols - c);
   }
 }
 
@@ -274,8 +316,8 @@ struct LseArgs {
   int row0;
   const int* label;
   const int* index;
-  const float* chosen;
-  float* lse;           // [rows] in the order of `index`
+  const float *chosen, *rest;
+  float2* lse;          // [rows] in the order of `index`: lse and 1 - p of the target
   float* losses;        // likewise, or by their rows
   int by_row;
 };
@@ -292,10 +334,14 @@ __global__ __launch_bounds__(1024) void lse_kernel(LseArgs a, int across) {
   const int live = *a.live - a.row0, rows = live < a.rows ? live : a.rows;
   const int row = static_cast<int>(blockIdx.x) * across + (threadIdx.x & (across - 1));
   if (static_cast<int>(blockIdx.x) * across >= rows) return;  // the whole workgroup
-  float2 sum = make_float2(-__builtin_inff(), 0.f);
+  float2 sum = make_float2(-__builtin_inff(), 0.f);  // of all but the target
+  const int label = row < rows ? a.label[row] : -1;
   if (row < rows) {
-    for (int g = threadIdx.x / across; g < a.groups; g += 1024 / across)
-      sum = join(sum, a.stats[static_cast<int64_t>(g) * a.ld + row]);
+    for (int g = threadIdx.x / across; g < a.groups; g += 1024 / across) {
+      float2 part = a.stats[static_cast<int64_t>(g) * a.ld + row];
+      if (label >= 0 && g == label / 64) part.y = a.rest[row];
+      sum = join(sum, part);
+    }
   }
   area[threadIdx.x] = sum;
   for (int d = 512; d >= across; d >>= 1) {
@@ -303,11 +349,13 @@ __global__ __launch_bounds__(1024) void lse_kernel(LseArgs a, int across) {
     if (static_cast<int>(threadIdx.x) < d) area[threadIdx.x] = sum = join(sum, area[threadIdx.x + d]);
   }
   if (static_cast<int>(threadIdx.x) < across && row < rows) {
-    const float log_sum = logf(sum.y);
-    a.lse[row] = sum.x + log_sum;
-    // In this order a loss close to zero keeps its digits: the target is then the maximum.
-    const float loss = a.label[row] >= 0 ? (sum.x - a.chosen[row]) + log_sum : __builtin_nanf("");
-    a.losses[a.by_row ? a.index[row] : row] = loss;
+    const float chosen = label >= 0 ? a.chosen[row] : -__builtin_inff();
+    const float below = sum.x - chosen;  // how far the target is below the maximum
+    const float all = sum.y + (label >= 0 ? expf(chosen - sum.x) : 0.f), log_all = logf(all);
+    a.lse[row] = make_float2(sum.x + log_all, sum.y / all);
+    // A loss close to zero keeps its digits as the logarithm of one more than the others' share.
+    const float loss = below < 16.f ? log1pf(sum.y * expf(below)) : below + log_all;
+    a.losses[a.by_row ? a.index[row] : row] = label >= 0 ? loss : __builtin_nanf("");
   }
 }
 
@@ -384,6 +432,16 @@ __global__ __launch_bounds__(256) void join_bias_kernel(BiasArgs a, int count) {
   put_bias<T>(a, c, sum);
 }
 
+// Column sums from those of each 64 rows, as far as rows are live.
+__global__ __launch_bounds__(256) void join_rows_kernel(const float* parts, const int* live, int ld, int cols, float* out) {
+  const int c = blockIdx.x * 256 + threadIdx.x, count = (*live + 63) / 64;
+  if (c >= cols) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) sum += parts[static_cast<int64_t>(i) * ld + c];
+  out[c] = sum;
+}
+
 int element(int dtype) { return dtype == F32::code ? 4 : 2; }
 
 char* bytes_on(const void* p, int64_t bytes) {
@@ -436,21 +494,22 @@ class BiasSums {
 // The rows with a target and x's rows of them.
 struct Rows {
   int *live, *index, *label;
-  Laid x;
+  Laid x, twice;  // and each row of x twice
 };
 
-hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, Workspace& ws, Rows& got, hipStream_t stream) {
+hipError_t gather(const LossArgs& a, RowsArgs r, bool backward, bool twice, Workspace& ws, Rows& got, hipStream_t stream) {
   const int64_t v = a.dtype == F32::code ? 4 : 8, ld = (a.cols + v - 1) / v * v;
   r.targets = a.targets;
   r.ignore = a.ignore;
   r.rows = static_cast<int>(a.rows);
   r.vocab = static_cast<int>(a.vocab);
-  r.live = got.live = a.places != nullptr ? a.places : ws.take<int>(1);
+  r.live = got.live = a.places != nullptr ? a.places : ws.take<int>(2);
   r.index = got.index = a.places != nullptr ? a.places + 1 : ws.take<int>(a.rows);
   r.label = got.label = ws.take<int>(a.rows);
-  GatherArgs g{a.x, a.x_stride, got.live, got.index, ws.take<char>(a.rows * ld * element(a.dtype)), ld,
-               static_cast<int>(a.cols), a.targets, a.ignore, a.rows, backward ? a.dx : nullptr};
+  GatherArgs g{a.x, a.x_stride, got.live, got.index, ws.take<char>(a.rows * ld * element(a.dtype)),
+               twice ? ws.take<char>(2 * a.rows * ld * element(a.dtype)) : nullptr, ld, static_cast<int>(a.cols), a.targets, a.ignore, a.rows, backward ? a.dx : nullptr};
   got.x = {g.out, ld};
+  got.twice = {g.twice, ld};
   if (ws.dry()) return hipSuccess;
   if (backward) rows_kernel<true><<<dim3(1), dim3(kRowThreads), 0, stream>>>(r);
   else rows_kernel<false><<<dim3(1), dim3(kRowThreads), 0, stream>>>(r);
@@ -504,6 +563,7 @@ int lse_rows(int64_t rows) {
   return across;
 }
 
+constexpr int64_t kTwoParts = 64;  // rows
 constexpr int64_t kStats = int64_t{1} << 25;  // maxima and sums at a time: 256 MB
 // Bytes of exponentials or dz at a time.  Half as many take 1 ms more of 44.7 for 16384 x 4096 into 131072 words: dW's
 // sum is read and written for each chunk.
@@ -517,7 +577,7 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
   RowsArgs r{};
   r.losses = by_row ? a.loss : nullptr;
   Rows rows;
-  hipError_t err = gather(a, r, false, ws, rows, stream);
+  hipError_t err = gather(a, r, false, false, ws, rows, stream);
   Laid w;
   if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
   const int64_t groups = (a.vocab + 63) / 64;
@@ -525,6 +585,7 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
                                          std::max<int64_t>(256, kStats / groups / 256 * 256));
   auto* stats = ws.take<float2>(groups * most);
   auto* chosen = ws.take<float>(most);
+  auto* rest = ws.take<float>(most);
   float* losses = by_row ? a.loss : ws.take<float>(a.rows);
   const int across = lse_rows(a.rows);
   if (err == hipSuccess) {
@@ -533,10 +594,11 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
       p.loss.stats = stats;
       p.loss.stats_ld = most;
       p.loss.chosen = chosen;
+      p.loss.rest = rest;
       const hipError_t e = multiply(p, rows_from(rows.x, row0, a.dtype), w, a.dtype, false, false, Finish::kStats, ws, stream);
       if (e != hipSuccess || ws.dry()) return e;
       const LseArgs l{stats, most, static_cast<int>(groups), static_cast<int>(count), rows.live, static_cast<int>(row0),
-                      rows.label + row0, rows.index + row0, chosen, a.lse + row0, by_row ? losses : losses + row0, by_row};
+                      rows.label + row0, rows.index + row0, chosen, rest, static_cast<float2*>(a.lse) + row0, by_row ? losses : losses + row0, by_row};
       lse_kernel<<<blocks_of(count, across), dim3(1024), 0, stream>>>(l, across);
       return hipGetLastError();
     });
@@ -552,7 +614,7 @@ hipError_t launch_cross_entropy(const LossArgs& a, void* workspace, int64_t* byt
 hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
   Workspace ws(workspace);
   Rows rows;
-  hipError_t err = gather(a, RowsArgs{}, false, ws, rows, stream);
+  hipError_t err = gather(a, RowsArgs{}, false, false, ws, rows, stream);
   Laid w;
   if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
   if (err != hipSuccess) return err;
@@ -562,15 +624,11 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
       std::max<int64_t>(256, std::min<int64_t>(kStats / groups, kPiece / (ld * element(a.dtype))) / 256 * 256));
   auto* stats = ws.take<float2>(groups * most);
   auto* chosen = ws.take<float>(most);
-  auto* lse = ws.take<float>(a.rows);
+  auto* rest = ws.take<float>(most);
+  auto* lse = ws.take<float2>(most);
   auto* losses = ws.take<float>(a.rows);
   const Laid dz{ws.take<char>(most * ld * element(a.dtype)), ld};
-  const BiasSums db(a.db_sums != nullptr, (a.rows + most - 1) / most, most, a.vocab, a.dtype, ws);
-  BiasArgs db_args{};
-  db_args.cols = static_cast<int>(a.vocab);
-  db_args.live = rows.live;
-  db_args.out = a.db_sums;
-  db_args.out_f32 = 1;
+  auto* db_parts = a.db_sums != nullptr ? ws.take<float>((a.rows + 63) / 64 * ld) : nullptr;
   const int64_t before = ws.used();
   int64_t most_used = before;
   // Products follow one another on the stream, and share the space for what their slices add up to.
@@ -586,23 +644,23 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
     p.loss.stats = stats;
     p.loss.stats_ld = most;
     p.loss.chosen = chosen;
+    p.loss.rest = rest;
     p.loss.ld = ld;
     p.out = const_cast<void*>(dz.data);
     hipError_t e = multiply_next(p, x, w, false, false, Finish::kExp);
     if (e == hipSuccess && !ws.dry()) {
       const int across = lse_rows(count);
       const LseArgs l{stats, most, static_cast<int>(groups), static_cast<int>(count), rows.live, static_cast<int>(row0),
-                      rows.label + row0, rows.index + row0, chosen, lse + row0, losses + row0, 0};
+                      rows.label + row0, rows.index + row0, chosen, rest, lse, losses + row0, 0};
       lse_kernel<<<blocks_of(count, across), dim3(1024), 0, stream>>>(l, across);
-      const SlopeArgs s{const_cast<void*>(dz.data), ld, stats, most, lse + row0, chosen, rows.live, rows.label + row0,
-                        static_cast<int>(row0), static_cast<int>(count)};
+      const SlopeArgs s{const_cast<void*>(dz.data), ld, stats, most, lse, rows.live, rows.label + row0,
+                        static_cast<int>(row0), static_cast<int>(count), db_parts};
       e = with_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         const dim3 grid(blocks_of(ld, 64 * kVec<T>).x, blocks_of(count, 64).x);
         slope_kernel<T><<<grid, dim3(256), 0, stream>>>(s);
         return hipGetLastError();
       });
-      if (e == hipSuccess && a.db_sums != nullptr) e = db.add(db_args, dz, row0, count, stream);
     }
     LossProductArgs s{};
     s.loss.live = rows.live;
@@ -628,8 +686,10 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   });
   if (err == hipSuccess && !ws.dry()) {
     loss_kernel<<<dim3(1), dim3(1024), 0, stream>>>(losses, rows.live, a.reduction == FH_REDUCE_MEAN, a.loss);
+    if (a.db_sums != nullptr)
+      join_rows_kernel<<<blocks_of(a.vocab, 256), dim3(256), 0, stream>>>(db_parts, rows.live, static_cast<int>(ld),
+                                                                         static_cast<int>(a.vocab), a.db_sums);
     err = hipGetLastError();
-    if (err == hipSuccess && a.db_sums != nullptr) err = db.join(db_args, stream);
   }
   if (bytes != nullptr) *bytes = most_used;
   return err;
@@ -664,16 +724,19 @@ hipError_t launch_cross_entropy_scale(const LossArgs& a, hipStream_t stream) {
 
 hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int64_t* bytes, hipStream_t stream) {
   Workspace ws(workspace);
+  // Few rows' gradients in two parts of 16 bits each, for as many rows more: the products are bound by reading the
+  // weight and writing its gradient.
+  const int parts = a.dtype != F32::code && a.rows <= kTwoParts ? 2 : 1;
   RowsArgs r{};
   r.grad = a.grad;
   r.per_row = a.reduction == FH_REDUCE_NONE;
   r.mean = a.reduction == FH_REDUCE_MEAN;
   r.scaled = a.dtype == F16::code;
-  r.lse = a.lse;
-  r.row = ws.take<float2>(a.rows);
+  r.lse = static_cast<const float2*>(a.lse);
+  r.row = ws.take<float4>(a.rows);
   r.scale = ws.take<float>(1);
   Rows rows;
-  hipError_t err = gather(a, r, true, ws, rows, stream);
+  hipError_t err = gather(a, r, true, parts == 2 && a.dweight != nullptr, ws, rows, stream);
   Laid w;
   if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
   if (err != hipSuccess) return err;
@@ -685,10 +748,10 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
   const int64_t pieces = (a.vocab + piece - 1) / piece;
   piece = std::min<int64_t>(a.vocab, ((a.vocab + pieces - 1) / pieces + 255) / 256 * 256);
   const int64_t ld = (piece + 7) / 8 * 8, chunks = (a.rows + most_rows - 1) / most_rows;
-  const Laid dz{ws.take<char>(most_rows * ld * es), ld};
-  auto* dx_sums = a.dx != nullptr && piece < a.vocab ? ws.take<float>(a.rows * a.cols) : nullptr;
+  const Laid dz{ws.take<char>(parts * most_rows * ld * es), ld};
+  auto* dx_sums = a.dx != nullptr && (parts == 2 || piece < a.vocab) ? ws.take<float>(parts * a.rows * a.cols) : nullptr;
   auto* dw_sums = a.dweight != nullptr && chunks > 1 ? ws.take<float>(piece * a.cols) : nullptr;
-  const BiasSums db(a.dbias != nullptr, chunks, most_rows, piece, a.dtype, ws);
+  const BiasSums db(a.dbias != nullptr, chunks, parts * most_rows, piece, a.dtype, ws);
   // Products follow one another on the stream, and share the space for what their slices add up to.
   const int64_t before = ws.used();
   int64_t most_used = before;
@@ -703,7 +766,7 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
       const Laid wp = rows_from(w, col0, a.dtype);
       BiasArgs db_args{};
       db_args.cols = static_cast<int>(outs);
-      db_args.live = rows.live;
+      db_args.live = rows.live + (parts - 1);
       db_args.scale = r.scale;
       db_args.out = bytes_on(a.dbias, col0 * element(a.bias_dtype));
       db_args.out_f32 = a.bias_dtype == F32::code;
@@ -712,24 +775,25 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
         hipError_t e = shared([&](Workspace& part) {
           LossProductArgs p = logits(a, rows, row0, count, col0, outs);
           p.loss.row = r.row + row0;
+          p.loss.parts = parts;
           p.loss.ld = (outs + 7) / 8 * 8;
           p.out = const_cast<void*>(dz.data);
           return multiply(p, xp, wp, a.dtype, false, false, Finish::kSlope, part, stream);
         });
         const Laid d{dz.data, (outs + 7) / 8 * 8};
         LossProductArgs s{};
-        s.loss.live = rows.live;
+        s.loss.live = rows.live + (parts - 1);  // two parts: twice the rows
         s.loss.row0 = static_cast<int>(row0);
         s.loss.scale = r.scale;
         if (e == hipSuccess && a.dx != nullptr) {
           e = shared([&](Workspace& part) {
             LossProductArgs p = s;
-            p.m = static_cast<int>(count);
+            p.m = static_cast<int>(parts * count);
             p.n = static_cast<int>(a.cols);
             p.k = static_cast<int>(outs);
             p.loss.sums = dx_sums != nullptr ? dx_sums + row0 * a.cols : nullptr;
             p.loss.first = col0 == 0;
-            p.loss.last = col0 + outs == a.vocab;
+            p.loss.last = parts == 1 && col0 + outs == a.vocab;
             p.loss.index = rows.index + row0;
             p.out = a.dx;
             return multiply(p, d, wp, a.dtype, false, true, Finish::kSum, part, stream);
@@ -740,18 +804,25 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
             LossProductArgs p = s;
             p.m = static_cast<int>(outs);
             p.n = static_cast<int>(a.cols);
-            p.k = static_cast<int>(count);
+            p.k = static_cast<int>(parts * count);
             p.loss.sums = dw_sums;
             p.loss.first = row0 == 0;
             p.loss.last = row0 + count == a.rows;
             p.out = bytes_on(a.dweight, col0 * a.cols * es);
-            return multiply(p, d, xp, a.dtype, true, true, Finish::kSum, part, stream);
+            return multiply(p, d, parts == 2 ? rows.twice : xp, a.dtype, true, true, Finish::kSum, part, stream);
           });
         }
-        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) e = db.add(db_args, d, row0, count, stream);
+        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) e = db.add(db_args, d, row0, parts * count, stream);
         return e;
       });
       return all != hipSuccess || a.dbias == nullptr || ws.dry() ? all : db.join(db_args, stream);
+    });
+  }
+  if (err == hipSuccess && a.dx != nullptr && parts == 2 && !ws.dry()) {
+    err = with_half_type(a.dtype, [&](auto t) {
+      parts_kernel<decltype(t)><<<blocks_of(a.rows, 4), dim3(256), 0, stream>>>(
+          dx_sums, rows.live, rows.index, r.scale, static_cast<int>(a.cols), a.dx);
+      return hipGetLastError();
     });
   }
   if (bytes != nullptr) *bytes = most_used;

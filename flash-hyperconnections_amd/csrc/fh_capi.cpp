@@ -268,7 +268,7 @@ int validate_loss(const fh::LossArgs& a) {
   if (a.reduction < FH_REDUCE_NONE || a.reduction > FH_REDUCE_MEAN)
     return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: unknown reduction");
   if (a.rows > 0 && (!rows_ok(a.x, a.x_stride, a.dtype) || !rows_ok(a.weight, a.w_stride, a.dtype) ||
-                     a.targets == nullptr || !aligned(a.targets, 8) || !aligned(a.lse, 4) ||
+                     a.targets == nullptr || !aligned(a.targets, 8) || !aligned(a.lse, 8) ||
                      (a.lse == nullptr && a.places == nullptr) ||
                      (a.bias != nullptr && !aligned(a.bias, element_size(a.bias_dtype)))))
     return fail(FH_ERR_INVALID_ARGUMENT, "linear_cross_entropy: null or misaligned pointer, or negative stride");
@@ -730,8 +730,8 @@ int fh_linear_cross_entropy_scale(const float* grad, const int64_t* targets, int
                                   void* dx, void* dweight, void* dbias, int bias_dtype, int dtype, int64_t rows,
                                   int64_t cols, int64_t vocab, hipStream_t stream) {
   // x and the weight have been read: their place is taken by what is there.
-  fh::LossArgs a = loss_args(grad, 0, grad, 0, nullptr, bias_dtype, targets, ignore, reduction, grad, dtype, rows, cols,
-                             vocab);
+  fh::LossArgs a = loss_args(grad, 0, grad, 0, nullptr, bias_dtype, targets, ignore, reduction, nullptr, dtype, rows,
+                             cols, vocab);
   a.grad = grad;
   a.places = const_cast<int*>(places);
   a.dx_sums = const_cast<float*>(dx_sums);

@@ -130,7 +130,7 @@ struct LossArgs {
   int64_t ignore;
   int reduction;
   float* loss;            // forward: one, or [rows]
-  float* lse;             // [rows], for the backward
+  void* lse;              // float [rows, 2], for the backward
   const float* grad;      // backward: one, or [rows]
   void *dx, *dweight, *dbias;  // contiguous; each may be null
   // Ahead: [1 + rows] how many rows have a target and which; the gradients for an upstream gradient of one,

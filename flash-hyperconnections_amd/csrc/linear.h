@@ -17,7 +17,8 @@ typedef float Floats4 __attribute__((ext_vector_type(4)));
 // statistics of logits, which are not kept; these and the logits' exponentials; the logits'
 // gradients; or a sum that goes on from another product's and is scaled at its end.
 enum class Finish { kLinear, kStats, kExp, kSlope, kSum };
-constexpr bool whole_sums(Finish f) { return f == Finish::kStats || f == Finish::kExp || f == Finish::kSlope; }
+// Those that go by whole rows of 64 logits.
+constexpr bool of_logits(Finish f) { return f == Finish::kStats || f == Finish::kExp || f == Finish::kSlope; }
 
 // What the others need beside the product.  Their rows are the first *live ones from
 // row0 on (of the sum where A is in columns), as many as there are targets.
@@ -28,8 +29,9 @@ struct LossParts {
   int col0;              // the vocabulary's entry of column 0
   float2* stats;         // kStats, kExp: [columns / 64, rows] maximum and sum of exponentials, groups stats_ld apart
   int64_t stats_ld;
-  float* chosen;         // kStats, kExp: [rows] logits of the targets
-  const float2* row;     // kSlope: [rows] the logarithm of the row's sum, and the factor of its gradient
+  float *chosen, *rest;  // kStats, kExp: [rows] logits of the targets, and the sums of their 64 without them
+  const float4* row;     // kSlope: [rows] the logarithm of the row's sum, the factor of its gradient, and p - 1 of its target
+  int parts;             // kSlope: 2 for dz in two parts, in rows next to each other
   int64_t ld;            // kExp, kSlope: rows of out, whole vectors, zero past n
   float* sums;           // kSum: [m, n] of the sum so far
   int first, last;       // kSum: whether sums is not read, or not written but scaled into out
@@ -99,7 +101,8 @@ __device__ __forceinline__ bool fit(ArgsOf<F>& p) {
         p.slices = slices > p.slices ? slices : p.slices;
       }
     }
-    return blockIdx.x + gridDim.x * blockIdx.y < static_cast<uint32_t>(tiles * p.slices);
+    if constexpr (F == Finish::kSum) return blockIdx.x + gridDim.x * blockIdx.y < static_cast<uint32_t>(tiles * p.slices);
+    return blockIdx.x < static_cast<uint32_t>(tiles);
   } else {
     fit_live<F, ACols>(p);
     if constexpr (F == Finish::kSum) return p.k > 0 || p.loss.first || p.loss.last;  // or nothing is added
@@ -312,10 +315,13 @@ struct RowOf<Finish::kExp> : RowOf<Finish::kStats> {};
 template <>
 struct RowOf<Finish::kSlope> {
   int label;
-  float2 row;
+  float lse, factor, hit;
   __device__ __forceinline__ void load(const LossProductArgs& p, int i) {
+    const float4 row = i < p.m ? p.loss.row[i] : make_float4(0.f, 0.f, 0.f, 0.f);
     label = i < p.m ? p.loss.label[i] - p.loss.col0 : 0;
-    row = i < p.m ? p.loss.row[i] : make_float2(0.f, 0.f);
+    lse = row.x;
+    factor = row.y;
+    hit = row.z;
   }
 };
 
@@ -364,13 +370,26 @@ __device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf
     v[k] = exp_from<T>(v[k], from);
     s += v[k];
   }
+  const int inside = of.label - (j & ~63);
+  if (inside >= 0 && inside < 64) {  // the same in all of these lanes
+    float rest = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) rest += k == at ? 0.f : v[k];
+    rest = over_lanes<Lanes>(rest, [](float a, float b) { return a + b; });
+    if (j % 64 == 0) p.loss.rest[i] = rest;
+  }
   if (F == Finish::kExp && j < p.loss.ld) {
     using Z = Saved<T>;
-    typename Z::storage e[V];
+    auto* to = static_cast<typename Z::storage*>(p.out) + static_cast<int64_t>(i) * p.loss.ld + j;
+    if constexpr (T::code == F32::code) {
+      __builtin_memcpy(to, v, sizeof(v));
+    } else {
+      typename Z::storage e[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= T::code == F32::code ? 1.f : kKept;
-    round_some<Z>(v, e);
-    store_some(e, static_cast<typename Z::storage*>(p.out) + static_cast<int64_t>(i) * p.loss.ld + j, V);
+      for (int k = 0; k < V; ++k) v[k] *= kKept;
+      round_some<Z>(v, e);
+      store_some(e, to, V);
+    }
   }
   s = over_lanes<Lanes>(s, [](float a, float b) { return a + b; });
   if (j % 64 == 0 && left > 0) p.loss.stats[static_cast<int64_t>(j / 64) * p.loss.stats_ld + i] = make_float2(m, s);
@@ -378,7 +397,8 @@ __device__ __forceinline__ void stats_some(const LossProductArgs& p, const RowOf
 
 // Logits on their way to the gradients of z: (exp(z - lse) - [target]) times the row's
 // factor, rounded to the storage type, which the products that follow take.  (Root mean
-// square 0.0017 of a term in bf16, beside as much for their results' own rounding.)
+// square 0.0017 of a term in bf16, beside as much for their results' own rounding.  Of few rows
+// one term makes most of a result, which may then be off by 2^-9: those come in two parts.)
 template <typename T, int V>
 __device__ __forceinline__ void slope_some(const LossProductArgs& p, const RowOf<Finish::kSlope>& of, int i, int j,
                                            float (&v)[V]) {
@@ -387,20 +407,28 @@ __device__ __forceinline__ void slope_some(const LossProductArgs& p, const RowOf
   const int left = p.n - j, at = of.label - j;
   if (left > 0) add_bias<T>(p, j, left, v);
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = exp_from<T>(v[k], of.row.x);
+  for (int k = 0; k < V; ++k) v[k] = exp_from<T>(v[k], of.lse);
   if (at >= 0 && at < V) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] -= k == at ? 1.f : 0.f;
+    for (int k = 0; k < V; ++k) v[k] = k == at ? of.hit : v[k];
   }
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] *= of.row.y;
+  for (int k = 0; k < V; ++k) v[k] *= of.factor;
   if (left < V) {
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = k < left ? v[k] : 0.f;
   }
   S e[V];
   round_some<T>(v, e);
-  __builtin_memcpy(static_cast<S*>(p.out) + static_cast<int64_t>(i) * p.loss.ld + j, e, sizeof(e));
+  S* to = static_cast<S*>(p.out) + static_cast<int64_t>(i) * p.loss.parts * p.loss.ld + j;
+  __builtin_memcpy(to, e, sizeof(e));
+  if (T::code != F32::code && p.loss.parts == 2) {
+    // What the first part leaves out, in the next row.
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] -= to_f32<T>(e[k]);
+    round_some<T>(v, e);
+    __builtin_memcpy(to + p.loss.ld, e, sizeof(e));
+  }
 }
 
 // V results of a sum on their way into the sum so far, or at its end scaled and out.
@@ -428,28 +456,35 @@ __device__ __forceinline__ void sum_some(const LossProductArgs& p, int i, int j,
   store_some(e, static_cast<S*>(p.out) + row * p.n + j, left);
 }
 
-// V neighbouring results (row i, columns j .. j + V - 1) on their way out: bias,
-// activation, residual; or into the slice's partial sums.  Lanes neighbouring lanes have
-// the results beside these.
+// V neighbouring results (row i, columns j .. j + V - 1) into the slice's partial sums.
+template <int V>
+__device__ __forceinline__ void keep_some(const ProductArgs& p, int slice, int i, int j, const float (&v)[V]) {
+  if (i < p.m && j < p.n)
+    store_some<true>(v, p.partial + (static_cast<int64_t>(slice) * p.m + i) * p.n + j, p.n - j);
+}
+
+// The same on their way out: bias, activation, residual; or into the slice's partial sums, but
+// for finishes of logits, which are whole sums here.  Lanes neighbouring lanes have the results
+// beside these.
 template <typename T, Finish F, int Lanes, int V>
 __device__ __forceinline__ void finish_some(const ArgsOf<F>& p, const RowOf<F>& of, int slice, int i, int j,
                                             float (&v)[V]) {
   using S = typename T::storage;
   using Z = Saved<T>;
-  if constexpr (F == Finish::kStats || F == Finish::kExp) {
-    stats_some<T, F, Lanes>(p, of, i, j, v);
-    return;
-  } else if constexpr (F == Finish::kSlope) {
+  if constexpr (F == Finish::kSlope) {
     slope_some<T>(p, of, i, j, v);
+    return;
+  } else if constexpr (of_logits(F)) {
+    stats_some<T, F, Lanes>(p, of, i, j, v);
     return;
   }
   if (i >= p.m || j >= p.n) return;
-  const int64_t at = static_cast<int64_t>(i) * p.n + j;
-  const int left = p.n - j;
   if (p.slices > 1) {
-    store_some<true>(v, p.partial + static_cast<int64_t>(slice) * p.m * p.n + at, left);
+    keep_some(p, slice, i, j, v);
     return;
   }
+  const int64_t at = static_cast<int64_t>(i) * p.n + j;
+  const int left = p.n - j;
   if constexpr (F == Finish::kSum) {
     sum_some<T>(p, i, j, v);
     return;
@@ -517,6 +552,20 @@ __device__ __forceinline__ void finish_parked(const ArgsOf<F>& p, int slice, con
   }
   constexpr int down = T::code == F32::code ? 4 : 8, turns = Rows / down;  // rows at a time
   const int first = T::code == F32::code ? lane >> 4 : lane >> 3;
+  if constexpr (of_logits(F)) {
+    if (p.slices > 1) {
+      asm volatile("" ::: "memory");
+#pragma unroll 2
+      for (int it = 0; it < Rows / 4; ++it) {
+        const int r = 4 * it + (lane >> 4), c = lane & 15;
+        float v[4];
+        __builtin_memcpy(v, area + r * 256 + ((c ^ (r & 15)) << 4), 16);
+        keep_some(p, slice, row + r, col + 4 * c, v);
+      }
+      asm volatile("" ::: "memory");
+      return;
+    }
+  }
   RowOf<F> of[turns];
 #pragma unroll
   for (int it = 0; it < turns; ++it) of[it].load(p, row + first + down * it);
@@ -536,7 +585,7 @@ __device__ __forceinline__ void finish_parked(const ArgsOf<F>& p, int slice, con
       finish_some<T, F, 8>(p, of[it], slice, row + r, col + 8 * (lane & 7), v);
     }
   };
-  if constexpr (whole_sums(F)) {
+  if constexpr (of_logits(F)) {
 #pragma unroll
     for (int it = 0; it < turns; ++it) turn(it);
   } else {
@@ -627,12 +676,11 @@ __device__ __forceinline__ void wait_loads() {
 constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16-bit tile within 2^31 bytes
 
 // Sets tiles and slices of a product; a sum in several slices needs slices * m * n
-// floats.  `dtype` is the operands' and the output's; some finishes need whole
-// sums, in one slice.
+// floats.  `dtype` is the operands' and the output's.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
 // vectors; false for others.  Not for Finish::kExp.
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices);
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 // `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
                           Finish finish = Finish::kLinear, const LossParts* loss = nullptr);

@@ -289,8 +289,6 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ArgsOf<F> p) {
     }
   } else {
     const int m = threadIdx.x / groups, n = threadIdx.x % groups * 8;
-    RowOf<F> of;
-    of.load(p, (LongA ? first : 0) + m);
     __syncthreads();
     static_assert(groups * down == 256, "one group of results a thread");
     float v[8], w[8];
@@ -301,13 +299,20 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ArgsOf<F> p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
-    finish_some<T, F, groups>(p, of, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+    const int i = (LongA ? first : 0) + m, j = (LongA ? 0 : first) + n;
+    if (of_logits(F) && p.slices > 1) {
+      keep_some(p, slice, i, j, v);
+    } else {
+      RowOf<F> of;
+      of.load(p, i);
+      finish_some<T, F, groups>(p, of, slice, i, j, v);
+    }
   }
 }
 
 }  // namespace
 
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, int most_slices) {
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols) {
   if (p.m > kShort && p.n > kShort) return false;
   const bool f32 = dtype == F32::code;
   if (f32) {
@@ -328,9 +333,8 @@ bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, in
   // Slices of at least four strips a wavefront until every compute unit has a workgroup; in
   // columns of 16 bits three for each (dW of 16384 x 16384 into 16: 149 us with 4 slices, 90
   // with 12); FP32 one (dx of 1 x 4096 x 16384: 69 us, with three 83).
-  const int64_t slices =
-      std::min<int64_t>((compute_units() * (cols && !f32 ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16));
-  p.slices = most_slices == 1 ? 1 : static_cast<int>(std::max<int64_t>(1, slices));
+  p.slices = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>((compute_units() * (cols && !f32 ? 3 : 1) + tiles - 1) / tiles, steps / (cols ? 4 : 16))));
   return true;
 }
 

@@ -245,11 +245,14 @@ template <typename T, Finish F>
 __global__ __launch_bounds__(256) void join_kernel(ArgsOf<F> p, bool a_cols) {
   if (a_cols) {
     if (!fit<F, true>(p)) return;
-  } else {
+  } else if constexpr (F == Finish::kSum) {
     (void)fit<F, false>(p);
     if (p.slices == 1) return;  // the products' workgroups finished
+  } else {
+    fit_live<F, false>(p);
   }
-  const int across = (p.n + 7) / 8, slices = p.slices;
+  // Eight neighbouring lanes have 64 logits of a row.
+  const int across = of_logits(F) ? (p.n + 63) / 64 * 8 : (p.n + 7) / 8, slices = p.slices;
   const int64_t total = static_cast<int64_t>(p.m) * across, size = static_cast<int64_t>(p.m) * p.n;
   p.slices = 1;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < total;
@@ -258,11 +261,15 @@ __global__ __launch_bounds__(256) void join_kernel(ArgsOf<F> p, bool a_cols) {
     float sum[8] = {};
     const float* from = p.partial + static_cast<int64_t>(row) * p.n + col;
     const int left = p.n - col;
-    for (int s = 8; s <= slices; s += 8) add_slices<8>(from, size, left, sum);
-    if (slices & 4) add_slices<4>(from, size, left, sum);
-    if (slices & 2) add_slices<2>(from, size, left, sum);
-    if (slices & 1) add_slices<1>(from, size, left, sum);
-    finish_some<T, F, 1>(p, RowOf<F>{}, 0, row, col, sum);
+    if (!of_logits(F) || left > 0) {
+      for (int s = 8; s <= slices; s += 8) add_slices<8>(from, size, left, sum);
+      if (slices & 4) add_slices<4>(from, size, left, sum);
+      if (slices & 2) add_slices<2>(from, size, left, sum);
+      if (slices & 1) add_slices<1>(from, size, left, sum);
+    }
+    RowOf<F> of;
+    of.load(p, row);
+    finish_some<T, F, 8>(p, of, 0, row, col, sum);
   }
 }
 
@@ -284,11 +291,17 @@ hipError_t run(const ProductArgs& p, bool a_cols, bool b_cols, Finish finish, co
 
 template <typename T>
 hipError_t join(const ProductArgs& p, bool a_cols, Finish finish, const LossParts* loss, hipStream_t stream) {
-  const int64_t groups = static_cast<int64_t>(p.m) * ((p.n + 7) / 8);
+  const int64_t groups = static_cast<int64_t>(p.m) * ((p.n + 63) / 64 * 8);
   const dim3 grid(static_cast<uint32_t>(std::min<int64_t>((groups + 255) / 256, 4096))), block(256);
-  if (finish == Finish::kSum) join_kernel<T, Finish::kSum><<<grid, block, 0, stream>>>(args_of<Finish::kSum>(p, loss), a_cols);
-  else join_kernel<T, Finish::kLinear><<<grid, block, 0, stream>>>(p, a_cols);
-  return hipGetLastError();
+  const auto run = [&](auto f) {
+    join_kernel<T, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss), a_cols);
+    return hipGetLastError();
+  };
+  if (finish == Finish::kStats) return run(FinishType<Finish::kStats>{});
+  if (finish == Finish::kExp) return run(FinishType<Finish::kExp>{});
+  if (finish == Finish::kSlope) return run(FinishType<Finish::kSlope>{});
+  if (finish == Finish::kSum) return run(FinishType<Finish::kSum>{});
+  return run(FinishType<Finish::kLinear>{});
 }
 
 void set_tiles(ProductArgs& p, int rows, int cols) {
@@ -302,8 +315,7 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
-  const int most = whole_sums(finish) ? 1 : 16;
-  if (finish != Finish::kExp && plan_narrow_product(p, dtype, a_cols, b_cols, most)) return;
+  if (finish != Finish::kExp && plan_narrow_product(p, dtype, a_cols, b_cols)) return;
   if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);
     p.slices = 1;
@@ -340,7 +352,7 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
     p.paired = c.paired;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     const int64_t at_once = c.paired ? 2 : 1;  // on a unit
-    for (int64_t s = 1; s <= most && s <= std::max<int64_t>(1, steps / 4); ++s) {
+    for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
       if (c.paired && tiles * s <= units) continue;
       const double full = std::min(1.0, static_cast<double>(tiles * s) / static_cast<double>(units));
       const double us =

@@ -99,7 +99,7 @@ std::tuple<at::Tensor, at::Tensor> loss_forward_hip(const at::Tensor& x, const a
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   const int64_t cols = x.size(-1), vocab = weight.size(0), rows = x.numel() / cols;
   const auto floats = x.options().dtype(at::kFloat);
-  at::Tensor lse = at::empty({rows}, floats);
+  at::Tensor lse = at::empty({rows, 2}, floats);
   if (rows == 0) {
     if (reduction == FH_REDUCE_NONE) return {at::empty(targets.sizes(), floats), lse};
     return {at::full({}, reduction == FH_REDUCE_MEAN ? NAN : 0.0, floats), lse};
@@ -132,8 +132,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> loss_backward_hip(const at::Tenso
   TORCH_CHECK(strided_on(grad, x) && grad.scalar_type() == at::kFloat &&
                   grad.sizes() == (reduction == FH_REDUCE_NONE ? targets.sizes() : at::IntArrayRef{}),
               "linear_cross_entropy: grad must match the result");
-  TORCH_CHECK(strided_on(lse, x) && lse.scalar_type() == at::kFloat && lse.dim() == 1 && lse.size(0) == rows &&
-                  lse.is_contiguous(),
+  TORCH_CHECK(strided_on(lse, x) && lse.scalar_type() == at::kFloat && lse.dim() == 2 && lse.size(0) == rows &&
+                  lse.size(1) == 2 && lse.is_contiguous(),
               "linear_cross_entropy: expected the forward's sums");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   const at::ScalarType bias_type = bias.has_value() ? bias->scalar_type() : x.scalar_type();

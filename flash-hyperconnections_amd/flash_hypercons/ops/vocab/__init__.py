@@ -65,7 +65,7 @@ def _linear_cross_entropy_fake(x, weight, targets, bias, ignore, reduction):
 @torch.library.register_fake("flash_hypercons::_linear_cross_entropy_forward")
 def _linear_cross_entropy_forward_fake(x, weight, targets, bias, ignore, reduction):
     loss = _linear_cross_entropy_fake(x, weight, targets, bias, ignore, reduction)
-    return loss, x.new_empty((x.numel() // x.shape[-1],), dtype=torch.float32)
+    return loss, x.new_empty((x.numel() // x.shape[-1], 2), dtype=torch.float32)
 
 
 @torch.library.register_fake("flash_hypercons::_linear_cross_entropy_backward")

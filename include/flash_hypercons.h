@@ -237,7 +237,8 @@ FH_API int fh_embedding_backward(const int64_t* tokens, const void* grad, int64_
  * 1 <= cols, vocab < 2^22.  A row whose target is `ignore` has a loss of 0 and no part in
  * anything else, whatever is in it; another target that is not in 0 .. vocab - 1 gives NaN.
  * bias ([vocab] or NULL) is of bias_dtype: dtype or FH_DTYPE_F32.  loss: a float, [rows] of
- * them for FH_REDUCE_NONE.  lse (float [rows]) is for the backward. */
+ * them for FH_REDUCE_NONE.  lse (float [rows, 2], 8-byte aligned) is
+ * for the backward. */
 FH_API int fh_linear_cross_entropy(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                             const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore, int reduction,
                             float* loss, float* lse, void* workspace, int64_t* workspace_bytes, int dtype,
