@@ -317,11 +317,15 @@ struct RowOf<Finish::kSlope> {
   int label;
   float lse, factor, hit;
   __device__ __forceinline__ void load(const LossProductArgs& p, int i) {
-    const float4 row = i < p.m ? p.loss.row[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-    label = i < p.m ? p.loss.label[i] - p.loss.col0 : 0;
-    lse = row.x;
-    factor = row.y;
-    hit = row.z;
+    label = 0;
+    lse = factor = hit = 0.f;
+    if (i < p.m) {
+      const float4 row = p.loss.row[i];
+      label = p.loss.label[i] - p.loss.col0;
+      lse = row.x;
+      factor = row.y;
+      hit = row.z;
+    }
   }
 };
 
@@ -679,7 +683,9 @@ constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16
 // floats.  `dtype` is the operands' and the output's.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
-// vectors; false for others.  Not for Finish::kExp.
+// vectors; false for others.  Not for all finishes: kExp's products have many rows, and FP32's kSlope kept a frame in
+// scratch memory (18 rows of 239 into 53413: 36 us in tiles, 32 so).
+constexpr bool narrow_finish(Finish f, bool f32) { return f != Finish::kExp && !(f32 && f == Finish::kSlope); }
 bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 // `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,

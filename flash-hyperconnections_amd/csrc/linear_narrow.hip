@@ -345,8 +345,8 @@ hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, b
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
-      if constexpr (f.value == Finish::kExp) {
-        return hipErrorInvalidValue;  // planned in tiles: those products have many rows
+      if constexpr (!narrow_finish(f.value, T::code == F32::code)) {
+        return hipErrorInvalidValue;  // planned in tiles
       } else {
         if (long_a) narrow_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
         else narrow_product_kernel<T, false, b.value, a.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));

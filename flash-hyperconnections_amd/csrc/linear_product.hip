@@ -315,7 +315,7 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
-  if (finish != Finish::kExp && plan_narrow_product(p, dtype, a_cols, b_cols)) return;
+  if (narrow_finish(finish, f32) && plan_narrow_product(p, dtype, a_cols, b_cols)) return;
   if (p.k <= (f32 ? 32 : kStep)) {
     set_tiles(p, kTile, kTile);
     p.slices = 1;
@@ -352,7 +352,9 @@ void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish fi
     p.paired = c.paired;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     const int64_t at_once = c.paired ? 2 : 1;  // on a unit
-    for (int64_t s = 1; s <= 16 && s <= std::max<int64_t>(1, steps / 4); ++s) {
+    // Up to 16 slices; a sum of the loss over a vocabulary into fewer than that many tiles up to one for each unit.
+    const int64_t most = finish == Finish::kSum ? std::max<int64_t>(16, units / tiles) : 16;
+    for (int64_t s = 1; s <= most && s <= std::max<int64_t>(1, steps / 4); ++s) {
       if (c.paired && tiles * s <= units) continue;
       const double full = std::min(1.0, static_cast<double>(tiles * s) / static_cast<double>(units));
       const double us =
