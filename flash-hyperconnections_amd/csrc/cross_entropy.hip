@@ -630,8 +630,9 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   if (err == hipSuccess) err = lay_out(a.weight, a.w_stride, a.vocab, a.cols, a.dtype, ws, w, stream);
   if (err != hipSuccess) return err;
   const int64_t groups = (a.vocab + 63) / 64, ld = (a.vocab + 7) / 8 * 8;
+  // Rows at a time: 2^18 at most, as slope_kernel's grid has a row for each 64.
   const int64_t most = std::min<int64_t>(
-      std::min<int64_t>(a.rows, most_product_rows(std::max(a.vocab, a.cols))),
+      std::min<int64_t>(std::min<int64_t>(a.rows, 1 << 18), most_product_rows(std::max(a.vocab, a.cols))),
       std::max<int64_t>(256, std::min<int64_t>(kStats / groups, kPiece / (ld * element(a.dtype))) / 256 * 256));
   auto* stats = ws.take<float2>(groups * most);
   auto* chosen = ws.take<float>(most);

@@ -383,6 +383,14 @@ def test_a_long_batch_over_many_words(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_millions_of_rows(dtype):
+    """More rows than a grid's second dimension has blocks of 64."""
+    x, w, t, b = _inputs(4_300_000, 8, 9, dtype, ignored=0.1)
+    _compare(x, w, t, b)
+
+
+@gpu
 @pytest.mark.parametrize("m", [5, 300, 1100])
 def test_a_weight_beyond_two_billion_elements(m):
     """Offsets past 2^31 elements: the loss, dx and some rows of dW against FP32 products, to FP32 and bf16 rounding."""
