@@ -18,6 +18,9 @@ typedef float Floats4 __attribute__((ext_vector_type(4)));
 // gradients; or a sum that goes on from another product's and is scaled at its end.
 enum class Finish { kLinear, kStats, kExp, kSlope, kSum };
 // Those that go by whole rows of 64 logits.
+// The narrow kernel leaves these to the join, in two slices at least: finishing them itself, it kept a frame in scratch
+// memory.
+constexpr bool joined_if_narrow(Finish f, bool f32) { return f == Finish::kSlope && f32; }
 constexpr bool of_logits(Finish f) { return f == Finish::kStats || f == Finish::kExp || f == Finish::kSlope; }
 
 // What the others need beside the product.  Their rows are the first *live ones from
@@ -683,9 +686,7 @@ constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16
 // floats.  `dtype` is the operands' and the output's.
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
-// vectors; false for others.  Not for all finishes: kExp's products have many rows, and FP32's kSlope kept a frame in
-// scratch memory (18 rows of 239 into 53413: 36 us in tiles, 32 so).
-constexpr bool narrow_finish(Finish f, bool f32) { return f != Finish::kExp && !(f32 && f == Finish::kSlope); }
+// vectors; false for others.  Not for kExp, whose products have many rows.
 bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
 // `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,

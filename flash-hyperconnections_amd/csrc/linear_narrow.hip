@@ -283,9 +283,14 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ArgsOf<F> p) {
       const int m = i / groups, n = i % groups * 8;
       float v[8];
       get(area, m, n, v);
-      RowOf<F> of;
-      of.load(p, (LongA ? first : 0) + m);
-      finish_some<T, F, groups>(p, of, slice, (LongA ? first : 0) + m, (LongA ? 0 : first) + n, v);
+      const int row = (LongA ? first : 0) + m, col = (LongA ? 0 : first) + n;
+      if constexpr (joined_if_narrow(F, f32)) {
+        keep_some(p, slice, row, col, v);
+      } else {
+        RowOf<F> of;
+        of.load(p, row);
+        finish_some<T, F, groups>(p, of, slice, row, col, v);
+      }
     }
   } else {
     const int m = threadIdx.x / groups, n = threadIdx.x % groups * 8;
@@ -300,7 +305,9 @@ __global__ __launch_bounds__(256) void narrow_product_kernel(ArgsOf<F> p) {
       for (int e = 0; e < 8; ++e) v[e] += w[e];
     }
     const int i = (LongA ? first : 0) + m, j = (LongA ? 0 : first) + n;
-    if (of_logits(F) && p.slices > 1) {
+    if constexpr (joined_if_narrow(F, f32)) {
+      keep_some(p, slice, i, j, v);
+    } else if (of_logits(F) && p.slices > 1) {
       keep_some(p, slice, i, j, v);
     } else {
       RowOf<F> of;
@@ -345,7 +352,7 @@ hipError_t launch_narrow_product(const ProductArgs& p, int dtype, bool a_cols, b
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_layout(a_cols, b_cols, finish, [&](auto a, auto b, auto f) {
-      if constexpr (!narrow_finish(f.value, T::code == F32::code)) {
+      if constexpr (f.value == Finish::kExp) {
         return hipErrorInvalidValue;  // planned in tiles
       } else {
         if (long_a) narrow_product_kernel<T, true, a.value, b.value, f.value><<<grid, block, 0, stream>>>(args_of<f.value>(p, loss));
