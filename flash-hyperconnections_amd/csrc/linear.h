@@ -687,7 +687,7 @@ constexpr int64_t kMostStride = int64_t{1} << 22;  // elements: 256 rows of a 16
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish = Finish::kLinear);
 // The same for a product with at most 32 rows or columns, and in FP32 whole aligned
 // vectors; false for others.  Not for kExp, whose products have many rows.
-bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols);
+bool plan_narrow_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish);
 // `loss` is null for Finish::kLinear.
 hipError_t launch_product(const ProductArgs& p, int dtype, bool a_cols, bool b_cols, hipStream_t stream,
                           Finish finish = Finish::kLinear, const LossParts* loss = nullptr);

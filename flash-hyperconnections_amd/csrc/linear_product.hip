@@ -314,14 +314,14 @@ void set_tiles(ProductArgs& p, int rows, int cols) {
 }  // namespace
 
 // Terms from which a narrow product that needs the join is faster than tiles.  FP32 gradients of 12 rows into 24448
-// and 122688 words: of 240 columns 76 and 164 us so, 71 and 161 in tiles; of 512 81 and 215, 85 and 236; of 3456 303
-// and 1326, 350 and 1585.
+// and 122688 words: of 240 columns 76 and 164 us so, 71 and 161 in tiles; of 512 81 and 215, 85 and 236; of 1024 104
+// and 369, 117 and 430.
 constexpr int kJoinedDepth = 384;
 
 void plan_product(ProductArgs& p, int dtype, bool a_cols, bool b_cols, Finish finish) {
   const bool f32 = dtype == F32::code;
   const bool joined = joined_if_narrow(finish, f32);
-  if (finish != Finish::kExp && !(joined && p.k < kJoinedDepth) && plan_narrow_product(p, dtype, a_cols, b_cols)) {
+  if (finish != Finish::kExp && !(joined && p.k < kJoinedDepth) && plan_narrow_product(p, dtype, a_cols, b_cols, finish)) {
     if (joined) p.slices = std::max(p.slices, 2);
     return;
   }
