@@ -456,27 +456,49 @@ __device__ __forceinline__ void add_found(const EmbeddingArgs& a, const Found& f
   }
 }
 
-// The gradient of up to 64 rows, 2^shift apart, and a strip of columns, for up to 2048 tokens: every
-// workgroup looks through them for its rows' itself, in one launch where sorting takes two more.  (The
-// frequent words of a vocabulary in the order of their frequency are neighbours: 64 rows in a row left
-// most of the work to one workgroup, 90 us.)  A wavefront to a row, all four to one that occurs often.
+// By a workgroup's 256 threads, in lines of 128 bytes.
+template <typename S>
+__device__ __forceinline__ void fill_zeros(S* to, int64_t count) {
+  constexpr int kLine = 128 / sizeof(S);
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(to) % 128 / sizeof(S));
+  const int64_t begin = (kLine - off) % kLine < count ? (kLine - off) % kLine : count;
+  const int64_t end = begin + (count - begin) / (16 / sizeof(S)) * (16 / sizeof(S));
+  const int t = static_cast<int>(threadIdx.x);
+  if (t < begin) to[t] = S{};
+  for (int64_t i = begin + t * (16 / sizeof(S)); i < end; i += 256 * (16 / sizeof(S)))
+    *reinterpret_cast<U32x4*>(to + i) = U32x4{0, 0, 0, 0};
+  if (t < count - end) to[end + t] = S{};
+}
+
+// The gradient for up to 2048 tokens, in one launch where sorting takes two more: every workgroup looks
+// through the tokens itself, adds up those of up to 64 rows, 2^shift apart, in a strip of columns, and
+// writes the zeros of up to 64 rows in a row.  (The frequent words of a vocabulary in the order of their
+// frequency are neighbours: sums of 64 rows in a row left most of the work to one workgroup, 90 us.  And
+// zeros of single rows far apart are written in part lines: FP32 735 tokens into 127539 x 450 took 81 us,
+// 164 into 25344 x 2195 71, now 49 and 44, filling as much memory alone 29 to 38.)  A wavefront to a row,
+// all four to one that occurs often; each die takes neighbouring rows.
 template <typename T>
 __global__ __launch_bounds__(256) void few_kernel(EmbeddingArgs a, int strips, int shift) {
   constexpr int V = kVec<T>;
-  __shared__ uint32_t list[4][kFew / 4], often[kRows], counts[4];
+  __shared__ uint32_t list[4][kFew / 4], often[kRows], counts[4], there[2];
   __shared__ float area[4][V][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t first = blockIdx.x / strips, apart = 1u << shift;
-  const int c = (static_cast<int>(blockIdx.x % strips) * 64 + lane) * V, cols = static_cast<int>(a.cols);
+  const uint32_t die = blockIdx.x % 8, each = gridDim.x / 8, more = gridDim.x % 8;
+  const uint32_t at = die * each + (die < more ? die : more) + blockIdx.x / 8;
+  const uint32_t first = at / strips, apart = 1u << shift;
+  const int c = (static_cast<int>(at % strips) * 64 + lane) * V, cols = static_cast<int>(a.cols);
+  const int64_t zero = a.vocab * at / gridDim.x;
+  const uint32_t zeros = static_cast<uint32_t>(a.vocab * (at + 1) / gridDim.x - zero);
   if (threadIdx.x < kRows) often[threadIdx.x] = 0;
+  if (threadIdx.x < 2) there[threadIdx.x] = 0;
   __syncthreads();
   const int begin = static_cast<int>(a.count * wave / 4), end = static_cast<int>(a.count * (wave + 1) / 4);
   constexpr int kTurns = kFew / 4 / 64;
   uint32_t keys[kTurns];
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
-    const int at = begin + 64 * i + lane;
-    keys[i] = at < end ? key_of(a, at) : static_cast<uint32_t>(a.vocab);
+    const int place = begin + 64 * i + lane;
+    keys[i] = place < end ? key_of(a, place) : static_cast<uint32_t>(a.vocab);
   }
   int count = 0;
 #pragma unroll
@@ -489,11 +511,12 @@ __global__ __launch_bounds__(256) void few_kernel(EmbeddingArgs a, int strips, i
       atomicAdd(often + row, 1u);
     }
     count += __popcll(those);
+    const uint32_t bit = keys[i] - static_cast<uint32_t>(zero);
+    if (bit < zeros) atomicOr(there + (bit >> 5), 1u << (bit & 31));
   }
   if (lane == 0) counts[wave] = count;
   __syncthreads();
   using S = typename T::storage;
-  const int rows = static_cast<int>((a.vocab - first + apart - 1) >> shift);
   const auto write = [&](int r, float (&sum)[V]) {
 #pragma unroll
     for (int k = 0; k < V; ++k) sum[k] *= a.scale;
@@ -502,12 +525,10 @@ __global__ __launch_bounds__(256) void few_kernel(EmbeddingArgs a, int strips, i
   };
   const uint32_t times = often[lane];
   const uint64_t here = __ballot(times != 0), many = __ballot(times >= kLong);
-  for (int r = wave; r < rows; r += 4) {
-    if (many >> r & 1) continue;
+  for (uint64_t left = here & ~many & 0x1111111111111111ull << wave; left != 0; left &= left - 1) {
+    const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
     float sum[V] = {};
-    if (here >> r & 1) {
-      for (int w = 0; w < 4; ++w) add_found<T>(a, {list[w], static_cast<int>(counts[w])}, r, c, sum);
-    }
+    for (int w = 0; w < 4; ++w) add_found<T>(a, {list[w], static_cast<int>(counts[w])}, r, c, sum);
     write(r, sum);
   }
   for (uint64_t left = many; left != 0; left &= left - 1) {
@@ -523,6 +544,16 @@ __global__ __launch_bounds__(256) void few_kernel(EmbeddingArgs a, int strips, i
       write(r, sum);
     }
     __syncthreads();
+  }
+  // Runs of rows that do not occur.
+  uint64_t left = ~(static_cast<uint64_t>(there[1]) << 32 | there[0]);
+  if (zeros < 64) left &= (uint64_t{1} << zeros) - 1;
+  while (left != 0) {
+    const int r = __ffsll(static_cast<unsigned long long>(left)) - 1;
+    const uint64_t rest = ~(left >> r);  // zero for 64 rows
+    const int run = rest != 0 ? __ffsll(static_cast<unsigned long long>(rest)) - 1 : 64;
+    fill_zeros(static_cast<S*>(a.out) + (zero + r) * a.cols, run * a.cols);
+    left = run + r < 64 ? left & ~uint64_t{0} << (run + r) : 0;
   }
 }
 
@@ -582,6 +613,9 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, int dtype, void* wo
   const int64_t strip = 64 * (dtype == F32::code ? 4 : 8), strips = (a.cols + strip - 1) / strip;
   int shift = 0;
   while ((int64_t{kRows} << shift) < a.vocab) ++shift;
+  // Two workgroups a compute unit, down to four rows in each: FP16 gradients of 1711 tokens of 2 x 1079 into 872 rows
+  // take 15 us, with 64 rows in each 66.
+  while ((int64_t{4} << shift) < a.vocab && (int64_t{1} << shift) * strips < 2 * compute_units()) ++shift;
   const int64_t few = std::min<int64_t>(int64_t{1} << shift, a.vocab) * strips;
   if (a.count <= kFew && few <= most_groups(256)) {
     if (bytes != nullptr) *bytes = 0;

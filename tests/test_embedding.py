@@ -176,6 +176,21 @@ def test_results_are_the_same_bits_again(tokens):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tokens,cols,vocab", [(0, 5, 300), (1, 3, 32768), (900, 7, 32768), (2048, 130, 32769),
+                                              (1711, 1079, 872), (2048, 65, 70001)])
+def test_rows_without_a_token_are_zero(tokens, cols, vocab, dtype):
+    """Whole blocks, parts and single rows of the table, whose memory held NaN before; padded ones too."""
+    t, w, g = _inputs(tokens, cols, vocab, dtype)
+    if tokens:
+        t[: tokens // 2] = torch.arange(tokens // 2, device="cuda") % vocab  # a dense block
+    for padding in (None, 0):
+        before = torch.full_like(w, float("nan"))
+        del before
+        _compare(t, w, g, padding=padding)
+
+
+@gpu
 def test_long_rows_of_a_large_table():
     """Offsets beyond 2^31 elements, in the table, the result and the gradients."""
     w = torch.empty(300000, 8192, dtype=torch.bfloat16, device="cuda")
