@@ -190,7 +190,7 @@ struct SlopeArgs {
   const float2* lse;    // lse and 1 - p of the target
   const int *live, *label;
   int row0, rows;
-  float* sums;          // [all rows / 64, ld] column sums of each 64 rows, or null
+  float* sums;          // [rows / 64, ld] column sums of each 64 rows, or null
 };
 
 // exp(z - lse) - [target] from exp(z - maximum of its 64): 64 vectors of 64 rows a workgroup, a
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
 #pragma unroll
   for (int k = 0; k < V; ++k) area[wave][k][lane] = sums[k];
   __syncthreads();
-  float* to = a.sums + (a.row0 / 64 + static_cast<int64_t>(blockIdx.y)) * a.ld + static_cast<int64_t>(blockIdx.x) * 64 * V;
+  float* to = a.sums + static_cast<int64_t>(blockIdx.y) * a.ld + static_cast<int64_t>(blockIdx.x) * 64 * V;
   for (int i = threadIdx.x; i < 64 * V && static_cast<int>(blockIdx.x) * 64 * V + i < a.ld; i += 256)
     to[i] = ((area[0][i % V][i / V] + area[1][i % V][i / V]) + area[2][i % V][i / V]) + area[3][i % V][i / V];
 }
@@ -387,6 +387,7 @@ struct BiasArgs {
   const int* live;
   int row0;
   float* partial;      // [gridDim.y, cols], or null where the sums are db already
+  float* sums;         // [cols] of the chunks so far, or null where there is one
   const float* scale;  // what db is times, or null
   void* out;
   int out_f32;         // its type: FP32, or dz's
@@ -428,22 +429,24 @@ __global__ __launch_bounds__(1024) void bias_kernel(BiasArgs a) {
   else put_bias<T>(a, to, sum);
 }
 
-// db from `count` partial sums.
+// A chunk's `count` partial sums added to those of the chunks before it; db after the last one.
 template <typename T>
-__global__ __launch_bounds__(256) void join_bias_kernel(BiasArgs a, int count) {
+__global__ __launch_bounds__(256) void join_bias_kernel(BiasArgs a, int count, bool first, bool last) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.cols) return;
-  float sum = 0.f;
+  float sum = first ? 0.f : a.sums[c];
 #pragma unroll 8
   for (int i = 0; i < count; ++i) sum += a.partial[static_cast<int64_t>(i) * a.cols + c];
-  put_bias<T>(a, c, sum);
+  if (last) put_bias<T>(a, c, sum);
+  else a.sums[c] = sum;
 }
 
-// Column sums from those of each 64 rows, as far as rows are live.
-__global__ __launch_bounds__(256) void join_rows_kernel(const float* parts, const int* live, int ld, int cols, float* out) {
-  const int c = blockIdx.x * 256 + threadIdx.x, count = (*live + 63) / 64;
+// Column sums of a chunk from those of each 64 rows, as far as rows are live, added to the chunks' before it.
+__global__ __launch_bounds__(256) void join_rows_kernel(const float* parts, const int* live, int row0, int rows, int ld,
+                                                        int cols, float* out) {
+  const int c = blockIdx.x * 256 + threadIdx.x, more = *live - row0, count = ((more < rows ? more : rows) + 63) / 64;
   if (c >= cols) return;
-  float sum = 0.f;
+  float sum = row0 == 0 ? 0.f : out[c];
 #pragma unroll 8
   for (int i = 0; i < count; ++i) sum += parts[static_cast<int64_t>(i) * ld + c];
   out[c] = sum;
@@ -461,41 +464,33 @@ dim3 blocks_of(int64_t items, int each) { return dim3(static_cast<uint32_t>((ite
 class BiasSums {
  public:
   BiasSums(bool wanted, int64_t chunks, int64_t most, int64_t cols, int dtype, Workspace& ws)
-      : dtype_(dtype), chunks_(static_cast<int>(chunks)), most_(most),
-        down_(most <= 512 ? 1 : static_cast<int>(std::min<int64_t>(most / 256, 64))) {
-    if (wanted && chunks_ * down_ > 1) partial_ = ws.take<float>(chunks * down_ * cols);
+      : dtype_(dtype), down_(most <= 512 ? 1 : static_cast<int>(std::min<int64_t>(most / 256, 64))) {
+    if (!wanted) return;
+    if (chunks * down_ > 1) partial_ = ws.take<float>(down_ * cols);
+    if (chunks > 1) sums_ = ws.take<float>(cols);
   }
-  // Adds rows row0 .. row0 + rows - 1; `args` has the output.
-  hipError_t add(BiasArgs args, const Laid& dz, int64_t row0, int64_t rows, hipStream_t stream) const {
+  // Adds `rows` rows from row0 on, the last ones or not; `args` has the output.
+  hipError_t add(BiasArgs args, const Laid& dz, int64_t row0, int64_t rows, bool last, hipStream_t stream) const {
     args.dz = dz.data;
     args.ld = dz.ld;
     args.row0 = static_cast<int>(row0);
     args.rows = static_cast<int>(rows);
-    const int64_t chunk = row0 / most_;
-    args.partial = partial_ != nullptr ? partial_ + chunk * down_ * args.cols : nullptr;
+    args.partial = partial_;
+    args.sums = sums_;
     return with_type(dtype_, [&](auto t) {
       using T = decltype(t);
       const int64_t each = 32 * kVec<T>;
       const dim3 grid(static_cast<uint32_t>((args.cols + each - 1) / each), static_cast<uint32_t>(down_));
       bias_kernel<T><<<grid, dim3(1024), 0, stream>>>(args);
-      return hipGetLastError();
-    });
-  }
-  hipError_t join(BiasArgs args, hipStream_t stream) const {
-    if (partial_ == nullptr) return hipSuccess;
-    args.partial = partial_;
-    return with_type(dtype_, [&](auto t) {
-      const dim3 grid(static_cast<uint32_t>((args.cols + 255) / 256));
-      join_bias_kernel<decltype(t)><<<grid, dim3(256), 0, stream>>>(args, chunks_ * down_);
+      if (partial_ != nullptr)
+        join_bias_kernel<T><<<blocks_of(args.cols, 256), dim3(256), 0, stream>>>(args, down_, row0 == 0, last);
       return hipGetLastError();
     });
   }
 
  private:
-  int dtype_, chunks_;
-  int64_t most_;
-  int down_;
-  float* partial_ = nullptr;
+  int dtype_, down_;
+  float *partial_ = nullptr, *sums_ = nullptr;
 };
 
 // The rows with a target and x's rows of them.
@@ -640,7 +635,7 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   auto* lse = ws.take<float2>(most);
   auto* losses = ws.take<float>(a.rows);
   const Laid dz{ws.take<char>(most * ld * element(a.dtype)), ld};
-  auto* db_parts = a.db_sums != nullptr ? ws.take<float>((a.rows + 63) / 64 * ld) : nullptr;
+  auto* db_parts = a.db_sums != nullptr ? ws.take<float>((most + 63) / 64 * ld) : nullptr;
   const int64_t before = ws.used();
   int64_t most_used = before;
   // Products follow one another on the stream, and share the space for what their slices add up to.
@@ -673,6 +668,12 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
         slope_kernel<T><<<grid, dim3(256), 0, stream>>>(s);
         return hipGetLastError();
       });
+      if (e == hipSuccess && db_parts != nullptr) {
+        join_rows_kernel<<<blocks_of(a.vocab, 256), dim3(256), 0, stream>>>(
+            db_parts, rows.live, static_cast<int>(row0), static_cast<int>(count), static_cast<int>(ld),
+            static_cast<int>(a.vocab), a.db_sums);
+        e = hipGetLastError();
+      }
     }
     LossProductArgs s{};
     s.loss.live = rows.live;
@@ -698,9 +699,6 @@ hipError_t launch_cross_entropy_ahead(const LossArgs& a, void* workspace, int64_
   });
   if (err == hipSuccess && !ws.dry()) {
     loss_kernel<<<dim3(1), dim3(1024), 0, stream>>>(losses, rows.live, a.reduction == FH_REDUCE_MEAN, a.loss);
-    if (a.db_sums != nullptr)
-      join_rows_kernel<<<blocks_of(a.vocab, 256), dim3(256), 0, stream>>>(db_parts, rows.live, static_cast<int>(ld),
-                                                                         static_cast<int>(a.vocab), a.db_sums);
     err = hipGetLastError();
   }
   if (bytes != nullptr) *bytes = most_used;
@@ -782,7 +780,7 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
       db_args.scale = r.scale;
       db_args.out = bytes_on(a.dbias, col0 * element(a.bias_dtype));
       db_args.out_f32 = a.bias_dtype == F32::code;
-      const hipError_t all = in_slices(a.rows, most_rows, [&](int64_t row0, int64_t count) {
+      return in_slices(a.rows, most_rows, [&](int64_t row0, int64_t count) {
         const Laid xp = rows_from(rows.x, row0, a.dtype);
         hipError_t e = shared([&](Workspace& part) {
           LossProductArgs p = logits(a, rows, row0, count, col0, outs);
@@ -824,10 +822,10 @@ hipError_t launch_cross_entropy_backward(const LossArgs& a, void* workspace, int
             return multiply(p, d, parts == 2 ? rows.twice : xp, a.dtype, true, true, Finish::kSum, part, stream);
           });
         }
-        if (e == hipSuccess && a.dbias != nullptr && !ws.dry()) e = db.add(db_args, d, row0, parts * count, stream);
+        if (e == hipSuccess && a.dbias != nullptr && !ws.dry())
+          e = db.add(db_args, d, row0, parts * count, row0 + count == a.rows, stream);
         return e;
       });
-      return all != hipSuccess || a.dbias == nullptr || ws.dry() ? all : db.join(db_args, stream);
     });
   }
   if (err == hipSuccess && a.dx != nullptr && parts == 2 && !ws.dry()) {
