@@ -11,7 +11,7 @@ Everything else -- CPU tensors, other types, tensor subclasses, function transfo
 or words -- is composed from native PyTorch operations, float16 and bfloat16 in float32; a backward that
 builds a graph takes differentiable native pieces.
 
-An index that is out of range raises on the CPU.  The kernels do not wait to find out: such a token's
+An index that is out of range raises on the CPU.  On the GPU nothing waits to find out: such a token's
 row, or such a target's loss, is NaN, and so are the gradients that the loss reaches; the embedding's
 gradient leaves such a token out.
 """
@@ -45,6 +45,13 @@ def _eligible(indices: torch.Tensor, *operands: Optional[torch.Tensor]) -> bool:
         and not torch._C._are_functorch_transforms_active()
         and _device_supported(indices.device.index)
     )
+
+
+def _in_range(indices: torch.Tensor, count: int) -> torch.Tensor:
+    """Which indices on the GPU are in 0 .. count - 1: PyTorch reads memory at the others without a check."""
+    if count == 0 and indices.numel():
+        raise IndexError("no index is in the range of a table with no rows")
+    return (indices >= 0) & (indices < count)
 
 
 @torch.library.register_fake("flash_hypercons::_embedding")
@@ -124,7 +131,12 @@ def embedding(
         and (streams or 1) < _STREAMS
     ):
         return _EMBEDDING(tokens, weight, scale, streams or 0, -1 if padding_idx is None else padding_idx)
-    y = torch.nn.functional.embedding(tokens, _wide(weight), padding_idx) * scale
+    if tokens.device.type == "cuda":
+        valid = _in_range(tokens, vocab)
+        y = torch.nn.functional.embedding(torch.where(valid, tokens, 0), _wide(weight), padding_idx) * scale
+        y = torch.where(valid.unsqueeze(-1), y, float("nan"))
+    else:
+        y = torch.nn.functional.embedding(tokens, _wide(weight), padding_idx) * scale
     if streams is not None:
         y = y.unsqueeze(-2).expand(*tokens.shape, streams, cols)
     return y.to(weight.dtype).contiguous()
@@ -165,10 +177,19 @@ def linear_cross_entropy(
         raise ValueError(f"linear_cross_entropy: expected targets of shape {tuple(x.shape[:-1])}, got {tuple(targets.shape)}")
     rows = _wide(x).reshape(-1, x.shape[-1])
     flat = targets.reshape(-1).long()
+    here = flat != ignore_index
     # What a position without a target holds takes no part, a NaN among it.
-    rows = torch.where((flat != ignore_index).unsqueeze(1), rows, rows.new_zeros(()))
+    rows = torch.where(here.unsqueeze(1), rows, rows.new_zeros(()))
     z = torch.nn.functional.linear(rows, _wide(weight), _wide(bias))
-    loss = torch.nn.functional.cross_entropy(z, flat, ignore_index=ignore_index, reduction=reduction)
+    if flat.device.type == "cuda":
+        valid = _in_range(flat, weight.shape[0])
+        z = z + torch.where(here & ~valid, float("nan"), 0.0).to(z.dtype).unsqueeze(1)  # so are its gradients
+        loss = torch.nn.functional.cross_entropy(z, torch.where(valid, flat, 0), reduction="none")
+        loss = torch.where(here, loss, 0.0)
+        if reduction != "none":
+            loss = loss.sum() / (here.sum() if reduction == "mean" else 1)
+    else:
+        loss = torch.nn.functional.cross_entropy(z, flat, ignore_index=ignore_index, reduction=reduction)
     return loss.reshape(targets.shape) if reduction == "none" else loss
 
 
