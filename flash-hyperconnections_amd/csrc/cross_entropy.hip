@@ -26,8 +26,9 @@
 // the exponentials), dx 13.4, dW 14.6, slope_kernel 1.6, scale_kernel 0.66; forming the logits again it took 56.4.
 // One row of it, the forward alone, 180 us: the weight at 6.0 TB/s.
 //
-// dz is rounded to the operands' type, as the products' operands have to be; that of up to 128 rows
-// comes in two parts of 16 bits, as if it were twice as many rows.  In FP16 dz is held times a
+// dz is rounded to the operands' type, as the products' operands have to be; that of batches of up to
+// 128 rows comes in two parts of 16 bits, as if it were twice as many rows (a larger batch of which few
+// rows have a target keeps one part).  In FP16 dz is held times a
 // power of two that puts the largest |f_i| between 2^14 and 2^15: probabilities down to 2^-39 of
 // the largest factor stay above zero then.  The results' last step divides by it, exactly.  The
 // other types have the range without.

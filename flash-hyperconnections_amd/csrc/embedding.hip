@@ -171,7 +171,8 @@ __global__ __launch_bounds__(kThreads) void sort_tile_kernel(EmbeddingArgs a, in
 
 // Several tiles, a count and a move for each digit.  Tiles of 1024 keys while there are at most 64 of them, as each
 // workgroup adds up the counts of all: 16384 tokens sort in 20 us, 131072, in 32 tiles of 4096, in 36 (in tiles
-// of 16384, on eight compute units, 92), 600000, in tiles of 16384, in 95.
+// of 16384, on eight compute units, 92), 600000, in tiles of 16384, in 95.  That addition goes by the square of the
+// tiles: 2^22 tokens take 0.23 ms in two passes, 2^24 1.1, 2^26 8.8 and 2^27 27.
 constexpr int kDigit = 9;  // bits of a pass
 
 // keys null: the tokens themselves.

@@ -17,10 +17,10 @@ typedef float Floats4 __attribute__((ext_vector_type(4)));
 // statistics of logits, which are not kept; these and the logits' exponentials; the logits'
 // gradients; or a sum that goes on from another product's and is scaled at its end.
 enum class Finish { kLinear, kStats, kExp, kSlope, kSum };
-// Those that go by whole rows of 64 logits.
 // The narrow kernel leaves these to the join, in two slices at least: finishing them itself, it kept a frame in scratch
 // memory.
 constexpr bool joined_if_narrow(Finish f, bool f32) { return f == Finish::kSlope && f32; }
+// Those that go by whole rows of 64 logits.
 constexpr bool of_logits(Finish f) { return f == Finish::kStats || f == Finish::kExp || f == Finish::kSlope; }
 
 // What the others need beside the product.  Their rows are the first *live ones from

@@ -159,8 +159,12 @@ def linear_cross_entropy(
     backward forms the logits again.  Losses are float32 (float64 for float64 operands): of each position for
     reduction "none", else their "sum", or their "mean" over the positions with a target (NaN where there
     is none).  A position whose target is `ignore_index` has a loss and gradients of zero, whatever x holds
-    there, and costs next to nothing.  Differentiable in x, weight and bias; the logits' gradients are
-    rounded to x's type before they are multiplied.
+    there, and costs next to nothing.  Differentiable in x, weight and bias.
+
+    What 16 bits cost beside float32 products rounded once: exponentials come from the hardware's exp2; where
+    gradients are formed with the loss they wait for their row's sum in float16, 11 bits each; and the
+    logits' gradients are rounded to x's type before they are multiplied, with batches of up to 128 positions
+    to twice its digits.  The batch's size decides, not how many positions have a target.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}; one of {', '.join(map(repr, _REDUCTIONS))}")

@@ -233,8 +233,9 @@ FH_API int fh_embedding_backward(const int64_t* tokens, const void* grad, int64_
 #define FH_REDUCE_MEAN 2
 
 /* loss[i] = log(sum over v of exp(z[i, v])) - z[i, targets[i]], z = x weight^T + bias for x
- * [rows, cols] and weight [vocab, cols], in FP32 and without keeping z; 0 <= rows < 2^24,
- * 1 <= cols, vocab < 2^22.  A row whose target is `ignore` has a loss of 0 and no part in
+ * [rows, cols] and weight [vocab, cols], in FP32 and without keeping z; 1 <= rows < 2^24,
+ * 1 <= cols, vocab < 2^22 (no rows are refused, here and below: their results are the
+ * caller's to fill in).  A row whose target is `ignore` has a loss of 0 and no part in
  * anything else, whatever is in it; another target that is not in 0 .. vocab - 1 gives NaN.
  * bias ([vocab] or NULL) is of bias_dtype: dtype or FH_DTYPE_F32.  loss: a float, [rows] of
  * them for FH_REDUCE_NONE.  lse (float [rows, 2], 8-byte aligned) is
@@ -257,7 +258,8 @@ FH_API int fh_linear_cross_entropy_backward(const void* x, int64_t x_stride, con
  * upstream gradient, which is one number: with a product fewer than the two calls above make of
  * the logits, for FP32 sums in their place.  places (int [1 + rows]) receives how many rows
  * have a target and which; dx_sums (float [rows, cols]), dw_sums (float [vocab, cols]) and
- * db_sums (float [vocab]) may each be NULL. */
+ * db_sums (float [vocab]) may each be NULL.  With 16-bit operands a row's exponentials wait in
+ * FP16 for its sum. */
 FH_API int fh_linear_cross_entropy_ahead(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                                   const void* bias, int bias_dtype, const int64_t* targets, int64_t ignore,
                                   int reduction, float* loss, int* places, float* dx_sums, float* dw_sums,
