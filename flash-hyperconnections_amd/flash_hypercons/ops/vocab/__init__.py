@@ -184,10 +184,13 @@ def linear_cross_entropy(
     here = flat != ignore_index
     # What a position without a target holds takes no part, a NaN among it.
     rows = torch.where(here.unsqueeze(1), rows, rows.new_zeros(()))
-    z = torch.nn.functional.linear(rows, _wide(weight), _wide(bias))
+    valid = None
     if flat.device.type == "cuda":
         valid = _in_range(flat, weight.shape[0])
-        z = z + torch.where(here & ~valid, float("nan"), 0.0).to(z.dtype).unsqueeze(1)  # so are its gradients
+        # The row's logits are NaN then, and its gradients too.
+        rows = rows + torch.where(here & ~valid, float("nan"), 0.0).to(rows.dtype).unsqueeze(1)
+    z = torch.nn.functional.linear(rows, _wide(weight), _wide(bias))
+    if valid is not None:
         loss = torch.nn.functional.cross_entropy(z, torch.where(valid, flat, 0), reduction="none")
         loss = torch.where(here, loss, 0.0)
         if reduction != "none":
